@@ -33,7 +33,7 @@ extern "C" {
 #define SFFFT_ERR_NO_MATCH 6
 #define SFFFT_ERR_ALLOC 7
 #define SFFFT_ERR_SCRATCH_LIMIT 8 /* problem too large for sffft_conv_noalloc's fixed scratch */
-#define SFFFT_ERR_WORKSPACE 9     /* composite plan called without a large enough workspace */
+#define SFFFT_ERR_WORKSPACE 9     /* the call needs a larger workspace (composite plans, linear attention, norms' backward) */
 
 #define SFFFT_IO_FP32 0
 #define SFFFT_IO_BF16 1
@@ -210,6 +210,109 @@ typedef struct sffft_multi* sffft_multi_t;
 int sffft_multi_pipe_create(sffft_multi_t* multi, const sffft_plan_t* plans, int G, int B, int H, int chunks);
 int sffft_conv_host_multi(sffft_multi_t multi, const void* u_host, const void* const* Kf, void* y_host);
 int sffft_multi_pipe_destroy(sffft_multi_t multi);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no reference counterpart): the causal mixer whose filter depends on
+ * the data.  For a head with decay lambda = exp(log_decay), lambda in [0, 1], and state S [D][Dv] in fp32,
+ *
+ *   S_n = lambda S_{n-1} + k_n v_n^T,     y_n = scale * S_n^T q_n,        n = 1 .. length
+ *
+ * i.e. y_n = scale * (sum_{m<=n} lambda^(n-m) (q_n . k_m) v_m + lambda^n S_0^T q_n): with D = Dv = 1 and q = k = 1 it
+ * is sffft_conv with the filter lambda^n.
+ *
+ *   q, y [B][H][L][D or Dv], k [B][Hkv][L][D], v [B][Hkv][L][Dv]   of type io; a position's D (Dv) values are
+ *        contiguous, the other axes have the element strides {row, head, position} of the descriptor, so that
+ *        [B][L][H][D] buffers and parts of a fused projection work as they are.  Query head h uses key and value head
+ *        h / (H / Hkv).
+ *   log_decay [H] fp32, <= 0 (-inf: no memory); a constant of the model, not trained.
+ *   lengths [B] int32 on the device, or NULL: tokens of each row (clamped to 0 .. L).  What q, k and v hold behind a
+ *        row's last token is not used, not even where it is NaN; y there is set to zero.
+ *   initial_state, final_state [B][H][D][Dv] fp32 contiguous; NULL: zero, not wanted.
+ *
+ * D up to 256 and Dv up to 4096 (backward: 256), any L; other sizes return SFFFT_ERR_UNSUPPORTED.  A value of q, k or v
+ * that is not finite may reach all outputs of its row and head.  Outputs must not overlap inputs.  `work`: caller-owned
+ * device memory of sffft_linear_attention_workspace_bytes (256-byte aligned), not shared by calls that can overlap.
+ * Calls run on `device` in stream order and can be captured in graphs; the caller's current device is left as it was.
+ * Results do not depend on scheduling: no atomics. */
+typedef struct {
+  int B, H, Hkv, L, D, Dv;
+  int io;                 /* SFFFT_IO_* of q, k, v, y and their gradients */
+  int device;
+  float scale;            /* finite, not 0 */
+  long long q_stride[3], k_stride[3], v_stride[3], y_stride[3];
+} sffft_linear_attention_t;
+int sffft_linear_attention_workspace_bytes(const sffft_linear_attention_t* p, int backward, size_t* bytes);
+int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, const void* k, const void* v,
+                           const float* log_decay, const int* lengths, const float* initial_state, void* y,
+                           float* final_state, void* work, size_t work_bytes, void* stream);
+
+/* Gradients of q, k, v and the initial state from those of y and of the final state (dfinal_state NULL: zero;
+ * dinitial_state NULL: not wanted).  dk and dv of a shared head are summed over its query heads in fp32.  Gradients
+ * behind a row's last token are zero.  y_stride of the descriptor is not used. */
+typedef struct {
+  long long dy_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} sffft_linear_attention_grads_t;
+int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sffft_linear_attention_grads_t* g,
+                                    const void* q, const void* k, const void* v, const float* log_decay,
+                                    const int* lengths, const float* initial_state, const void* dy,
+                                    const float* dfinal_state, void* dq, void* dk, void* dv, float* dinitial_state,
+                                    void* work, size_t work_bytes, void* stream);
+
+/* One token for each of B rows: S <- lambda S + k v^T in place, y = scale * S^T q.  The states lie in a pool of slots
+ * of [H][D][Dv] fp32, state_stride elements apart; row b uses slot slots[b] (int32, device), or slot b where slots is
+ * NULL.  A row whose slot is not in [0, pool) is padding: it gets y = 0 and no state changes.  The same holds for a row
+ * that names a slot which an earlier row of the call names.  Strides are {row, head}. */
+typedef struct {
+  int B, H, Hkv, D, Dv, pool;
+  int io, device;
+  float scale;
+  long long q_stride[2], k_stride[2], v_stride[2], y_stride[2], state_stride;
+} sffft_linear_attention_step_t;
+int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const void* q, const void* k, const void* v,
+                                const float* log_decay, float* state, const int* slots, void* y, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * The joint between two blocks (no reference counterpart): the norm behind a block, its gate and residual scale, the
+ * residual stream, and the norm before the next block, in one pass.  On each row of `channels` values
+ *
+ *   a = y * rstd_g(y) * post_weight     (a = y where post_weight is NULL; rstd over each of `groups` runs of channels)
+ *   h = x + scale * act(gate) * a       (without x where it is NULL; without the gate where gate is NULL)
+ *   n = h * rstd(h) * weight            (not computed where weight is NULL)
+ *
+ * with rstd(z) = (mean(z^2) + eps)^(-1/2).  y NULL: h = x (not written), n alone.
+ *
+ *   inner = 0: x, y and gate are rows of contiguous channels, x_stride (..) elements apart; h and n are contiguous
+ *   inner > 0: all tensors are [rows / inner][channels][inner] contiguous, the layout of sffft_conv's u and y
+ *   gate: SFFFT_GATE_NONE, _FULL (shaped like y) or _CHANNEL ([channels])
+ *   y, gate and n are of type io, x and h of type res_io (io, or fp32 beside bf16), the weights [channels] of weight_io
+ *   rstd_post [rows][groups] and rstd [rows] fp32: written for the backward pass, NULL: not wanted
+ *
+ * Up to 8192 channels (and 256 groups with inner > 0).  h may be x's and n y's own buffer where the strides agree and inner = 0. */
+#define SFFFT_GATE_NONE 0
+#define SFFFT_GATE_FULL 1
+#define SFFFT_GATE_CHANNEL 2
+#define SFFFT_ACT_NONE 0
+#define SFFFT_ACT_SILU 1
+#define SFFFT_ACT_SIGMOID 2
+typedef struct {
+  long long rows;
+  int channels, inner, groups;
+  int io, res_io, weight_io;
+  int gate, act;
+  float scale, eps;
+  int device;
+  long long x_stride, y_stride, gate_stride;
+} sffft_block_norm_t;
+int sffft_block_norm(const sffft_block_norm_t* p, const void* x, const void* y, const void* gate, const void* post_weight,
+                     const void* weight, void* h, void* n, float* rstd_post, float* rstd, void* stream);
+/* Gradients from dh (NULL: zero) and dn, which are laid out like h and n, and the forward pass's rstd_post and rstd.
+ * dx, dy and a full dgate are contiguous in the same layout; dpost_weight, dweight and a channel's dgate are summed
+ * over the rows in fp32 and a fixed order.  work: sffft_block_norm_workspace_bytes, 256-byte aligned. */
+int sffft_block_norm_workspace_bytes(const sffft_block_norm_t* p, size_t* bytes);
+int sffft_block_norm_backward(const sffft_block_norm_t* p, const void* x, const void* y, const void* gate,
+                              const void* post_weight, const void* weight, const float* rstd_post, const float* rstd,
+                              const void* dh, const void* dn, void* dx, void* dy, void* dgate, void* dpost_weight,
+                              void* dweight, void* work, size_t work_bytes, void* stream);
 
 /* Debug: a kernel waits on a barrier that nothing arrives at, using the same bounded wait as the fused
  * kernel; returns SFFFT_ERR_TIMEOUT after about limit_us microseconds (1..1e6) with the context intact.

@@ -25,6 +25,8 @@ IO = {"fp32": 0, "bf16": 1}
 ACC = {"fp32": 0, "fp16": 1}
 KERNEL = {"legacy": 0, "cached": 1}
 FILTER = {"causal": 0, "two_sided": 1, "circular": 2}
+GATE = {"none": 0, "full": 1, "channel": 2}
+ACT = {"none": 0, "silu": 1, "sigmoid": 2}
 
 _lib = None
 _emu = None
@@ -40,6 +42,32 @@ class PlanInfo(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in (
         "L", "N", "stages", "R0", "R1", "R2", "pairs_per_cta", "warps", "threads", "smem_bytes",
         "tmem_cols", "occupancy", "io", "acc", "kernel_mode", "device", "blocks")] + [("config", ctypes.c_char * 96)]
+
+
+class LinearAttentionDesc(ctypes.Structure):
+    """sffft_linear_attention_t"""
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "H", "Hkv", "L", "D", "Dv", "io", "device")] + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_longlong * 3) for n in ("q_stride", "k_stride", "v_stride", "y_stride")])
+
+
+class LinearAttentionGrads(ctypes.Structure):
+    """sffft_linear_attention_grads_t"""
+    _fields_ = [(n, ctypes.c_longlong * 3) for n in ("dy_stride", "dq_stride", "dk_stride", "dv_stride")]
+
+
+class LinearAttentionStepDesc(ctypes.Structure):
+    """sffft_linear_attention_step_t"""
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "H", "Hkv", "D", "Dv", "pool", "io", "device")] + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_longlong * 2) for n in ("q_stride", "k_stride", "v_stride", "y_stride")]
+                + [("state_stride", ctypes.c_longlong)])
+
+
+class BlockNormDesc(ctypes.Structure):
+    """sffft_block_norm_t"""
+    _fields_ = ([("rows", ctypes.c_longlong)]
+                + [(n, ctypes.c_int) for n in ("channels", "inner", "groups", "io", "res_io", "weight_io", "gate", "act")]
+                + [("scale", ctypes.c_float), ("eps", ctypes.c_float), ("device", ctypes.c_int)]
+                + [(n, ctypes.c_longlong) for n in ("x_stride", "y_stride", "gate_stride")])
 
 
 class _Candidate(ctypes.Structure):
@@ -86,6 +114,13 @@ def _declare(lib):
         "sffft_multi_pipe_create": (I, [ctypes.POINTER(P), ctypes.POINTER(P), I, I, I, I]),
         "sffft_conv_host_multi": (I, [P, V, ctypes.POINTER(V), V]),
         "sffft_multi_pipe_destroy": (I, [P]),
+        "sffft_linear_attention_workspace_bytes": (I, [V, I, ctypes.POINTER(ctypes.c_size_t)]),
+        "sffft_linear_attention": (I, [V] * 10 + [ctypes.c_size_t, V]),
+        "sffft_linear_attention_backward": (I, [V] * 15 + [ctypes.c_size_t, V]),
+        "sffft_linear_attention_step": (I, [V] * 9),
+        "sffft_block_norm": (I, [V] * 11),
+        "sffft_block_norm_workspace_bytes": (I, [V, ctypes.POINTER(ctypes.c_size_t)]),
+        "sffft_block_norm_backward": (I, [V] * 16 + [ctypes.c_size_t, V]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -472,3 +507,333 @@ def emu_conv(config: str, u, Kf, io: str = "fp32", acc: str = "fp32"):
     if rc:
         raise ValueError(f"unknown config {config}")
     return y
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Linear attention with a decay for each head, and the norms that join a block to the residual stream
+# ---------------------------------------------------------------------------------------------------------------
+
+def _io_of(t, what):
+    import torch
+    if t.dtype == torch.float32:
+        return 0
+    if t.dtype == torch.bfloat16:
+        return 1
+    raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}")
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _call_stream(stream, device):
+    """(raw stream, torch stream) of a call: the given one, or the device's current stream."""
+    import torch
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream, None
+    if isinstance(stream, int):
+        return stream, torch.cuda.ExternalStream(stream, device=device)
+    return stream.cuda_stream, stream
+
+
+def _used_on(stream, *tensors):
+    """Tells the allocator that buffers this call made are in use on a stream other than the current one."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def _heads_like(like, B, H, L, D, dtype):
+    """An empty [B][H][L][D] tensor whose memory is ordered like `like`'s: [B][L][H][D] where its positions are outermost."""
+    import torch
+    if like.stride(2) > like.stride(1) and H > 1:
+        return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=dtype, device=like.device)
+    return torch.empty((B, H, L, D), dtype=dtype, device=like.device)
+
+
+def _unit(t):
+    """The tensor with contiguous last axis (a copy where it is not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, final_grad=None):
+    """Raises ValueError where the arguments of linear_attention do not fit each other."""
+    import math
+
+    import torch
+    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k and v must be [B][H][L][D], [B][Hkv][L][D] and [B][Hkv][L][Dv]")
+    B, H, L, D = q.shape
+    Hkv, Dv = k.shape[1], v.shape[3]
+    _need(tuple(k.shape) == (B, Hkv, L, D) and tuple(v.shape) == (B, Hkv, L, Dv),
+          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    _need(H > 0 and Hkv > 0 and H % Hkv == 0, f"{H} query heads cannot share {Hkv} key and value heads evenly")
+    _need(D > 0 and Dv > 0, "head sizes must be positive")
+    _io_of(q, "q")
+    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type")
+    _need(tuple(log_decay.shape) == (H,) and log_decay.dtype == torch.float32, f"log_decay must be a float32 [{H}] tensor")
+    _need(not log_decay.requires_grad, "log_decay is a constant: it has no gradient (pass log_decay.detach())")
+    _need(math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
+    state = (B, H, D, Dv)
+    for t, what in ((initial_state, "initial_state"), (final_grad, "the final state's gradient")):
+        _need(t is None or (tuple(t.shape) == state and t.dtype == torch.float32), f"{what} must be a float32 {list(state)} tensor")
+    _need(lengths is None or (tuple(lengths.shape) == (B,) and lengths.dtype == torch.int32), f"lengths must be an int32 [{B}] tensor")
+    for t in (k, v, log_decay, initial_state, lengths):
+        _need(t is None or t.device == q.device, "all tensors must be on one device")
+
+
+def _la_desc(q, k, v, scale, y_stride):
+    B, H, L, D = q.shape
+    d = LinearAttentionDesc(B, H, k.shape[1], L, D, v.shape[3], _io_of(q, "q"), q.device.index, scale)
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    d.y_stride[:] = y_stride
+    return d
+
+
+def _la_workspace(desc, backward, device):
+    import torch
+    need = ctypes.c_size_t()
+    _check(lib().sffft_linear_attention_workspace_bytes(ctypes.byref(desc), int(backward), ctypes.byref(need)),
+           "linear_attention_workspace_bytes")
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def linear_attention(q, k, v, log_decay, scale=1.0, initial_state=None, lengths=None, stream=None):
+    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n with lambda = exp(log_decay) for each head.
+
+    q [B][H][L][D], k [B][Hkv][L][D], v [B][Hkv][L][Dv], float32 or bfloat16; log_decay [H] float32, <= 0;
+    initial_state and final_state [B][H][D][Dv] float32; lengths [B] int32: tokens of each row (default L).  y has
+    q's type and order of axes, and is zero behind a row's last token.  Runs on `stream` (default: the current one)."""
+    import torch
+    check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+    _need(q.device.type == "cuda", "linear_attention needs CUDA tensors (there is no CPU path)")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    B, H, L, D = q.shape
+    Dv = v.shape[3]
+    raw, side = _call_stream(stream, q.device)
+    y = _heads_like(q, B, H, L, Dv, q.dtype)
+    s1 = torch.empty((B, H, D, Dv), dtype=torch.float32, device=q.device)
+    desc = _la_desc(q, k, v, scale, y.stride()[:3])
+    work = _la_workspace(desc, False, q.device)
+    ld = log_decay.contiguous()
+    s0 = None if initial_state is None else initial_state.contiguous()
+    ln = None if lengths is None else lengths.contiguous()
+    _check(lib().sffft_linear_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(), _ptr(ln),
+                                        _ptr(s0), y.data_ptr(), s1.data_ptr(), _ptr(work), 0 if work is None else work.numel(),
+                                        raw), f"linear_attention(q {list(q.shape)}, v {list(v.shape)})")
+    _used_on(side, q, k, v, ld, s0, ln, y, s1, work)
+    return y, s1
+
+
+def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1.0, initial_state=None, lengths=None,
+                              stream=None):
+    """(dq, dk, dv, dinitial_state) of linear_attention; dinitial_state is None where there was no initial state."""
+    import torch
+    check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, dfinal_state)
+    _need(q.device.type == "cuda", "linear_attention_backward needs CUDA tensors (there is no CPU path)")
+    B, H, L, D = q.shape
+    Hkv, Dv = k.shape[1], v.shape[3]
+    _need(tuple(dy.shape) == (B, H, L, Dv) and dy.dtype == q.dtype and dy.device == q.device,
+          f"dy must be a {q.dtype} {[B, H, L, Dv]} tensor on q's device")
+    _need(dfinal_state is None or dfinal_state.device == q.device, "all tensors must be on one device")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    dy = dy if dy.stride(-1) == 1 and 0 not in dy.stride() else dy.contiguous()   # a sum's gradient comes expanded
+    raw, side = _call_stream(stream, q.device)
+    dq, dk, dv = _heads_like(q, B, H, L, D, q.dtype), _heads_like(k, B, Hkv, L, D, q.dtype), _heads_like(v, B, Hkv, L, Dv, q.dtype)
+    ds0 = None if initial_state is None else torch.empty((B, H, D, Dv), dtype=torch.float32, device=q.device)
+    desc = _la_desc(q, k, v, scale, (0, 0, 0))
+    grads = LinearAttentionGrads()
+    grads.dy_stride[:], grads.dq_stride[:], grads.dk_stride[:], grads.dv_stride[:] = (t.stride()[:3] for t in (dy, dq, dk, dv))
+    work = _la_workspace(desc, True, q.device)
+    ld = log_decay.contiguous()
+    s0 = None if initial_state is None else initial_state.contiguous()
+    ds1 = None if dfinal_state is None else dfinal_state.contiguous()
+    ln = None if lengths is None else lengths.contiguous()
+    _check(lib().sffft_linear_attention_backward(
+        ctypes.byref(desc), ctypes.byref(grads), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(), _ptr(ln), _ptr(s0),
+        dy.data_ptr(), _ptr(ds1), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ds0), _ptr(work),
+        0 if work is None else work.numel(), raw), f"linear_attention_backward(q {list(q.shape)}, v {list(v.shape)})")
+    _used_on(side, q, k, v, ld, s0, ln, dy, ds1, dq, dk, dv, ds0, work)
+    return dq, dk, dv, ds0
+
+
+def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=1.0, stream=None):
+    """One token for each row: state[slot] <- lambda state[slot] + k v^T in place, y = scale state[slot]^T q.
+
+    q [B][H][D], k [B][Hkv][D], v [B][Hkv][Dv]; state [pool][H][D][Dv] float32, of which only the slots' axis may have a
+    stride of its own; slots [B] int32 (default: row b uses slot b).  A slot outside the pool marks a padded row, whose
+    y is zero; so does a slot that an earlier row of the call has."""
+    import math
+
+    import torch
+    _need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be [B][H][D], [B][Hkv][D] and [B][Hkv][Dv]")
+    B, H, D = q.shape
+    Hkv, Dv = k.shape[1], v.shape[2]
+    _need(tuple(k.shape) == (B, Hkv, D) and tuple(v.shape) == (B, Hkv, Dv),
+          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    _need(H > 0 and Hkv > 0 and H % Hkv == 0, f"{H} query heads cannot share {Hkv} key and value heads evenly")
+    _need(D > 0 and Dv > 0, "head sizes must be positive")
+    io = _io_of(q, "q")
+    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type")
+    _need(tuple(log_decay.shape) == (H,) and log_decay.dtype == torch.float32, f"log_decay must be a float32 [{H}] tensor")
+    _need(math.isfinite(scale), "scale must be finite")
+    _need(state.dim() == 4 and tuple(state.shape[1:]) == (H, D, Dv) and state.dtype == torch.float32,
+          f"state must be a float32 [pool, {H}, {D}, {Dv}] tensor")
+    _need(state.stride()[1:] == (D * Dv, Dv, 1) and (state.stride(0) >= H * D * Dv or state.shape[0] <= 1),
+          "a slot's state must be contiguous and slots must not overlap")
+    _need(slots is None or (tuple(slots.shape) == (B,) and slots.dtype == torch.int32), f"slots must be an int32 [{B}] tensor")
+    _need(slots is not None or state.shape[0] >= B, f"{B} rows need {B} slots")
+    for t in (k, v, log_decay, state, slots):
+        _need(t is None or t.device == q.device, "all tensors must be on one device")
+    _need(q.device.type == "cuda", "linear_attention_step needs CUDA tensors (there is no CPU path)")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    raw, side = _call_stream(stream, q.device)
+    y = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
+    d = LinearAttentionStepDesc(B, H, Hkv, D, Dv, state.shape[0], io, q.device.index, scale)
+    d.q_stride[:], d.k_stride[:], d.v_stride[:], d.y_stride[:] = (t.stride()[:2] for t in (q, k, v, y))
+    d.state_stride = state.stride(0)
+    ld = log_decay.contiguous()
+    sl = None if slots is None else slots.contiguous()
+    _check(lib().sffft_linear_attention_step(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(),
+                                             state.data_ptr(), _ptr(sl), y.data_ptr(), raw),
+           f"linear_attention_step(q {list(q.shape)}, v {list(v.shape)})")
+    _used_on(side, q, k, v, ld, sl, state, y)
+    return y
+
+
+def check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
+    """(channels, kind of gate) of a block_norm call; raises ValueError where its arguments do not fit each other."""
+    import math
+
+    import torch
+    lead = y if y is not None else x
+    _need(lead is not None, "block_norm needs x or y")
+    _need(dim in (-1, 1, lead.dim() - 1), "dim must be -1, or 1 for [B][C][L] tensors")
+    first = dim == 1 and lead.dim() != 2
+    _need(not first or lead.dim() == 3, "dim 1 is for [B][C][L] tensors")
+    _need(lead.dim() >= 1 and lead.shape[dim] > 0, "there must be channels")
+    C = lead.shape[dim]
+    if y is None:
+        _need(gate is None and post_weight is None, "a gate and post_weight act on y")
+        _need(weight is not None, "without y there must be a weight to norm x with")
+    io = _io_of(lead, "x" if y is None else "y")
+    if x is not None and y is not None:
+        _need(x.shape == y.shape, f"x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
+        _need(x.dtype == y.dtype or (x.dtype == torch.float32 and io == 1), "x must have y's type, or be float32 beside bfloat16")
+    kind = "none"
+    if gate is not None:
+        kind = "full" if gate.shape == y.shape and gate.dim() > 1 or (gate.dim() == 1 and y.dim() == 1) else "channel"
+        _need(kind == "full" or tuple(gate.shape) == (C,), f"gate must be shaped like y or [{C}]")
+        _need(gate.dtype == y.dtype, "gate must have y's type")
+    for w, what in ((post_weight, "post_weight"), (weight, "weight")):
+        if w is not None:
+            _need(tuple(w.shape) == (C,), f"{what} must be [{C}]")
+            _io_of(w, what)
+    _need(post_weight is None or weight is None or post_weight.dtype == weight.dtype, "the weights must have one type")
+    _need(groups >= 1 and C % groups == 0, f"{C} channels do not fall into {groups} groups")
+    _need(groups == 1 or post_weight is not None, "groups are those of the norm with post_weight")
+    _need(act in ACT, f"act must be one of {sorted(ACT)}")
+    _need(math.isfinite(scale), "scale must be finite")
+    _need(math.isfinite(eps) and eps >= 0, "eps must be finite and not negative")
+    for t in (x, gate, post_weight, weight):
+        _need(t is None or t.device == lead.device, "all tensors must be on one device")
+    return C, kind, first
+
+
+def _as_rows(t, C):
+    """(tensor, stride of a row) of a [..., C] tensor whose rows are evenly spaced (a copy where they are not)."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    step, rows = None, 1
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step = s
+        elif s != step * rows:
+            t = t.contiguous()
+            return t, C
+        rows *= n
+    return t, C if step is None else step
+
+
+def _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
+    C, kind, first = check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    lead = y if y is not None else x
+    _need(lead.device.type == "cuda", "block_norm needs CUDA tensors (there is no CPU path)")
+    strides = [0, 0, 0]
+    ts = [x, y, gate]
+    for i, t in enumerate(ts):
+        if t is None or (i == 2 and kind == "channel"):
+            ts[i] = None if t is None else t.contiguous()
+        elif first:
+            ts[i] = t.contiguous()
+        else:
+            ts[i], strides[i] = _as_rows(t, C)
+    pw, w = (None if t is None else t.contiguous() for t in (post_weight, weight))
+    wio = _io_of(pw if pw is not None else w, "weight") if pw is not None or w is not None else 0
+    rows = lead.numel() // C
+    inner = lead.shape[2] if first else 0
+    d = BlockNormDesc(rows, C, inner, groups, _io_of(lead, "y"), _io_of(x if x is not None else lead, "x"), wio, GATE[kind],
+                      ACT[act], scale, eps, lead.device.index, *strides)
+    return d, ts, pw, w, lead, kind
+
+
+def block_norm(x=None, y=None, gate=None, post_weight=None, weight=None, scale=1.0, eps=1e-6, groups=1, act="none", dim=-1,
+               stats=False, stream=None):
+    """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight, each part only where its
+    tensor is given; rstd(z) = (mean z^2 + eps)^-1/2 over the channels (over each of `groups` runs of them for y).
+
+    The channels are the last axis, or axis 1 of [B][C][L] tensors (`dim=1`, the layout of the convolution).  gate: shaped
+    like y, or [C]; act: "none", "silu" or "sigmoid".  y, gate and n have one type (float32 or bfloat16); x and h have it
+    too, or are float32.  Without y, h is x; without weight, n is None.  `stats=True` also returns the rstd of y's groups
+    and of h, for block_norm_backward."""
+    import torch
+    d, (x, y, gate), pw, w, lead, _ = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    raw, side = _call_stream(stream, lead.device)
+    h = x if y is None else torch.empty(lead.shape, dtype=lead.dtype if x is None else x.dtype, device=lead.device)
+    n = None if w is None else torch.empty(lead.shape, dtype=lead.dtype, device=lead.device)
+    r1 = torch.empty((d.rows, groups), dtype=torch.float32, device=lead.device) if stats and pw is not None else None
+    r2 = torch.empty((d.rows,), dtype=torch.float32, device=lead.device) if stats and w is not None else None
+    if lead.numel():
+        _check(lib().sffft_block_norm(ctypes.byref(d), _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(h), _ptr(n),
+                                      _ptr(r1), _ptr(r2), raw), f"block_norm({list(lead.shape)})")
+    _used_on(side, x, y, gate, pw, w, h, n, r1, r2)
+    return (h, n, r1, r2) if stats else (h, n)
+
+
+def block_norm_backward(dh, dn, x=None, y=None, gate=None, post_weight=None, weight=None, rstd_post=None, rstd=None, scale=1.0,
+                        eps=1e-6, groups=1, act="none", dim=-1, stream=None):
+    """(dx, dy, dgate, dpost_weight, dweight) of block_norm from the gradients of h (None: zero) and n; None where the tensor
+    was not given."""
+    import torch
+    d, (x, y, gate), pw, w, lead, kind = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    _need(w is None or dn is not None, "dn is needed where there is a weight")
+    _need(dn is None or (dn.shape == lead.shape and dn.dtype == lead.dtype and w is not None), "dn must be like n")
+    ht = lead.dtype if x is None else x.dtype
+    _need(dh is None or (dh.shape == lead.shape and dh.dtype == ht), "dh must be like h")
+    _need(dh is not None or w is not None, "dh or dn is needed")
+    _need(pw is None or rstd_post is not None, "rstd_post of the forward pass is needed")
+    _need(w is None or rstd is not None, "rstd of the forward pass is needed")
+    for t in (dh, dn, rstd_post, rstd):
+        _need(t is None or t.device == lead.device, "all tensors must be on one device")
+    for t, n in ((rstd_post, d.rows * groups), (rstd, d.rows)):
+        _need(t is None or (t.numel() == n and t.dtype == torch.float32 and t.is_contiguous()), "rstd must be the forward pass's")
+    raw, side = _call_stream(stream, lead.device)
+    dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
+    new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)  # noqa: E731
+    dx, dy, dgate, dpw, dw = new(x), new(y), new(gate), new(pw), new(w)
+    need = ctypes.c_size_t()
+    _check(lib().sffft_block_norm_workspace_bytes(ctypes.byref(d), ctypes.byref(need)), "block_norm_workspace_bytes")
+    work = torch.empty(need.value, dtype=torch.uint8, device=lead.device) if need.value else None
+    if not lead.numel():   # no rows: empty buffers have no address to pass
+        for t in (dgate if kind == "channel" else None, dpw, dw):
+            if t is not None:
+                t.zero_()
+        return dx, dy, dgate, dpw, dw
+    _check(lib().sffft_block_norm_backward(
+        ctypes.byref(d), _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(rstd_post), _ptr(rstd), _ptr(dh), _ptr(dn),
+        _ptr(dx), _ptr(dy), _ptr(dgate), _ptr(dpw), _ptr(dw), _ptr(work), need.value, raw), f"block_norm_backward({list(lead.shape)})")
+    _used_on(side, x, y, gate, pw, w, rstd_post, rstd, dh, dn, dx, dy, dgate, dpw, dw, work)
+    return dx, dy, dgate, dpw, dw

@@ -56,6 +56,9 @@ static int cuda_fail(cudaError_t e) {
   return SFFFT_ERR_CUDA;
 }
 
+// The same for the library's other translation units.
+int sffft_note_cuda_error(cudaError_t e) { return cuda_fail(e); }
+
 static const BlockEntry* block_entry(const char* name) {
   static const std::vector<const BlockEntry*> all = [] {
     std::vector<const BlockEntry*> v;
@@ -120,7 +123,7 @@ const char* sffft_status_string(int s) {
     case SFFFT_ERR_NO_MATCH: return "no candidate meets the error budget";
     case SFFFT_ERR_ALLOC: return "device allocation failed";
     case SFFFT_ERR_SCRATCH_LIMIT: return "problem exceeds the fixed scratch of the allocation-free entry point";
-    case SFFFT_ERR_WORKSPACE: return "composite plan needs a workspace of sffft_conv_workspace_bytes";
+    case SFFFT_ERR_WORKSPACE: return "the call needs a workspace of its workspace_bytes function (composite plans: sffft_conv_workspace_bytes)";
     default: return "unknown status";
   }
 }

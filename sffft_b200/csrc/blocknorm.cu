@@ -1,0 +1,902 @@
+// The joint between two blocks of a network, on rows of C channels:
+//
+//   a = y * rstd_g(y) * post_weight      norm of the block's output, over each of `groups` equal runs of channels
+//   h = x + scale * act(gate) * a        gate, residual scale and residual stream
+//   n = h * rstd(h) * weight             norm before the next block
+//
+// with rstd(z) = (mean z^2 + eps)^-1/2; each norm, the gate and x may be absent.  One pass: x, y and gate are read
+// once, h and n written once, a row's values stay in fp32 registers between the two norms.
+//
+// Backward, with u = y rstd_g(y), z = h rstd(h), f = act(gate) and the two norms' rstd kept from the forward pass:
+//   t  = dn * weight          dx    = dh + rstd(h) (t - z mean(t z))                 dweight      = sum_rows dn z
+//   da = scale f dx           dgate = scale dx a act'(gate)                          dpost_weight = sum_rows da u
+//   s  = da * post_weight     dy    = rstd_g(y) (s - u mean_g(s u))
+// h is computed again from x, y and gate, which are read anyway (it would cost as much to read, and in bf16 the kept h is
+// rounded).  The sums over rows are taken in a fixed order: each block of a fixed grid adds its rows in registers (or,
+// channels first, in shared memory), a second launch adds the blocks.
+//
+// Two layouts: rows of contiguous channels, and the convolution's [B][C][L], where a row is a column of stride L.
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include <climits>
+#include <cmath>
+
+#include "../../include/sffft.h"
+#include "launch.h"
+
+int sffft_note_cuda_error(cudaError_t e);
+
+namespace sffft {
+namespace {
+
+enum { GATE_NONE = 0, GATE_FULL = 1, GATE_CHANNEL = 2 };
+
+struct NormParams {
+  const void *x, *y, *gate, *pw, *w;
+  void *h, *n;
+  float *r1, *r2;             // rstd of the groups of y [rows][groups] and of h [rows] (written forward, read backward)
+  const void *dh, *dn;
+  void *dx, *dy, *dgate;
+  float* part;                // [blocks][3][C]: sums of dweight, dpost_weight, dgate of a channel gate
+  long long rows, xs, ys, gs; // rows layout: row strides
+  int C, groups, gc, inner;   // gc channels in a group; inner: L of [B][C][L]
+  int gate_kind, act, w_bf16;
+  int blocks;                 // backward: blocks of the grid
+  float scale, eps;
+};
+
+__device__ __forceinline__ float ldf(const float* p) { return *p; }
+__device__ __forceinline__ float ldf(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// VEC consecutive values; VEC > 1 in 16-byte (fp32 x 4, bf16 x 8) or 8-byte (bf16 x 4) pieces.
+template <int VEC>
+__device__ __forceinline__ void ldv(const float* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) v[0] = *p;
+  else
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const float4 a = *(const float4*)(p + i);
+      v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
+    }
+}
+__device__ __forceinline__ void unpack(uint32_t u, float& a, float& b) {
+  a = __uint_as_float(u << 16);
+  b = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *(const uint32_t*)&t;
+}
+template <int VEC>
+__device__ __forceinline__ void ldv(const __nv_bfloat16* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) v[0] = __bfloat162float(*p);
+  else if constexpr (VEC == 4) {
+    const uint2 a = *(const uint2*)p;
+    unpack(a.x, v[0], v[1]);
+    unpack(a.y, v[2], v[3]);
+  } else {
+    const uint4 a = *(const uint4*)p;
+    unpack(a.x, v[0], v[1]);
+    unpack(a.y, v[2], v[3]);
+    unpack(a.z, v[4], v[5]);
+    unpack(a.w, v[6], v[7]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void stv(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) *p = v[0];
+  else
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+template <int VEC>
+__device__ __forceinline__ void stv(__nv_bfloat16* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) *p = __float2bfloat16_rn(v[0]);
+  else if constexpr (VEC == 4) *(uint2*)p = make_uint2(pack(v[0], v[1]), pack(v[2], v[3]));
+  else *(uint4*)p = make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+}
+template <int VEC>
+__device__ __forceinline__ void ldw(const void* w, int bf16, int c, float (&v)[VEC]) {
+  if (bf16) ldv<VEC>((const __nv_bfloat16*)w + c, v);
+  else ldv<VEC>((const float*)w + c, v);
+}
+
+__device__ __forceinline__ float sigmoidf(float x) { return 1.f / (1.f + expf(-x)); }
+
+// act(gate) and its derivative
+__device__ __forceinline__ void act_fwd(int act, float g, float& f) {
+  if (act == SFFFT_ACT_SILU) f = g * sigmoidf(g);
+  else if (act == SFFFT_ACT_SIGMOID) f = sigmoidf(g);
+  else f = g;
+}
+__device__ __forceinline__ void act_both(int act, float g, float& f, float& df) {
+  if (act == SFFFT_ACT_SILU) {
+    const float s = sigmoidf(g);
+    f = g * s;
+    df = s * (1.f + g * (1.f - s));
+  } else if (act == SFFFT_ACT_SIGMOID) {
+    f = sigmoidf(g);
+    df = f * (1.f - f);
+  } else {
+    f = g;
+    df = 1.f;
+  }
+}
+
+// Sum over the threads of a row: a warp (TPR = 32), or the block.  `red` holds a float for each warp.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float s, float* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  if constexpr (TPR > 32) {
+    __syncthreads();   // earlier readers of red
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = red[threadIdx.x & (TPR / 32 - 1)];
+#pragma unroll
+    for (int o = TPR / 64; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  }
+  return s;
+}
+
+template <int TPR>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (TPR > 32) __syncthreads();
+  else __syncwarp();
+}
+
+// Sums over the groups of channels: v[j] is the sum over the thread's j-th vector, replaced by its group's sum.  Where
+// a group is a power of two of at most 32 vectors its vectors lie in neighbouring lanes (a row's threads start at a
+// multiple of 32); otherwise the vectors' sums go through shared memory, one warp adding up a group.
+template <int TPR, int NV>
+__device__ __forceinline__ void group_sums(float (&v)[NV], int nvec, int per, int groups, float* vec, float* grp, float* red,
+                                           int t) {
+  if (groups == 1) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) s += v[j];
+    s = row_sum<TPR>(s, red);
+#pragma unroll
+    for (int j = 0; j < NV; j++) v[j] = s;
+    return;
+  }
+  if (per <= 32 && (per & (per - 1)) == 0) {
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      for (int o = per >> 1; o; o >>= 1) v[j] += __shfl_xor_sync(~0u, v[j], o);
+    return;
+  }
+  row_sync<TPR>();
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+    if (j * TPR + t < nvec) vec[j * TPR + t] = v[j];
+  row_sync<TPR>();
+  for (int g = t >> 5; g < groups; g += TPR / 32) {
+    float s = 0.f;
+    for (int e = t & 31; e < per; e += 32) s += vec[g * per + e];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if ((t & 31) == 0) grp[g] = s;
+  }
+  row_sync<TPR>();
+#pragma unroll
+  for (int j = 0; j < NV; j++) v[j] = j * TPR + t < nvec ? grp[(j * TPR + t) / per] : 0.f;
+}
+
+// Shared memory of a block's rows: vector sums and group sums (only where group_sums needs them), 32 floats for row_sum.
+__host__ __device__ inline int rows_smem_floats(int nvec, int groups) { return groups > 1 ? nvec + groups : 0; }
+
+template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
+__global__ void __launch_bounds__(TPR* RPB) norm_rows_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) float dyn[];
+  __shared__ float red[32];
+  const int t = threadIdx.x % TPR, nvec = p.C / VEC;
+  float* vec = dyn + (threadIdx.x / TPR) * rows_smem_floats(nvec, p.groups);
+  float* grp = vec + nvec;
+  const long long r = blockIdx.x * (long long)RPB + threadIdx.x / TPR;
+  if (r >= p.rows) return;   // whole warps (RPB > 1 only with TPR = 32)
+  float v[NV][VEC], a[NV][VEC];
+  const TY* y = (const TY*)p.y + r * p.ys;
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int i = j * TPR + t;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) v[j][e] = 0.f;
+    if (p.y && i < nvec) ldv<VEC>(y + i * VEC, v[j]);
+  }
+  if (p.x) {
+    const TX* x = (const TX*)p.x + r * p.xs;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * TPR + t;
+      if (i < nvec) ldv<VEC>(x + i * VEC, a[j]);
+    }
+  }
+  if (p.pw) {
+    float s[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      s[j] = 0.f;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) s[j] = fmaf(v[j][e], v[j][e], s[j]);
+    }
+    const int per = p.gc / VEC;
+    group_sums<TPR, NV>(s, nvec, per, p.groups, vec, grp, red, t);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * TPR + t;
+      if (i >= nvec) continue;
+      const float rs = rsqrtf(s[j] / (float)p.gc + p.eps);
+      if (p.r1 && i % per == 0) p.r1[r * p.groups + i / per] = rs;
+      float w[VEC];
+      ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) v[j][e] *= rs * w[e];
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int i = j * TPR + t;
+    if (i >= nvec) continue;
+    if (p.y) {
+      if (p.gate_kind) {
+        float g[VEC];
+        ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          float f;
+          act_fwd(p.act, g[e], f);
+          v[j][e] *= f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; e++) v[j][e] = p.x ? fmaf(p.scale, v[j][e], a[j][e]) : p.scale * v[j][e];
+      if (p.h) stv<VEC>((TX*)p.h + r * p.C + i * VEC, v[j]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) v[j][e] = a[j][e];
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e++) ss = fmaf(v[j][e], v[j][e], ss);
+  }
+  if (!p.w) return;
+  ss = row_sum<TPR>(ss, red);
+  const float rs = rsqrtf(ss / (float)p.C + p.eps);
+  if (p.r2 && t == 0) p.r2[r] = rs;
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int i = j * TPR + t;
+    if (i >= nvec) continue;
+    float w[VEC];
+    ldw<VEC>(p.w, p.w_bf16, i * VEC, w);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) v[j][e] *= rs * w[e];
+    stv<VEC>((TY*)p.n + r * p.C + i * VEC, v[j]);
+  }
+}
+
+template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
+__global__ void __launch_bounds__(TPR* RPB) norm_rows_bwd_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) float dyn[];
+  __shared__ float red[32];
+  const int t = threadIdx.x % TPR, nvec = p.C / VEC, per = p.gc / VEC, sub = threadIdx.x / TPR;
+  float* vec = dyn + sub * rows_smem_floats(nvec, p.groups);
+  float* grp = vec + nvec;
+  float sw[NV][VEC], sp[NV][VEC], sg[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+#pragma unroll
+    for (int e = 0; e < VEC; e++) sw[j][e] = sp[j][e] = sg[j][e] = 0.f;
+
+  for (long long r = blockIdx.x * (long long)RPB + sub; r < p.rows; r += (long long)p.blocks * RPB) {
+    const float r2 = p.w ? p.r2[r] : 0.f;
+    float u[NV][VEC], z[NV][VEC], d[NV][VEC];   // u, then s u's parts; h, then z; dx
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * TPR + t;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) d[j][e] = z[j][e] = u[j][e] = 0.f;
+      if (i >= nvec) continue;
+      float a[VEC], f[VEC];
+      if (p.y) {
+        ldv<VEC>((const TY*)p.y + r * p.ys + i * VEC, u[j]);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) a[e] = u[j][e];
+        if (p.pw) {
+          const float r1 = p.r1[r * p.groups + i / per];
+          float w[VEC];
+          ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            u[j][e] *= r1;
+            a[e] = u[j][e] * w[e];
+          }
+        }
+        if (p.gate_kind) {
+          float g[VEC];
+          ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) act_fwd(p.act, g[e], f[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) f[e] = 1.f;
+        }
+      }
+      if (p.dh) ldv<VEC>((const TX*)p.dh + r * p.C + i * VEC, d[j]);
+      if (p.w) {
+        float tn[VEC], w[VEC];
+        if (p.x) ldv<VEC>((const TX*)p.x + r * p.xs + i * VEC, z[j]);
+        ldv<VEC>((const TY*)p.dn + r * p.C + i * VEC, tn);
+        ldw<VEC>(p.w, p.w_bf16, i * VEC, w);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          if (p.y) z[j][e] = fmaf(p.scale * f[e], a[e], z[j][e]);
+          z[j][e] *= r2;
+          sw[j][e] = fmaf(tn[e], z[j][e], sw[j][e]);
+          const float tt = tn[e] * w[e];
+          s = fmaf(tt, z[j][e], s);
+          d[j][e] = fmaf(r2, tt, d[j][e]);
+        }
+      }
+    }
+    if (p.w) {
+      s = row_sum<TPR>(s, red) / (float)p.C * r2;
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) d[j][e] = fmaf(-s, z[j][e], d[j][e]);
+    }
+    float gs[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * TPR + t;
+      gs[j] = 0.f;
+      if (i >= nvec) continue;
+      if (p.dx) stv<VEC>((TX*)p.dx + r * p.C + i * VEC, d[j]);
+      if (!p.y) continue;
+      float w[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) w[e] = 1.f;
+      if (p.pw) ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
+      float f[VEC], g[VEC];
+      if (p.gate_kind) {
+        ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          float df;
+          act_both(p.act, g[e], f[e], df);
+          g[e] = p.scale * d[j][e] * u[j][e] * w[e] * df;
+          sg[j][e] += g[e];
+        }
+        if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + r * p.C + i * VEC, g);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) f[e] = 1.f;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const float da = p.scale * f[e] * d[j][e];
+        if (p.pw) sp[j][e] = fmaf(da, u[j][e], sp[j][e]);
+        d[j][e] = da * w[e];
+        gs[j] = fmaf(d[j][e], u[j][e], gs[j]);
+      }
+    }
+    if (!p.y) continue;
+    if (p.pw) group_sums<TPR, NV>(gs, nvec, per, p.groups, vec, grp, red, t);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * TPR + t;
+      if (i >= nvec) continue;
+      if (p.pw) {
+        const float r1 = p.r1[r * p.groups + i / per], m = gs[j] / (float)p.gc;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) d[j][e] = r1 * fmaf(-m, u[j][e], d[j][e]);
+      }
+      stv<VEC>((TY*)p.dy + r * p.C + i * VEC, d[j]);
+    }
+  }
+  // this block's sums over its rows, its warps' one after the other
+  float* out = p.part + (long long)blockIdx.x * 3 * p.C;
+  for (int q = 0; q < RPB; q++) {
+    if (q == sub) {
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = j * TPR + t;
+        if (i >= nvec) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          const int c = i * VEC + e;
+          if (p.w) out[c] = (q ? out[c] : 0.f) + sw[j][e];
+          if (p.pw) out[p.C + c] = (q ? out[p.C + c] : 0.f) + sp[j][e];
+          if (p.gate_kind == GATE_CHANNEL) out[2 * p.C + c] = (q ? out[2 * p.C + c] : 0.f) + sg[j][e];
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Channels first: [B][C][L].  A block takes kPos positions of one row of the batch, all channels: kPos / VEC threads
+// across the positions, the others down the channels.  The sums over channels are taken by each thread for its own
+// positions and channels, then over the threads that share the positions, through shared memory.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kPos = 32, kFirstThreads = 256;
+
+template <int VEC>
+struct FirstShape {
+  static constexpr int TX = kPos / VEC, TY = kFirstThreads / TX;
+};
+
+// Sum over ty of each position's value; red: [TY][kPos].
+template <int VEC>
+__device__ __forceinline__ void first_sum(float (&s)[VEC], float* red, int tx, int ty) {
+  constexpr int TY = FirstShape<VEC>::TY;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < VEC; e++) red[ty * kPos + tx * VEC + e] = s[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < VEC; e++) {
+    float z = 0.f;
+    for (int q = 0; q < TY; q++) z += red[q * kPos + tx * VEC + e];
+    s[e] = z;
+  }
+}
+
+struct FirstTile {
+  long long base;   // element (channel 0, first position of the thread)
+  long long row;    // row index of that position
+  int left;         // positions of the thread inside L
+};
+
+template <int VEC>
+__device__ __forceinline__ FirstTile first_tile(const NormParams& p, long long tile, int tx) {
+  const int per = (p.inner + kPos - 1) / kPos;
+  const long long b = tile / per;
+  const int l = (int)(tile % per) * kPos + tx * VEC;
+  return {b * p.C * p.inner + l, b * p.inner + l, l < p.inner ? min(VEC, p.inner - l) : 0};
+}
+
+template <class TX, class TY, int VEC>
+__global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_constant__ NormParams p) {
+  constexpr int TXN = FirstShape<VEC>::TX, TYN = FirstShape<VEC>::TY;
+  extern __shared__ __align__(16) float dyn[];
+  float* red = dyn;                 // [TYN][kPos]
+  float* r1 = dyn + TYN * kPos;     // [groups][kPos]
+  const int tx = threadIdx.x % TXN, ty = threadIdx.x / TXN;
+  const FirstTile ft = first_tile<VEC>(p, blockIdx.x, tx);
+  const bool in = ft.left > 0;   // VEC 4: L is a multiple of 4
+  const TY *y = (const TY*)p.y + ft.base, *gate = (const TY*)p.gate;
+  const TX* x = (const TX*)p.x + ft.base;
+  const long long L = p.inner;
+  if (p.pw) {
+    for (int g = 0; g < p.groups; g++) {
+      float s[VEC] = {};
+      if (in)
+        for (int c = g * p.gc + ty; c < (g + 1) * p.gc; c += TYN) {
+          float v[VEC];
+          ldv<VEC>(y + c * L, v);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) s[e] = fmaf(v[e], v[e], s[e]);
+        }
+      first_sum<VEC>(s, red, tx, ty);
+      if (ty == 0)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          const float rs = rsqrtf(s[e] / (float)p.gc + p.eps);
+          r1[g * kPos + tx * VEC + e] = rs;
+          if (p.r1 && in) p.r1[(ft.row + e) * p.groups + g] = rs;
+        }
+    }
+    __syncthreads();
+  }
+  auto value = [&](int c, float (&h)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; e++) h[e] = 0.f;
+    if (p.y) {
+      ldv<VEC>(y + c * L, h);
+      if (p.pw) {
+        float w[1];
+        ldw<1>(p.pw, p.w_bf16, c, w);
+        const int g = c / p.gc;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) h[e] *= r1[g * kPos + tx * VEC + e] * w[0];
+      }
+      if (p.gate_kind) {
+        float gv[VEC];
+        if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
+        else
+#pragma unroll
+          for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          float f;
+          act_fwd(p.act, gv[e], f);
+          h[e] *= f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; e++) h[e] *= p.scale;
+    }
+    if (p.x) {
+      float xv[VEC];
+      ldv<VEC>(x + c * L, xv);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) h[e] += xv[e];
+    }
+  };
+  float s[VEC] = {};
+  if (in)
+    for (int c = ty; c < p.C; c += TYN) {
+      float h[VEC];
+      value(c, h);
+      if (p.h) stv<VEC>((TX*)p.h + ft.base + c * L, h);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) s[e] = fmaf(h[e], h[e], s[e]);
+    }
+  if (!p.w) return;
+  first_sum<VEC>(s, red, tx, ty);
+  if (!in) return;
+#pragma unroll
+  for (int e = 0; e < VEC; e++) {
+    s[e] = rsqrtf(s[e] / (float)p.C + p.eps);
+    if (p.r2 && ty == 0) p.r2[ft.row + e] = s[e];
+  }
+  for (int c = ty; c < p.C; c += TYN) {
+    float h[VEC], w[1];
+    value(c, h);
+    ldw<1>(p.w, p.w_bf16, c, w);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) h[e] *= s[e] * w[0];
+    stv<VEC>((TY*)p.n + ft.base + c * L, h);
+  }
+}
+
+template <class TX, class TY, int VEC>
+__global__ void __launch_bounds__(kFirstThreads) norm_first_bwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr int TXN = FirstShape<VEC>::TX, TYN = FirstShape<VEC>::TY;
+  extern __shared__ __align__(16) float dyn[];
+  float* red = dyn;                     // [TYN][kPos]
+  float* m1 = dyn + TYN * kPos;         // [groups][kPos]
+  const int tx = threadIdx.x % TXN, ty = threadIdx.x / TXN;
+  float* out = p.part + (long long)blockIdx.x * 3 * p.C;   // this block's sums; a channel always belongs to one ty
+  const long long L = p.inner;
+  const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
+  const TY* gate = (const TY*)p.gate;
+  bool first = true;
+  for (long long tile = blockIdx.x; tile < tiles; tile += p.blocks, first = false) {
+    const FirstTile ft = first_tile<VEC>(p, tile, tx);
+    const bool in = ft.left > 0;
+    float r2[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) r2[e] = p.w && in ? p.r2[ft.row + e] : 0.f;
+    // u, a = u * post_weight, gate, z and dh + rstd t of channel c
+    auto load = [&](int c, float (&u)[VEC], float& pw, float (&gv)[VEC], float (&z)[VEC], float (&d)[VEC], float (&tn)[VEC],
+                    float& w, float (&q1)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) u[e] = z[e] = d[e] = tn[e] = 0.f, gv[e] = 1.f, q1[e] = 1.f;
+      pw = 1.f;
+      w = 0.f;
+      if (p.y) {
+        ldv<VEC>((const TY*)p.y + ft.base + c * L, u);
+        if (p.pw) {
+          float t[1];
+          ldw<1>(p.pw, p.w_bf16, c, t);
+          pw = t[0];
+          const int g = c / p.gc;
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            q1[e] = p.r1[(ft.row + e) * p.groups + g];
+            u[e] *= q1[e];
+          }
+        }
+        if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
+        else if (p.gate_kind == GATE_CHANNEL)
+#pragma unroll
+          for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
+      }
+      if (p.dh) ldv<VEC>((const TX*)p.dh + ft.base + c * L, d);
+      if (p.w) {
+        float t[1];
+        ldw<1>(p.w, p.w_bf16, c, t);
+        w = t[0];
+        if (p.x) ldv<VEC>((const TX*)p.x + ft.base + c * L, z);
+        ldv<VEC>((const TY*)p.dn + ft.base + c * L, tn);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          if (p.y) {
+            float f = 1.f;
+            if (p.gate_kind) act_fwd(p.act, gv[e], f);
+            z[e] = fmaf(p.scale * f, u[e] * pw, z[e]);
+          }
+          z[e] *= r2[e];
+          d[e] = fmaf(r2[e], tn[e] * w, d[e]);
+        }
+      }
+    };
+    float u[VEC], gv[VEC], z[VEC], d[VEC], tn[VEC], q1[VEC], pw, w;
+    float m2[VEC] = {};
+    if (p.w) {
+      if (in)
+        for (int c = ty; c < p.C; c += TYN) {
+          load(c, u, pw, gv, z, d, tn, w, q1);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) m2[e] = fmaf(tn[e] * w, z[e], m2[e]);
+        }
+      first_sum<VEC>(m2, red, tx, ty);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) m2[e] *= r2[e] / (float)p.C;
+    }
+    if (p.y && p.pw) {
+      for (int g = 0; g < p.groups; g++) {
+        float s[VEC] = {};
+        if (in)
+          for (int c = g * p.gc + ty; c < (g + 1) * p.gc; c += TYN) {
+            load(c, u, pw, gv, z, d, tn, w, q1);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+              float f = 1.f;
+              if (p.gate_kind) act_fwd(p.act, gv[e], f);
+              s[e] = fmaf(p.scale * f * fmaf(-m2[e], z[e], d[e]) * pw, u[e], s[e]);
+            }
+          }
+        first_sum<VEC>(s, red, tx, ty);
+        if (ty == 0)
+#pragma unroll
+          for (int e = 0; e < VEC; e++) m1[g * kPos + tx * VEC + e] = s[e] / (float)p.gc;
+      }
+      __syncthreads();
+    }
+    for (int c = ty; c < p.C; c += TYN) {
+      float sw = 0.f, sp = 0.f, sg = 0.f;
+      if (in) {
+        load(c, u, pw, gv, z, d, tn, w, q1);
+        float dg[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          sw = fmaf(tn[e], z[e], sw);
+          d[e] = fmaf(-m2[e], z[e], d[e]);
+        }
+        if (p.dx) stv<VEC>((TX*)p.dx + ft.base + c * L, d);
+        if (p.y) {
+          const int g = c / p.gc;
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            float f = 1.f, df = 0.f;
+            if (p.gate_kind) act_both(p.act, gv[e], f, df);
+            dg[e] = p.scale * d[e] * u[e] * pw * df;
+            sg += dg[e];
+            const float da = p.scale * f * d[e];
+            sp = fmaf(da, u[e], sp);
+            d[e] = p.pw ? q1[e] * fmaf(-m1[g * kPos + tx * VEC + e], u[e], da * pw) : da;
+          }
+          if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + ft.base + c * L, dg);
+          stv<VEC>((TY*)p.dy + ft.base + c * L, d);
+        }
+      }
+      // the TXN threads of a channel are neighbouring lanes (TXN divides 32); lanes of a warp whose channel is
+      // beyond C have left the loop together with their whole group
+      const unsigned mask = TXN == 32 ? ~0u : ((1u << TXN) - 1) << ((threadIdx.x & 31) / TXN * TXN);
+#pragma unroll
+      for (int o = TXN / 2; o; o >>= 1) {
+        sw += __shfl_xor_sync(mask, sw, o);
+        sp += __shfl_xor_sync(mask, sp, o);
+        sg += __shfl_xor_sync(mask, sg, o);
+      }
+      if (tx == 0) {
+        if (p.w) out[c] = (first ? 0.f : out[c]) + sw;
+        if (p.pw) out[p.C + c] = (first ? 0.f : out[p.C + c]) + sp;
+        if (p.gate_kind == GATE_CHANNEL) out[2 * p.C + c] = (first ? 0.f : out[2 * p.C + c]) + sg;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Sums the blocks' parts: a block takes 32 channels, 8 threads down the parts, added in a fixed order.
+struct PartParams {
+  const float* part;
+  void* out[3];       // dweight, dpost_weight, dgate (null: not wanted)
+  int C, blocks, w_bf16, g_bf16;
+};
+
+__global__ void __launch_bounds__(256) norm_part_kernel(const __grid_constant__ PartParams p) {
+  __shared__ float sm[8][33];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c = blockIdx.x * 32 + tx, k = blockIdx.y;
+  if (!p.out[k]) return;
+  float s = 0.f;
+  if (c < p.C)
+    for (int b = ty; b < p.blocks; b += 8) s += p.part[((long long)b * 3 + k) * p.C + c];
+  sm[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < p.C) {
+    s = 0.f;
+    for (int q = 0; q < 8; q++) s += sm[q][tx];
+    if (k == 2 ? p.g_bf16 : p.w_bf16) ((__nv_bfloat16*)p.out[k])[c] = __float2bfloat16_rn(s);
+    else ((float*)p.out[k])[c] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kMaxChannels = 8192;   // what a block's registers hold in the backward pass
+
+template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
+cudaError_t rows_t(const NormParams& p, bool bwd, cudaStream_t st) {
+  const int smem = 4 * RPB * rows_smem_floats(p.C / VEC, p.groups);
+  if (bwd) return launch(norm_rows_bwd_kernel<TX, TY, VEC, TPR, NV, RPB>, dim3((unsigned)p.blocks), TPR * RPB, smem, st, p);
+  return launch(norm_rows_kernel<TX, TY, VEC, TPR, NV, RPB>, dim3((unsigned)((p.rows + RPB - 1) / RPB)), TPR * RPB, smem, st, p);
+}
+
+// Threads for a row: a warp holds up to 4 vectors a thread; wider rows take a block, of which NV vectors a thread.
+template <class TX, class TY, int VEC>
+cudaError_t rows_v(const NormParams& p, bool bwd, cudaStream_t st) {
+  const int nvec = p.C / VEC;
+  if (nvec <= 32) return rows_t<TX, TY, VEC, 32, 1, 4>(p, bwd, st);
+  if (nvec <= 64) return rows_t<TX, TY, VEC, 32, 2, 4>(p, bwd, st);
+  if (nvec <= 128) return rows_t<TX, TY, VEC, 128, 1, 1>(p, bwd, st);
+  if (nvec <= 256) return rows_t<TX, TY, VEC, 256, 1, 1>(p, bwd, st);
+  if (nvec <= 512) return rows_t<TX, TY, VEC, 512, 1, 1>(p, bwd, st);
+  if constexpr (VEC == 8) return rows_t<TX, TY, VEC, 512, 2, 1>(p, bwd, st);
+  else {
+    if (nvec <= 1024) return rows_t<TX, TY, VEC, 512, 2, 1>(p, bwd, st);
+    if constexpr (VEC > 1) return rows_t<TX, TY, VEC, 512, 4, 1>(p, bwd, st);
+    else return rows_t<TX, TY, 1, 1024, 8, 1>(p, bwd, st);
+  }
+}
+
+template <class TX, class TY, int VEC>
+cudaError_t first_v(const NormParams& p, bool bwd, cudaStream_t st) {
+  const int smem = 4 * (FirstShape<VEC>::TY * kPos + p.groups * kPos);
+  const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
+  if (bwd) return launch(norm_first_bwd_kernel<TX, TY, VEC>, dim3((unsigned)p.blocks), kFirstThreads, smem, st, p);
+  return launch(norm_first_kernel<TX, TY, VEC>, dim3((unsigned)tiles), kFirstThreads, smem, st, p);
+}
+
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+template <class TX, class TY>
+cudaError_t norm_t(const NormParams& p, bool bwd, cudaStream_t st) {
+  if (p.inner) {
+    const bool v4 = p.inner % 4 == 0 && aligned(p.x, 4 * sizeof(TX)) && aligned(p.h, 4 * sizeof(TX)) &&
+                    aligned(p.dh, 4 * sizeof(TX)) && aligned(p.dx, 4 * sizeof(TX)) && aligned(p.y, 4 * sizeof(TY)) &&
+                    aligned(p.n, 4 * sizeof(TY)) && aligned(p.dn, 4 * sizeof(TY)) && aligned(p.dy, 4 * sizeof(TY)) &&
+                    (p.gate_kind != GATE_FULL || (aligned(p.gate, 4 * sizeof(TY)) && aligned(p.dgate, 4 * sizeof(TY))));
+    return v4 ? first_v<TX, TY, 4>(p, bwd, st) : first_v<TX, TY, 1>(p, bwd, st);
+  }
+  constexpr int V = 16 / sizeof(TY);
+  const bool vec = p.C % V == 0 && p.gc % V == 0 && p.xs % V == 0 && p.ys % V == 0 && p.gs % V == 0 && aligned(p.x, 16) &&
+                   aligned(p.y, 16) && aligned(p.gate, 16) && aligned(p.h, 16) && aligned(p.n, 16) && aligned(p.dh, 16) &&
+                   aligned(p.dn, 16) && aligned(p.dx, 16) && aligned(p.dy, 16) &&
+                   (p.gate_kind != GATE_FULL || aligned(p.dgate, 16)) && aligned(p.pw, 16) && aligned(p.w, 16);
+  return vec ? rows_v<TX, TY, V>(p, bwd, st) : rows_v<TX, TY, 1>(p, bwd, st);
+}
+
+cudaError_t norm_any(const NormParams& p, int res_io, int io, bool bwd, cudaStream_t st) {
+  if (res_io == SFFFT_IO_FP32 && io == SFFFT_IO_FP32) return norm_t<float, float>(p, bwd, st);
+  if (res_io == SFFFT_IO_FP32) return norm_t<float, __nv_bfloat16>(p, bwd, st);
+  return norm_t<__nv_bfloat16, __nv_bfloat16>(p, bwd, st);
+}
+
+int check(const sffft_block_norm_t* d, const void* x, const void* y, const void* gate, const void* pw, const void* w) {
+  auto io_ok = [](int v) { return v == SFFFT_IO_FP32 || v == SFFFT_IO_BF16; };
+  if (!d || d->rows < 0 || d->channels < 1 || d->inner < 0 || d->groups < 1 || d->channels % d->groups != 0 ||
+      !io_ok(d->io) || !io_ok(d->res_io) || !io_ok(d->weight_io) || d->gate < 0 || d->gate > 2 || d->act < 0 || d->act > 2 ||
+      !std::isfinite(d->scale) || !(d->eps >= 0.f) || !std::isfinite(d->eps) || d->device < 0)
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  if (d->inner && d->rows % d->inner != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!y && (!x || gate || pw || d->gate)) return SFFFT_ERR_INVALID_ARGUMENT;   // nothing to norm, or a gate of nothing
+  if (!y && !w) return SFFFT_ERR_INVALID_ARGUMENT;                              // nothing to do
+  if ((d->gate != 0) != (gate != nullptr)) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (d->groups > 1 && !pw) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (d->res_io == SFFFT_IO_BF16 && d->io == SFFFT_IO_FP32) return SFFFT_ERR_UNSUPPORTED;
+  if (!x && d->res_io != d->io) return SFFFT_ERR_UNSUPPORTED;
+  if (d->channels > kMaxChannels || d->rows > INT_MAX) return SFFFT_ERR_UNSUPPORTED;
+  if (d->inner && d->groups > 256) return SFFFT_ERR_UNSUPPORTED;
+  return SFFFT_OK;
+}
+
+int backward_blocks(const sffft_block_norm_t* d, int sms) {
+  const long long units = d->inner ? (d->rows / d->inner) * ((d->inner + kPos - 1) / kPos) : d->rows;
+  const long long most = 4ll * sms;
+  return (int)(units < most ? units : most);
+}
+
+int facts(int device, int* sms) {
+  int major = 0, minor = 0;
+  cudaError_t ce = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+  if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+  if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
+  if (ce != cudaSuccess) return sffft_note_cuda_error(ce);
+  return major == 10 && minor == 0 ? SFFFT_OK : SFFFT_ERR_DEVICE;
+}
+
+NormParams params(const sffft_block_norm_t* d, const void* x, const void* y, const void* gate, const void* pw, const void* w) {
+  NormParams p = {};
+  p.x = x; p.y = y; p.gate = gate; p.pw = pw; p.w = w;
+  p.rows = d->rows; p.xs = d->x_stride; p.ys = d->y_stride; p.gs = d->gate_stride;
+  if (d->gate != GATE_FULL) p.gs = 0;
+  if (!x) p.xs = 0;
+  if (!y) p.ys = 0;
+  p.C = d->channels; p.groups = d->groups; p.gc = d->channels / d->groups; p.inner = d->inner;
+  p.gate_kind = d->gate; p.act = d->act; p.w_bf16 = d->weight_io == SFFFT_IO_BF16;
+  p.scale = d->scale; p.eps = d->eps;
+  return p;
+}
+
+}  // namespace
+}  // namespace sffft
+
+using namespace sffft;
+
+extern "C" {
+
+int sffft_block_norm(const sffft_block_norm_t* d, const void* x, const void* y, const void* gate, const void* post_weight,
+                     const void* weight, void* h, void* n, float* rstd_post, float* rstd, void* stream) {
+  int rc = check(d, x, y, gate, post_weight, weight);
+  if (rc) return rc;
+  if ((y && !h) || (weight && !n)) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (d->rows == 0) return SFFFT_OK;
+  int sms;
+  if ((rc = facts(d->device, &sms))) return rc;
+  NormParams p = params(d, x, y, gate, post_weight, weight);
+  p.h = y ? h : nullptr;
+  p.n = n;
+  p.r1 = rstd_post;
+  p.r2 = rstd;
+  DeviceScope scope(d->device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  const cudaError_t ce = norm_any(p, d->res_io, d->io, false, (cudaStream_t)stream);
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+int sffft_block_norm_workspace_bytes(const sffft_block_norm_t* d, size_t* bytes) {
+  if (!d || !bytes || d->rows < 0 || d->channels < 1 || d->inner < 0 || d->device < 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (d->channels > kMaxChannels || d->rows > INT_MAX) return SFFFT_ERR_UNSUPPORTED;
+  int sms;
+  const int rc = facts(d->device, &sms);
+  if (rc) return rc;
+  *bytes = (size_t)backward_blocks(d, sms) * 3 * d->channels * sizeof(float);
+  return SFFFT_OK;
+}
+
+int sffft_block_norm_backward(const sffft_block_norm_t* d, const void* x, const void* y, const void* gate,
+                              const void* post_weight, const void* weight, const float* rstd_post, const float* rstd,
+                              const void* dh, const void* dn, void* dx, void* dy, void* dgate, void* dpost_weight,
+                              void* dweight, void* work, size_t work_bytes, void* stream) {
+  int rc = check(d, x, y, gate, post_weight, weight);
+  if (rc) return rc;
+  if ((x && !dx) || (y && !dy) || (gate && !dgate) || (post_weight && (!dpost_weight || !rstd_post)) ||
+      (weight && (!dweight || !rstd || !dn)) || (!weight && !dh))
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  int sms;
+  if ((rc = facts(d->device, &sms))) return rc;
+  NormParams p = params(d, x, y, gate, post_weight, weight);
+  p.r1 = const_cast<float*>(rstd_post);
+  p.r2 = const_cast<float*>(rstd);
+  p.dh = dh; p.dn = weight ? dn : nullptr; p.dx = x ? dx : nullptr; p.dy = dy; p.dgate = dgate;
+  p.blocks = backward_blocks(d, sms);
+  p.part = (float*)work;
+  const size_t need = (size_t)p.blocks * 3 * d->channels * sizeof(float);
+  if (need && (!work || work_bytes < need)) return SFFFT_ERR_WORKSPACE;
+  DeviceScope scope(d->device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t ce = cudaSuccess;
+  if (p.blocks) ce = norm_any(p, d->res_io, d->io, true, st);
+  const bool cg = d->gate == GATE_CHANNEL;
+  if (ce == cudaSuccess && (weight || post_weight || cg)) {   // with no rows the sums are zero
+    PartParams q = {p.part, {weight ? dweight : nullptr, post_weight ? dpost_weight : nullptr, cg ? dgate : nullptr},
+                    d->channels, p.blocks, p.w_bf16, d->io == SFFFT_IO_BF16};
+    ce = launch(norm_part_kernel, dim3((unsigned)((d->channels + 31) / 32), 3), 256, 0, st, q);
+  }
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+}  // extern "C"

@@ -1,0 +1,45 @@
+// Kernel launches that report their own error code (and leave an earlier one of the thread alone), and the device
+// that a call runs on.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace sffft {
+
+template <class K, class P>
+cudaError_t launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& prm) {
+  if (smem > 48 * 1024) {   // a property of the kernel on the current device; setting it again costs under 1 us
+    const cudaError_t ce =
+        cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (ce != cudaSuccess) return ce;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, kernel, prm);
+}
+
+// Makes a call's device current and puts the caller's back at its end.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    err = cudaGetDevice(&prev_);
+    if (err == cudaSuccess && prev_ != device) {
+      err = cudaSetDevice(device);
+      back_ = err == cudaSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (back_) cudaSetDevice(prev_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  cudaError_t err;
+
+ private:
+  int prev_ = 0;
+  bool back_ = false;
+};
+
+}  // namespace sffft

@@ -1,0 +1,390 @@
+// Linear attention with a decay for each head: C ABI, planning, the single-token kernel and the sum over the heads
+// that share a key and value head.
+#include <cuda_bf16.h>
+
+#include <climits>
+#include <cmath>
+
+#include "../../include/sffft.h"
+#include "launch.h"
+#include "linattn.h"
+
+int sffft_note_cuda_error(cudaError_t e);
+
+namespace sffft {
+namespace {
+
+__device__ __forceinline__ float ldf(const float* p) { return *p; }
+__device__ __forceinline__ float ldf(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void stf(float* p, float x) { *p = x; }
+__device__ __forceinline__ void stf(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// ---------------------------------------------------------------------------------------------------------------
+// Single tokens: S <- lambda S + k v^T, y = scale q^T S.
+//
+// Bound by the state, D Dv fp32 values read and written once for each head and row.  A block takes 32 columns of one
+// state (128-byte rows): 8 threads across with 4 columns each, 16 rows at a time, so that a single row of 12 heads
+// still spreads over 24 blocks at Dv = 64; each thread issues kStepAhead loads before it uses the first.
+// ---------------------------------------------------------------------------------------------------------------
+struct LaStepParams {
+  const void *q, *k, *v;
+  void* y;
+  float* state;
+  const int* slots;
+  const float* ld;
+  long long qs[2], ks[2], vs[2], ys[2], ss;   // row, head; state: slot
+  int B, H, kv_div, D, Dv, pool;
+  float scale;
+};
+
+constexpr int kStepThreads = 128, kStepCols = 32, kStepAhead = 8;
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(kStepThreads) la_step_kernel(const __grid_constant__ LaStepParams prm) {
+  constexpr int TX = kStepCols / VEC, TY = kStepThreads / TX;
+  __shared__ float part[TY][kStepCols];
+  const int bh = blockIdx.x, b = bh / prm.H, h = bh % prm.H;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int c = blockIdx.y * kStepCols + tx * VEC;
+  const bool in = c < prm.Dv;   // VEC 4: Dv is a multiple of 4
+  const int slot = prm.slots ? prm.slots[b] : b;
+  const bool ok = slot >= 0 && slot < prm.pool;
+  const T* q = (const T*)prm.q + b * prm.qs[0] + h * prm.qs[1];
+  const T* k = (const T*)prm.k + b * prm.ks[0] + (h / prm.kv_div) * prm.ks[1];
+  const T* v = (const T*)prm.v + b * prm.vs[0] + (h / prm.kv_div) * prm.vs[1];
+  float* S = prm.state + (ok ? slot : 0) * prm.ss + (long long)h * prm.D * prm.Dv + c;
+  const float lam = LaDecay(prm.ld[h]).pow(1);
+  float vv[VEC], acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; e++) vv[e] = in ? ldf(v + c + e) : 0.f, acc[e] = 0.f;
+  // Rows that name a slot again after an earlier row of the call leave it alone: the first one alone updates it.
+  int again = 0;
+  if (prm.slots)
+    for (int r = threadIdx.x; r < b; r += kStepThreads) again |= prm.slots[r] == slot;
+  const bool act = !__syncthreads_or(again) && ok;
+  if (act && in) {
+    for (int d0 = ty; d0 < prm.D; d0 += TY * kStepAhead) {
+      float s[kStepAhead][VEC];
+#pragma unroll
+      for (int a = 0; a < kStepAhead; a++) {
+        const int d = d0 + a * TY;
+        if (d >= prm.D) continue;
+        if constexpr (VEC == 4) {
+          const float4 x = *(const float4*)(S + (long long)d * prm.Dv);
+          s[a][0] = x.x, s[a][1] = x.y, s[a][2] = x.z, s[a][3] = x.w;
+        } else {
+          s[a][0] = S[(long long)d * prm.Dv];
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < kStepAhead; a++) {
+        const int d = d0 + a * TY;
+        if (d >= prm.D) continue;
+        const float kd = ldf(k + d), qd = ldf(q + d);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          s[a][e] = fmaf(lam, s[a][e], kd * vv[e]);
+          acc[e] = fmaf(qd, s[a][e], acc[e]);
+        }
+        if constexpr (VEC == 4) *(float4*)(S + (long long)d * prm.Dv) = make_float4(s[a][0], s[a][1], s[a][2], s[a][3]);
+        else S[(long long)d * prm.Dv] = s[a][0];
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; e++) part[ty][tx * VEC + e] = acc[e];
+  __syncthreads();
+  const int col = threadIdx.x, cc = blockIdx.y * kStepCols + col;
+  if (col < kStepCols && cc < prm.Dv) {
+    float z = 0.f;
+#pragma unroll
+    for (int r = 0; r < TY; r++) z += part[r][col];
+    stf((T*)prm.y + b * prm.ys[0] + h * prm.ys[1] + cc, prm.scale * z);
+  }
+}
+
+// Sum over the query heads that share a key and value head, in head order: out[b][g][t] = sum_r w[b][g R + r][t].
+struct LaReduceParams {
+  const float* w;   // [B][G R][L][D]
+  void* out;
+  long long os[3];
+  int B, G, R, L, D;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) la_reduce_kernel(const __grid_constant__ LaReduceParams p) {
+  const long long total = (long long)p.B * p.G * p.L * p.D, plane = (long long)p.L * p.D;
+  for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+    const long long bg = e / plane, at = e % plane, t = at / p.D, d = at % p.D, b = bg / p.G, g = bg % p.G;
+    const float* w = p.w + bg * p.R * plane + at;
+    float s = 0.f;
+    for (int r = 0; r < p.R; r++) s += w[r * plane];
+    stf((T*)p.out + b * p.os[0] + g * p.os[1] + t * p.os[2] + d, s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Planning
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kMaxSegments = 32;
+
+struct DeviceFacts {
+  int sms = 0, ok = 0;
+};
+
+cudaError_t device_facts(int device, DeviceFacts* f) {
+  int major = 0, minor = 0;
+  cudaError_t ce = cudaDeviceGetAttribute(&f->sms, cudaDevAttrMultiProcessorCount, device);
+  if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+  if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
+  f->ok = major == 10 && minor == 0;
+  return ce;
+}
+
+// Segments for the general kernel: enough blocks to give every SM two, each of at least four chunks (the first launch
+// and the sum of earlier states cost about one chunk).
+void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
+  const int chunk = la_general_chunk(D);
+  const long long base = (long long)B * H * ((Dv + 63) / 64) * ntask;
+  const long long chunks = ((long long)L + chunk - 1) / chunk;
+  long long g = (2ll * sms + base - 1) / base;
+  if (g > chunks / 4) g = chunks / 4;
+  if (g > kMaxSegments) g = kMaxSegments;
+  if (g < 1) g = 1;
+  const long long per = (chunks + g - 1) / g;
+  *seg = (int)(per < 1 ? chunk : per * chunk);
+  *G = chunks ? (int)((chunks + per - 1) / per) : 1;
+}
+
+struct Sizes {
+  size_t loc[kLaMaxTasks], grad_k, grad_v, total;
+};
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+bool bad_shape(const sffft_linear_attention_t* p) {
+  return !p || p->B < 0 || p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0 || p->L < 0 || p->D < 1 || p->Dv < 1 ||
+         (p->io != SFFFT_IO_FP32 && p->io != SFFFT_IO_BF16) || p->device < 0 || !std::isfinite(p->scale) || p->scale == 0.f;
+}
+
+int too_large(const sffft_linear_attention_t* p) {
+  if (p->D > 256 || p->Dv > 4096) return 1;
+  return (long long)p->B * p->H * kMaxSegments > INT_MAX || p->L > INT_MAX - 4096;
+}
+
+Sizes sizes(const sffft_linear_attention_t* p, int backward, int G) {
+  Sizes s = {};
+  const size_t bh = (size_t)p->B * p->H, st = bh * (size_t)p->D * p->Dv * 4;
+  for (int i = 0; i < (backward ? 3 : 1); i++) {
+    s.loc[i] = G > 1 ? up256(st * G) : 0;
+    s.total += s.loc[i];
+  }
+  if (backward && p->Hkv < p->H) {
+    s.grad_k = up256(bh * p->L * (size_t)p->D * 4);
+    s.grad_v = up256(bh * p->L * (size_t)p->Dv * 4);
+    s.total += s.grad_k + s.grad_v;
+  }
+  return s;
+}
+
+void plan(const sffft_linear_attention_t* p, int backward, int sms, int* G, int* seg) {
+  const int D = backward ? (p->D > p->Dv ? p->D : p->Dv) : p->D, Dv = backward ? D : p->Dv;
+  plan_general(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
+}
+
+template <class T>
+void copy3(long long (&d)[3], const T* s) {
+  for (int i = 0; i < 3; i++) d[i] = s[i];
+}
+
+// Element strides of a contiguous state [B][H][D][Dv], or of its transposed use.
+void state_strides(long long (&s)[4], const sffft_linear_attention_t* p, bool transposed) {
+  const long long n = (long long)p->D * p->Dv;
+  s[0] = p->H * n;
+  s[1] = n;
+  s[2] = transposed ? 1 : p->Dv;
+  s[3] = transposed ? p->Dv : 1;
+}
+
+int common_checks(const sffft_linear_attention_t* p, const void* log_decay) {
+  if (bad_shape(p) || !log_decay) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (too_large(p)) return SFFFT_ERR_UNSUPPORTED;
+  return SFFFT_OK;
+}
+
+int start(const sffft_linear_attention_t* p, DeviceFacts* f) {
+  const cudaError_t ce = device_facts(p->device, f);
+  if (ce != cudaSuccess) return sffft_note_cuda_error(ce);
+  return f->ok ? SFFFT_OK : SFFFT_ERR_DEVICE;
+}
+
+template <class T>
+cudaError_t reduce_t(const LaReduceParams& r, int sms, cudaStream_t st) {
+  const long long total = (long long)r.B * r.G * r.L * r.D;
+  if (total == 0) return cudaSuccess;
+  long long blocks = (total + 255) / 256;
+  if (blocks > 16ll * sms) blocks = 16ll * sms;
+  return launch(la_reduce_kernel<T>, dim3((unsigned)blocks), 256, 0, st, r);
+}
+
+}  // namespace
+}  // namespace sffft
+
+using namespace sffft;
+
+extern "C" {
+
+int sffft_linear_attention_workspace_bytes(const sffft_linear_attention_t* p, int backward, size_t* bytes) {
+  if (bad_shape(p) || !bytes) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (too_large(p)) return SFFFT_ERR_UNSUPPORTED;
+  *bytes = 0;
+  if (p->B == 0) return SFFFT_OK;
+  DeviceFacts f;
+  const int rc = start(p, &f);
+  if (rc) return rc;
+  int G, seg;
+  plan(p, backward, f.sms, &G, &seg);
+  *bytes = sizes(p, backward, G).total;
+  return SFFFT_OK;
+}
+
+int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, const void* k, const void* v,
+                           const float* log_decay, const int* lengths, const float* initial_state, void* y,
+                           float* final_state, void* work, size_t work_bytes, void* stream) {
+  int rc = common_checks(p, log_decay);
+  if (rc) return rc;
+  if (p->B == 0) return SFFFT_OK;
+  if (p->L > 0 && (!q || !k || !v || !y)) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  DeviceFacts f;
+  if ((rc = start(p, &f))) return rc;
+  LaParams prm = {};
+  plan(p, 0, f.sms, &prm.G, &prm.seg);
+  const Sizes sz = sizes(p, 0, prm.G);
+  if (sz.total && (!work || work_bytes < sz.total)) return SFFFT_ERR_WORKSPACE;
+  prm.ld = log_decay; prm.len = lengths;
+  prm.ntask = 1; prm.B = p->B; prm.H = p->H; prm.L = p->L; prm.sms = f.sms;
+  LaTask& t = prm.task[0];
+  t.q = q; t.k = k; t.v = v; t.y = y;
+  copy3(t.qs, p->q_stride); copy3(t.ks, p->k_stride); copy3(t.vs, p->v_stride); copy3(t.ys, p->y_stride);
+  t.qdiv = 1; t.kdiv = t.vdiv = p->H / p->Hkv;
+  t.s0 = initial_state; t.s0_mul = 1.f; state_strides(t.s0s, p, false);
+  t.s1 = final_state; t.s1_mul = 1.f; state_strides(t.s1s, p, false);
+  t.loc = (float*)work;
+  t.D = p->D; t.Dv = p->Dv; t.scale = p->scale;
+  DeviceScope scope(p->device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  const cudaError_t ce = launch_la_general(prm, p->io == SFFFT_IO_BF16, (cudaStream_t)stream);
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sffft_linear_attention_grads_t* g,
+                                    const void* q, const void* k, const void* v, const float* log_decay,
+                                    const int* lengths, const float* initial_state, const void* dy,
+                                    const float* dfinal_state, void* dq, void* dk, void* dv, float* dinitial_state,
+                                    void* work, size_t work_bytes, void* stream) {
+  int rc = common_checks(p, log_decay);
+  if (rc) return rc;
+  if (!g) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (p->Dv > 256) return SFFFT_ERR_UNSUPPORTED;   // v takes the place of q in two of the three passes
+  if (p->B == 0) return SFFFT_OK;
+  if (p->L > 0 && (!q || !k || !v || !dy || !dq || !dk || !dv)) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  DeviceFacts f;
+  if ((rc = start(p, &f))) return rc;
+  LaParams prm = {};
+  plan(p, 1, f.sms, &prm.G, &prm.seg);
+  const Sizes sz = sizes(p, 1, prm.G);
+  if (sz.total && (!work || work_bytes < sz.total)) return SFFFT_ERR_WORKSPACE;
+  prm.ld = log_decay; prm.len = lengths;
+  prm.ntask = 3; prm.B = p->B; prm.H = p->H; prm.L = p->L; prm.sms = f.sms;
+  char* w = (char*)work;
+  for (int i = 0; i < 3; i++) {
+    prm.task[i].loc = (float*)w;
+    prm.task[i].scale = p->scale;
+    prm.task[i].s0_mul = prm.task[i].s1_mul = 1.f;
+    w += sz.loc[i];
+  }
+  const int share = p->H / p->Hkv;
+  float *wk = (float*)w, *wv = (float*)(w + sz.grad_k);
+  LaTask& a = prm.task[0];   // dq
+  a.q = dy; a.k = v; a.v = k; a.y = dq;
+  copy3(a.qs, g->dy_stride); copy3(a.ks, p->v_stride); copy3(a.vs, p->k_stride); copy3(a.ys, g->dq_stride);
+  a.qdiv = 1; a.kdiv = a.vdiv = share;
+  a.s0 = initial_state; state_strides(a.s0s, p, true);
+  a.D = p->Dv; a.Dv = p->D;
+  LaTask& c = prm.task[1];   // dk
+  c.q = v; c.k = dy; c.v = q;
+  copy3(c.qs, p->v_stride); copy3(c.ks, g->dy_stride); copy3(c.vs, p->q_stride);
+  c.qdiv = share; c.kdiv = c.vdiv = 1;
+  c.s0 = dfinal_state; c.s0_mul = 1.f / p->scale; state_strides(c.s0s, p, true);
+  c.D = p->Dv; c.Dv = p->D; c.rev = c.off = 1;
+  LaTask& e = prm.task[2];   // dv and the start state's gradient
+  e.q = k; e.k = q; e.v = dy;
+  copy3(e.qs, p->k_stride); copy3(e.ks, p->q_stride); copy3(e.vs, g->dy_stride);
+  e.qdiv = share; e.kdiv = e.vdiv = 1;
+  e.s0 = dfinal_state; e.s0_mul = 1.f / p->scale; state_strides(e.s0s, p, false);
+  e.s1 = dinitial_state; e.s1_mul = p->scale; e.s1_decay = 1; state_strides(e.s1s, p, false);
+  e.D = p->D; e.Dv = p->Dv; e.rev = e.off = 1;
+  if (share > 1) {   // a gradient for each query head in fp32, then their sum
+    const long long hk[3] = {(long long)p->H * p->L * p->D, (long long)p->L * p->D, p->D};
+    const long long hv[3] = {(long long)p->H * p->L * p->Dv, (long long)p->L * p->Dv, p->Dv};
+    c.y = wk; c.y_f32 = 1; copy3(c.ys, hk);
+    e.y = wv; e.y_f32 = 1; copy3(e.ys, hv);
+  } else {
+    c.y = dk; copy3(c.ys, g->dk_stride);
+    e.y = dv; copy3(e.ys, g->dv_stride);
+  }
+  DeviceScope scope(p->device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  const bool bf = p->io == SFFFT_IO_BF16;
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t ce = launch_la_general(prm, bf, st);
+  if (ce == cudaSuccess && share > 1) {
+    LaReduceParams r = {wk, dk, {}, p->B, p->Hkv, share, p->L, p->D};
+    copy3(r.os, g->dk_stride);
+    ce = bf ? reduce_t<__nv_bfloat16>(r, f.sms, st) : reduce_t<float>(r, f.sms, st);
+    if (ce == cudaSuccess) {
+      r.w = wv; r.out = dv; r.D = p->Dv;
+      copy3(r.os, g->dv_stride);
+      ce = bf ? reduce_t<__nv_bfloat16>(r, f.sms, st) : reduce_t<float>(r, f.sms, st);
+    }
+  }
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const void* q, const void* k, const void* v,
+                                const float* log_decay, float* state, const int* slots, void* y, void* stream) {
+  if (!p || p->B < 0 || p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0 || p->D < 1 || p->Dv < 1 || p->pool < 0 ||
+      (p->io != SFFFT_IO_FP32 && p->io != SFFFT_IO_BF16) || p->device < 0 || !std::isfinite(p->scale))
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!slots && p->pool < p->B) return SFFFT_ERR_INVALID_ARGUMENT;
+  if ((long long)p->B * p->H > INT_MAX || (long long)p->D * p->Dv > INT_MAX || p->Dv > 32 * 65535) return SFFFT_ERR_UNSUPPORTED;
+  if (p->B == 0) return SFFFT_OK;
+  if (!q || !k || !v || !log_decay || !state || !y) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)state & 3) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  DeviceFacts f;
+  const cudaError_t fe = device_facts(p->device, &f);
+  if (fe != cudaSuccess) return sffft_note_cuda_error(fe);
+  if (!f.ok) return SFFFT_ERR_DEVICE;
+  LaStepParams s = {q, k, v, y, state, slots, log_decay, {}, {}, {}, {}, p->state_stride,
+                    p->B, p->H, p->H / p->Hkv, p->D, p->Dv, p->pool, p->scale};
+  for (int i = 0; i < 2; i++) {
+    s.qs[i] = p->q_stride[i]; s.ks[i] = p->k_stride[i]; s.vs[i] = p->v_stride[i]; s.ys[i] = p->y_stride[i];
+  }
+  DeviceScope scope(p->device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  const dim3 grid((unsigned)(p->B * p->H), (unsigned)((p->Dv + kStepCols - 1) / kStepCols));
+  const bool vec = p->Dv % 4 == 0 && p->state_stride % 4 == 0 && ((uintptr_t)state & 15) == 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t ce;
+  if (p->io == SFFFT_IO_BF16)
+    ce = vec ? launch(la_step_kernel<__nv_bfloat16, 4>, grid, kStepThreads, 0, st, s)
+             : launch(la_step_kernel<__nv_bfloat16, 1>, grid, kStepThreads, 0, st, s);
+  else
+    ce = vec ? launch(la_step_kernel<float, 4>, grid, kStepThreads, 0, st, s)
+             : launch(la_step_kernel<float, 1>, grid, kStepThreads, 0, st, s);
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+}  // extern "C"

@@ -1,0 +1,70 @@
+// Linear attention with a decay for each head: the problem as its kernels see it.
+//
+//   S_n = lambda S_{n-1} + k_n v_n^T,   y_n = scale * q_n^T S_n          (S_0 given or zero)
+//
+// The backward pass is the same recurrence on other operands, so one description ("task") serves all of it:
+//   dq_n = scale * dy_n^T (S_n)^T          forward in time,  (q, k, v) <- (dy, v, k), start S_0^T
+//   dk_n = scale * v_n^T R_n^T             backward in time, (q, k, v) <- (v, dy, q), start dS_L^T / scale
+//   dv_n = scale * k_n^T R_n               backward in time, (q, k, v) <- (k, q, dy), start dS_L / scale
+// with R_n = lambda R_{n+1} + q_n dy_n^T, R_{L+1} = dS_L / (scale * lambda), and dS_0 = scale * lambda * R_1.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sffft {
+
+struct LaTask {
+  const void *q, *k, *v;
+  void* y;
+  long long qs[3], ks[3], vs[3], ys[3];   // element strides: row, head, position; a head's values are contiguous
+  int qdiv, kdiv, vdiv;                   // head h reads head h / div of the tensor
+  const float* s0;                        // start state (may be null), element (b, h, d, e) at s0s
+  long long s0s[4];
+  float s0_mul;
+  float* s1;                              // end state (may be null)
+  long long s1s[4];
+  float s1_mul;
+  int s1_decay;                           // the end state takes one more factor lambda (where there is a token)
+  float* loc;                             // G > 1: state that each segment alone leaves, [B*H][G][D][Dv]
+  int D, Dv;
+  int rev;                                // tokens are taken from the last one to the first
+  int off;                                // the first token takes the start state as it is, without a factor lambda
+  int y_f32;                              // y is fp32 whatever the type of q, k, v
+  float scale;
+};
+
+constexpr int kLaMaxTasks = 3;
+
+struct LaParams {
+  LaTask task[kLaMaxTasks];
+  const float* ld;   // natural logarithm of lambda, [H]
+  const int* len;    // tokens of each row (null: L)
+  int ntask, B, H, L;
+  int G, seg;        // segments that the positions are cut into, and positions in each
+  int sms;
+};
+
+// lambda^n from log2(lambda) held as the sum hi + lo of two floats: hi * n is split exactly, so that the error is
+// that of one exp2f, not of |hi * n| roundings.
+struct LaDecay {
+  float hi, lo;
+  __device__ __forceinline__ explicit LaDecay(float ld) {
+    const double l2 = (double)ld * 1.4426950408889634074;
+    hi = (float)l2;
+    lo = isinf(hi) ? 0.f : (float)(l2 - (double)hi);
+  }
+  __device__ __forceinline__ float pow(int n) const {
+    if (n <= 0) return 1.f;
+    const float x = (float)n, p = hi * x;
+    if (p < -160.f) return 0.f;   // below the smallest float (also lambda = 0, where p is -inf)
+    const float e = fmaf(hi, x, -p) + lo * x;
+    return exp2f(p) * fmaf(e, 0.69314718f, 1.f);
+  }
+};
+
+// fp32 on CUDA cores: any type, strides and head sizes up to 256 (launches: G > 1 two, else one).
+cudaError_t launch_la_general(const LaParams& prm, bool bf16, cudaStream_t st);
+// positions in a chunk of the general kernel for head sizes up to dmax
+inline int la_general_chunk(int dmax) { return dmax > 128 ? 32 : 64; }
+
+}  // namespace sffft

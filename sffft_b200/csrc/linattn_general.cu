@@ -1,0 +1,251 @@
+// Linear attention with a decay for each head, fp32 arithmetic on CUDA cores.
+//
+// A block takes one head of one row, up to 64 columns of v and one segment of positions, C at a time.  With P the
+// C x C products q_i . k_j times lambda^(i-j) for j <= i, and S the state before the chunk (D x 64, in shared memory):
+//   y_i = scale * (sum_j P_ij v_j + lambda^(i+1) q_i^T S),   S <- lambda^C S + sum_j lambda^(C-1-j) k_j v_j^T
+// so that a token costs 2 C (D + 64) + 4 * 64 D flop instead of L (D + 64).
+//
+// Few heads and a long row leave most SMs idle, so the positions are then cut into G segments: a first launch leaves
+// the state that each segment builds from zero, and a block of the main launch starts from the sum of the earlier
+// ones (in segment order, so results do not depend on scheduling).  Its price is a second reading of k and v.
+//
+// Time reversal (the gradients of k and v) is a matter of addressing: processing position p reads token n-1-p.
+#include <cuda_bf16.h>
+
+#include "launch.h"
+#include "linattn.h"
+
+namespace sffft {
+namespace {
+
+constexpr int kCols = 64;   // columns of v in a block
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f(float& d, float x) { d = x; }
+__device__ __forceinline__ void from_f(__nv_bfloat16& d, float x) { d = __float2bfloat16_rn(x); }
+
+template <int DM, int C>
+struct GeneralSmem {
+  static constexpr int PT = C + 4;   // pitch of the [d][token] images: a multiple of 4, and 4-way conflicts at worst
+  static constexpr int bytes = 4 * (2 * DM * PT + C * kCols + C * PT + DM * kCols + C + 4);
+};
+
+template <class T, int DM, int C, bool LOCAL>
+__global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_constant__ LaParams prm) {
+  constexpr int PT = GeneralSmem<DM, C>::PT, TI = C / 16;
+  extern __shared__ __align__(16) float sm[];
+  float* Qt = sm;                  // [DM][PT]
+  float* Kt = Qt + DM * PT;        // [DM][PT]
+  float* V = Kt + DM * PT;         // [C][kCols]
+  float* Pt = V + C * kCols;       // [C][PT], transposed: Pt[j][i]
+  float* S = Pt + C * PT;          // [DM][kCols]
+  float* pw = S + DM * kCols;      // lambda^0 .. lambda^C
+  const LaTask& tk = prm.task[blockIdx.z];
+  const int D = tk.D, Dv = tk.Dv, c0 = blockIdx.y * kCols;
+  if (c0 >= Dv) return;
+  const int g = blockIdx.x % prm.G, bh = blockIdx.x / prm.G, b = bh / prm.H, h = bh % prm.H;
+  if (LOCAL && g == prm.G - 1) return;   // nothing follows the last segment
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  int n = prm.L;
+  if (prm.len) n = min(max(prm.len[b], 0), prm.L);
+  const int ps = min(g * prm.seg, n), pe = min((g + 1) * prm.seg, n);
+  const LaDecay dec(prm.ld[h]);
+  for (int i = tid; i <= C; i += kThreads) pw[i] = dec.pow(i);
+
+  const T* q = (const T*)tk.q + b * tk.qs[0] + (h / tk.qdiv) * tk.qs[1];
+  const T* k = (const T*)tk.k + b * tk.ks[0] + (h / tk.kdiv) * tk.ks[1];
+  const T* v = (const T*)tk.v + b * tk.vs[0] + (h / tk.vdiv) * tk.vs[1];
+  const long long ybase = b * tk.ys[0] + h * tk.ys[1];
+
+  // state before the segment
+  const float* loc = LOCAL ? nullptr : tk.loc + (long long)bh * prm.G * D * Dv;
+  for (int e = tid; e < DM * kCols; e += kThreads) {
+    const int d = e / kCols, c = c0 + e % kCols;
+    float s = 0.f;
+    if (!LOCAL && d < D && c < Dv) {
+      for (int gg = 0; gg < g; gg++) {
+        const int m = min((gg + 1) * prm.seg, n) - min(gg * prm.seg, n);
+        if (m > 0) s = fmaf(dec.pow(m), s, loc[((long long)gg * D + d) * Dv + c]);
+      }
+      if (tk.s0) {
+        const float z = tk.s0[b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + c * tk.s0s[3]] * tk.s0_mul;
+        s = fmaf(dec.pow(ps - (tk.off && ps > 0)), z, s);
+      }
+    }
+    S[e] = s;
+  }
+  __syncthreads();
+
+  for (int p0 = ps; p0 < pe; p0 += C) {
+    const int m = min(C, pe - p0);
+    const int off = (tk.off && p0 == 0) ? 1 : 0;
+    for (int e = tid; e < DM * C; e += kThreads) {
+      const int d = e % DM, i = e / DM;
+      float a = 0.f, c = 0.f;
+      if (i < m && d < D) {
+        const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
+        if (!LOCAL) a = to_f(q[t * tk.qs[2] + d]);
+        c = to_f(k[t * tk.ks[2] + d]);
+      }
+      if (!LOCAL) Qt[d * PT + i] = a;
+      Kt[d * PT + i] = LOCAL ? c * pw[max(m - 1 - i, 0)] : c;
+    }
+    for (int e = tid; e < C * kCols; e += kThreads) {
+      const int i = e / kCols, c = c0 + e % kCols;
+      float a = 0.f;
+      if (i < m && c < Dv) {
+        const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
+        a = to_f(v[t * tk.vs[2] + c]);
+      }
+      V[e] = a;
+    }
+    __syncthreads();
+    if (!LOCAL) {
+      {
+        float acc[TI][TI] = {};
+        for (int d = 0; d < D; d++) {
+          float a[TI], c[TI];
+#pragma unroll
+          for (int x = 0; x < TI; x++) a[x] = Qt[d * PT + ty * TI + x], c[x] = Kt[d * PT + tx * TI + x];
+#pragma unroll
+          for (int x = 0; x < TI; x++)
+#pragma unroll
+            for (int y = 0; y < TI; y++) acc[x][y] = fmaf(a[x], c[y], acc[x][y]);
+        }
+#pragma unroll
+        for (int y = 0; y < TI; y++)
+#pragma unroll
+          for (int x = 0; x < TI; x++) {
+            const int i = ty * TI + x, j = tx * TI + y;
+            Pt[j * PT + i] = i >= j ? acc[x][y] * pw[max(i - j, 0)] : 0.f;
+          }
+      }
+      __syncthreads();
+      float o[TI][4] = {}, r[TI][4] = {};
+      for (int j = 0; j < m; j++) {
+        float a[TI], c[4];
+#pragma unroll
+        for (int x = 0; x < TI; x++) a[x] = Pt[j * PT + ty * TI + x];
+#pragma unroll
+        for (int y = 0; y < 4; y++) c[y] = V[j * kCols + tx * 4 + y];
+#pragma unroll
+        for (int x = 0; x < TI; x++)
+#pragma unroll
+          for (int y = 0; y < 4; y++) o[x][y] = fmaf(a[x], c[y], o[x][y]);
+      }
+      for (int d = 0; d < D; d++) {
+        float a[TI], c[4];
+#pragma unroll
+        for (int x = 0; x < TI; x++) a[x] = Qt[d * PT + ty * TI + x];
+#pragma unroll
+        for (int y = 0; y < 4; y++) c[y] = S[d * kCols + tx * 4 + y];
+#pragma unroll
+        for (int x = 0; x < TI; x++)
+#pragma unroll
+          for (int y = 0; y < 4; y++) r[x][y] = fmaf(a[x], c[y], r[x][y]);
+      }
+#pragma unroll
+      for (int x = 0; x < TI; x++) {
+        const int i = ty * TI + x;
+        if (i >= m) continue;
+        const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
+        const float w = pw[i + 1 - off];
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const int c = c0 + tx * 4 + y;
+          if (c >= Dv) continue;
+          const float z = tk.scale * fmaf(w, r[x][y], o[x][y]);
+          const long long at = ybase + t * tk.ys[2] + c;
+          if (tk.y_f32) ((float*)tk.y)[at] = z;
+          else from_f(((T*)tk.y)[at], z);
+        }
+      }
+      __syncthreads();
+      for (int e = tid; e < DM * C; e += kThreads) Kt[(e % DM) * PT + e / DM] *= pw[max(m - 1 - e / DM, 0)];
+      __syncthreads();
+    }
+    const float ws = pw[m - off];
+    for (int d0 = ty * 4; d0 < D; d0 += 64) {
+      float acc[4][4];
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) acc[x][y] = 0.f;
+      for (int j = 0; j < m; j++) {
+        float a[4], c[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) a[x] = Kt[(d0 + x) * PT + j];
+#pragma unroll
+        for (int y = 0; y < 4; y++) c[y] = V[j * kCols + tx * 4 + y];
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+          for (int y = 0; y < 4; y++) acc[x][y] = fmaf(a[x], c[y], acc[x][y]);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          float& s = S[(d0 + x) * kCols + tx * 4 + y];
+          s = fmaf(ws, s, acc[x][y]);
+        }
+    }
+    __syncthreads();
+  }
+
+  if (LOCAL) {
+    float* out = tk.loc + ((long long)bh * prm.G + g) * D * Dv;
+    for (int e = tid; e < DM * kCols; e += kThreads) {
+      const int d = e / kCols, c = c0 + e % kCols;
+      if (d < D && c < Dv) out[(long long)d * Dv + c] = S[e];
+    }
+    return;
+  }
+  if (tk.s1 && g == prm.G - 1) {
+    const float w = tk.s1_mul * (tk.s1_decay && n > 0 ? pw[1] : 1.f);
+    for (int e = tid; e < DM * kCols; e += kThreads) {
+      const int d = e / kCols, c = c0 + e % kCols;
+      if (d < D && c < Dv) tk.s1[b * tk.s1s[0] + h * tk.s1s[1] + d * tk.s1s[2] + c * tk.s1s[3]] = w * S[e];
+    }
+  }
+  // positions behind the row's last token
+  const int z0 = max(g * prm.seg, n), z1 = min((g + 1) * prm.seg, prm.L);
+  for (long long e = tid; e < (long long)(z1 - z0) * kCols; e += kThreads) {
+    const long long t = z0 + e / kCols;
+    const int c = c0 + (int)(e % kCols);
+    if (c >= Dv) continue;
+    const long long at = ybase + t * tk.ys[2] + c;
+    if (tk.y_f32) ((float*)tk.y)[at] = 0.f;
+    else from_f(((T*)tk.y)[at], 0.f);
+  }
+}
+
+template <class T, int DM, int C>
+cudaError_t launch_t(const LaParams& prm, int dv_max, cudaStream_t st) {
+  const dim3 grid((unsigned)(prm.B * prm.H * prm.G), (unsigned)((dv_max + kCols - 1) / kCols), (unsigned)prm.ntask);
+  constexpr int bytes = GeneralSmem<DM, C>::bytes;
+  if (prm.G > 1) {
+    const cudaError_t ce = launch(la_general_kernel<T, DM, C, true>, grid, kThreads, bytes, st, prm);
+    if (ce != cudaSuccess) return ce;
+  }
+  return launch(la_general_kernel<T, DM, C, false>, grid, kThreads, bytes, st, prm);
+}
+
+template <class T>
+cudaError_t launch_d(const LaParams& prm, cudaStream_t st) {
+  int d = 0, dv = 0;
+  for (int i = 0; i < prm.ntask; i++) d = max(d, prm.task[i].D), dv = max(dv, prm.task[i].Dv);
+  if (d <= 64) return launch_t<T, 64, 64>(prm, dv, st);
+  if (d <= 128) return launch_t<T, 128, 64>(prm, dv, st);
+  return launch_t<T, 256, 32>(prm, dv, st);
+}
+
+}  // namespace
+
+cudaError_t launch_la_general(const LaParams& prm, bool bf16, cudaStream_t st) {
+  return bf16 ? launch_d<__nv_bfloat16>(prm, st) : launch_d<float>(prm, st);
+}
+
+}  // namespace sffft

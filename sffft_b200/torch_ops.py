@@ -9,10 +9,14 @@
     X = torch.ops.sffft.rfft(x)                        # x [..., N] fp32/bf16 -> X [..., N/2+1] complex64
     x = torch.ops.sffft.irfft(X)                       # X [..., N/2+1] complex64 -> x [..., N] fp32
 
-Both run on the current CUDA stream of the tensors' device through sffft_filter_spectrum / sffft_conv, so
-they order with surrounding PyTorch work and can be captured in CUDA graphs once a first call has created
-the plan (plan creation allocates).  Fake implementations give output shapes and types without running
-anything, so the operators trace under torch.compile.  Forward only: the path has no backward kernel.
+    y, S = sffft_b200.torch_ops.linear_attention(q, k, v, log_decay)      # prompts and training, with gradients
+    y = sffft_b200.torch_ops.linear_attention_step(q, k, v, log_decay, S) # single tokens, S updated in place
+    h, n = sffft_b200.torch_ops.block_norm(x, y, gate, post_weight, weight)   # norms, gate, residual; with gradients
+
+All run on the current CUDA stream of the tensors' device through the C ABI, so they order with surrounding
+PyTorch work and can be captured in CUDA graphs once a first call has created the plan (plan creation allocates).  Fake implementations give output shapes and types without running
+anything, so the operators trace under torch.compile.  The convolution and the FFTs are forward only (the path has
+no backward kernel); linear_attention and block_norm have first derivatives.
 
 `acc` is "fp32" or "fp16" (accumulation mode); `config` names a catalog plan ("" = the default for L).
 filter_spectrum and conv must use the same config: the spectrum is in that plan's digit order.
@@ -20,6 +24,7 @@ filter_spectrum and conv must use the same config: the spectrum is in that plan'
 fused kernel is the same for all three.
 """
 import threading
+from typing import Optional
 
 import torch
 from torch import Tensor
@@ -147,3 +152,170 @@ def irfft(X: Tensor, config: str = "") -> Tensor:
 @irfft.register_fake
 def _(X: Tensor, config: str = "") -> Tensor:
     return X.new_empty(tuple(X.shape[:-1]) + (2 * (X.shape[-1] - 1),), dtype=torch.float32)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Linear attention and the norms around a block
+# ---------------------------------------------------------------------------------------------------------------
+
+@torch.library.custom_op("sffft::linear_attention", mutates_args=())
+def _linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                      lengths: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor]:
+    return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+
+
+@_linear_attention.register_fake
+def _(q, k, v, log_decay, initial_state, lengths, scale):
+    sf.check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+    B, H, L, D = q.shape
+    return sf._heads_like(q, B, H, L, v.shape[3], q.dtype), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
+
+
+@torch.library.custom_op("sffft::linear_attention_backward", mutates_args=())
+def _linear_attention_backward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                               lengths: Optional[Tensor], scale: float, dy: Tensor,
+                               dfinal_state: Optional[Tensor]) -> list[Tensor]:
+    out = sf.linear_attention_backward(q, k, v, log_decay, dy, dfinal_state, scale, initial_state, lengths)
+    return [t for t in out if t is not None]
+
+
+@_linear_attention_backward.register_fake
+def _(q, k, v, log_decay, initial_state, lengths, scale, dy, dfinal_state):
+    out = [sf._heads_like(t, *t.shape, q.dtype) for t in (q, k, v)]
+    return out if initial_state is None else out + [torch.empty_like(initial_state, memory_format=torch.contiguous_format)]
+
+
+def _la_setup(ctx, inputs, output):
+    q, k, v, log_decay, initial_state, lengths, scale = inputs
+    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+    ctx.scale = scale
+
+
+def _la_backward(ctx, dy, dfinal_state):
+    q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+    if dy is None:
+        dy = q.new_zeros((*q.shape[:3], v.shape[3]))
+    out = torch.ops.sffft.linear_attention_backward(q, k, v, log_decay, initial_state, lengths, ctx.scale, dy, dfinal_state)
+    return out[0], out[1], out[2], None, out[3] if initial_state is not None else None, None, None
+
+
+_linear_attention.register_autograd(_la_backward, setup_context=_la_setup)
+
+
+def _plain_call(*tensors) -> bool:
+    """Whether the call needs neither a gradient nor a trace, so that the operator's dispatch can be left out."""
+    if torch.compiler.is_compiling():
+        return False
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return False
+    return all(t is None or type(t) in (Tensor, torch.nn.Parameter) and t.device.type == "cuda" for t in tensors)
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: float = 1.0,
+                     initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n with lambda = exp(log_decay) for each
+    head (see sffft_b200.linear_attention).  Differentiable in q, k, v and initial_state."""
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is a constant: it has no gradient (pass log_decay.detach())")
+    if _plain_call(q, k, v, log_decay, initial_state, lengths):
+        return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+    return _linear_attention(q, k, v, log_decay, initial_state, lengths, scale)
+
+
+@torch.library.custom_op("sffft::linear_attention_step", mutates_args=("state",))
+def _linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor],
+                           scale: float) -> Tensor:
+    return sf.linear_attention_step(q, k, v, log_decay, state, slots, scale)
+
+
+@_linear_attention_step.register_fake
+def _(q, k, v, log_decay, state, slots, scale):
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor] = None,
+                          scale: float = 1.0) -> Tensor:
+    """One token for each row, state[slot] updated in place (see sffft_b200.linear_attention_step).  No gradient."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise ValueError("linear_attention_step updates its state in place and has no gradient: use linear_attention, or no_grad")
+    if _plain_call(q, k, v, log_decay, state, slots):
+        return sf.linear_attention_step(q, k, v, log_decay, state, slots, scale)
+    return _linear_attention_step(q, k, v, log_decay, state, slots, scale)
+
+
+@torch.library.custom_op("sffft::block_norm", mutates_args=())
+def _block_norm(x: Optional[Tensor], y: Optional[Tensor], gate: Optional[Tensor], post_weight: Optional[Tensor],
+                weight: Optional[Tensor], scale: float, eps: float, groups: int, act: str, dim: int) -> list[Tensor]:
+    """h (with y), n (with weight), then the rstd of y's groups (with post_weight) and of h (with weight)."""
+    h, n, r1, r2 = sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim, stats=True)
+    return [t for t in (None if y is None else h, n, r1, r2) if t is not None]
+
+
+@_block_norm.register_fake
+def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
+    C, _, _ = sf.check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    lead = y if y is not None else x
+    rows = lead.numel() // C
+    out = []
+    if y is not None:
+        out.append(lead.new_empty(lead.shape, dtype=lead.dtype if x is None else x.dtype))
+    if weight is not None:
+        out.append(lead.new_empty(lead.shape))
+    if post_weight is not None:
+        out.append(lead.new_empty((rows, groups), dtype=torch.float32))
+    if weight is not None:
+        out.append(lead.new_empty((rows,), dtype=torch.float32))
+    return out
+
+
+@torch.library.custom_op("sffft::block_norm_backward", mutates_args=())
+def _block_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Optional[Tensor], y: Optional[Tensor],
+                         gate: Optional[Tensor], post_weight: Optional[Tensor], weight: Optional[Tensor],
+                         rstd_post: Optional[Tensor], rstd: Optional[Tensor], scale: float, eps: float, groups: int, act: str,
+                         dim: int) -> list[Tensor]:
+    out = sf.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, scale, eps, groups, act, dim)
+    return [t for t in out if t is not None]
+
+
+@_block_norm_backward.register_fake
+def _(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, scale, eps, groups, act, dim):
+    return [t.new_empty(t.shape) for t in (x, y, gate, post_weight, weight) if t is not None]
+
+
+def _bn_setup(ctx, inputs, output):
+    x, y, gate, post_weight, weight, *rest = inputs
+    ctx.rest = rest
+    kept = list(output)
+    rstd = kept.pop() if weight is not None else None
+    rstd_post = kept.pop() if post_weight is not None else None
+    ctx.save_for_backward(x, y, gate, post_weight, weight, rstd_post, rstd)
+
+
+def _bn_backward(ctx, grads):
+    x, y, gate, post_weight, weight, rstd_post, rstd = ctx.saved_tensors
+    grads = list(grads)
+    lead = y if y is not None else x
+    dh = grads.pop(0) if y is not None else None
+    dn = grads.pop(0) if weight is not None else None
+    if weight is not None and dn is None:
+        dn = lead.new_zeros(lead.shape)
+    if weight is None and dh is None:
+        dh = lead.new_zeros(lead.shape, dtype=lead.dtype if x is None else x.dtype)
+    out = torch.ops.sffft.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, *ctx.rest)
+    out = list(out)
+    return tuple(out.pop(0) if t is not None else None for t in (x, y, gate, post_weight, weight)) + (None,) * 5
+
+
+_block_norm.register_autograd(_bn_backward, setup_context=_bn_setup)
+
+
+def block_norm(x: Optional[Tensor] = None, y: Optional[Tensor] = None, gate: Optional[Tensor] = None,
+               post_weight: Optional[Tensor] = None, weight: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6,
+               groups: int = 1, act: str = "none", dim: int = -1) -> tuple[Tensor, Optional[Tensor]]:
+    """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight: the norms before and after a
+    block with its gate and residual scale (see sffft_b200.block_norm).  Differentiable in all its tensors."""
+    if _plain_call(x, y, gate, post_weight, weight):
+        return sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    out = _block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    h = x if y is None else out[0]
+    return h, None if weight is None else out[0 if y is None else 1]
