@@ -258,6 +258,10 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
                                     const float* dfinal_state, void* dq, void* dk, void* dv, float* dinitial_state,
                                     void* work, size_t work_bytes, void* stream);
 
+/* Waits for the device and returns (and clears) what its linear attention kernels reported: SFFFT_OK, or
+ * SFFFT_ERR_TIMEOUT when a barrier wait of one gave up, and its outputs are not valid. */
+int sffft_linear_attention_check(int device);
+
 /* One token for each of B rows: S <- lambda S + k v^T in place, y = scale * S^T q.  The states lie in a pool of slots
  * of [H][D][Dv] fp32, state_stride elements apart; row b uses slot slots[b] (int32, device), or slot b where slots is
  * NULL.  A row whose slot is not in [0, pool) is padding: it gets y = 0 and no state changes.  The same holds for a row

@@ -117,6 +117,7 @@ def _declare(lib):
         "sffft_linear_attention_workspace_bytes": (I, [V, I, ctypes.POINTER(ctypes.c_size_t)]),
         "sffft_linear_attention": (I, [V] * 10 + [ctypes.c_size_t, V]),
         "sffft_linear_attention_backward": (I, [V] * 15 + [ctypes.c_size_t, V]),
+        "sffft_linear_attention_check": (I, [I]),
         "sffft_linear_attention_step": (I, [V] * 9),
         "sffft_block_norm": (I, [V] * 11),
         "sffft_block_norm_workspace_bytes": (I, [V, ctypes.POINTER(ctypes.c_size_t)]),
@@ -656,6 +657,11 @@ def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1
         0 if work is None else work.numel(), raw), f"linear_attention_backward(q {list(q.shape)}, v {list(v.shape)})")
     _used_on(side, q, k, v, ld, s0, ln, dy, ds1, dq, dk, dv, ds0, work)
     return dq, dk, dv, ds0
+
+
+def linear_attention_check(device: int = 0):
+    """Waits for the device and raises if one of its linear attention kernels reported a device-side error."""
+    _check(lib().sffft_linear_attention_check(device), "device status")
 
 
 def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=1.0, stream=None):

@@ -156,6 +156,27 @@ void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G
   *G = chunks ? (int)((chunks + per - 1) / per) : 1;
 }
 
+// Segments for the tensor-core kernel.  An SM holds two CTAs of head size 64, else one; a CTA's time is that of its
+// chunks one after the other, so cutting pays until the CTAs fill the SMs, and costs a second reading of k and v
+// (half a chunk's work), a launch and the sum of earlier states (together about kCutCost chunks).
+constexpr double kCutCost = 4.0;
+
+void plan_tc(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
+  const long long slots = (long long)sms * (D <= 64 && Dv <= 64 ? 2 : 1), units = (long long)B * H * ntask;
+  const int chunks = (L + kLaTcChunk - 1) / kLaTcChunk;
+  double best = 0;
+  *G = 1;
+  for (int g = 1; g <= kMaxSegments && g <= chunks; g++) {
+    const long long waves = (units * g + slots - 1) / slots;
+    const int per = (chunks + g - 1) / g;
+    const double cost = (double)waves * per * (g > 1 ? 1.5 : 1.0) + (g > 1 ? kCutCost : 0.0);
+    if (g == 1 || cost < best) best = cost, *G = g;
+  }
+  const int per = chunks ? (chunks + *G - 1) / *G : 1;
+  *seg = per * kLaTcChunk;
+  *G = chunks ? (chunks + per - 1) / per : 1;
+}
+
 struct Sizes {
   size_t loc[kLaMaxTasks], grad_k, grad_v, total;
 };
@@ -169,7 +190,7 @@ bool bad_shape(const sffft_linear_attention_t* p) {
 
 int too_large(const sffft_linear_attention_t* p) {
   if (p->D > 256 || p->Dv > 4096) return 1;
-  return (long long)p->B * p->H * kMaxSegments > INT_MAX || p->L > INT_MAX - 4096;
+  return (long long)p->B * p->H * kMaxSegments > INT_MAX || p->L > (1 << 30);
 }
 
 Sizes sizes(const sffft_linear_attention_t* p, int backward, int G) {
@@ -187,9 +208,25 @@ Sizes sizes(const sffft_linear_attention_t* p, int backward, int G) {
   return s;
 }
 
-void plan(const sffft_linear_attention_t* p, int backward, int sms, int* G, int* seg) {
+void plan(const sffft_linear_attention_t* p, int backward, bool tc, int sms, int* G, int* seg) {
   const int D = backward ? (p->D > p->Dv ? p->D : p->Dv) : p->D, Dv = backward ? D : p->Dv;
-  plan_general(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
+  (tc ? plan_tc : plan_general)(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
+}
+
+// Chooses the kernel and the segments, hands out the workspace, and launches.
+int run(const sffft_linear_attention_t* p, int backward, LaParams* prm, const DeviceFacts& f, char* work, size_t work_bytes,
+        cudaStream_t st) {
+  const bool bf = p->io == SFFFT_IO_BF16, tc = bf && la_tc_takes(*prm);
+  plan(p, backward, tc, f.sms, &prm->G, &prm->seg);
+  const Sizes sz = sizes(p, backward, prm->G);
+  const size_t need = sz.total - sz.grad_k - sz.grad_v;
+  if (need && (!work || work_bytes < need)) return SFFFT_ERR_WORKSPACE;
+  for (int i = 0; i < prm->ntask; i++) {
+    prm->task[i].loc = (float*)work;
+    work += sz.loc[i];
+  }
+  const cudaError_t ce = tc ? launch_la_tc(*prm, st) : launch_la_general(*prm, bf, st);
+  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
 }
 
 template <class T>
@@ -242,9 +279,12 @@ int sffft_linear_attention_workspace_bytes(const sffft_linear_attention_t* p, in
   DeviceFacts f;
   const int rc = start(p, &f);
   if (rc) return rc;
-  int G, seg;
-  plan(p, backward, f.sms, &G, &seg);
-  *bytes = sizes(p, backward, G).total;
+  for (int tc = 0; tc < 2; tc++) {   // which kernel runs also depends on the tensors' addresses and strides
+    int G, seg;
+    plan(p, backward, tc != 0, f.sms, &G, &seg);
+    const size_t n = sizes(p, backward, G).total;
+    if (n > *bytes) *bytes = n;
+  }
   return SFFFT_OK;
 }
 
@@ -259,9 +299,6 @@ int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, con
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
-  plan(p, 0, f.sms, &prm.G, &prm.seg);
-  const Sizes sz = sizes(p, 0, prm.G);
-  if (sz.total && (!work || work_bytes < sz.total)) return SFFFT_ERR_WORKSPACE;
   prm.ld = log_decay; prm.len = lengths;
   prm.ntask = 1; prm.B = p->B; prm.H = p->H; prm.L = p->L; prm.sms = f.sms;
   LaTask& t = prm.task[0];
@@ -270,12 +307,10 @@ int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, con
   t.qdiv = 1; t.kdiv = t.vdiv = p->H / p->Hkv;
   t.s0 = initial_state; t.s0_mul = 1.f; state_strides(t.s0s, p, false);
   t.s1 = final_state; t.s1_mul = 1.f; state_strides(t.s1s, p, false);
-  t.loc = (float*)work;
   t.D = p->D; t.Dv = p->Dv; t.scale = p->scale;
   DeviceScope scope(p->device);
   if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
-  const cudaError_t ce = launch_la_general(prm, p->io == SFFFT_IO_BF16, (cudaStream_t)stream);
-  return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+  return run(p, 0, &prm, f, (char*)work, work_bytes, (cudaStream_t)stream);
 }
 
 int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sffft_linear_attention_grads_t* g,
@@ -293,20 +328,17 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
-  plan(p, 1, f.sms, &prm.G, &prm.seg);
-  const Sizes sz = sizes(p, 1, prm.G);
-  if (sz.total && (!work || work_bytes < sz.total)) return SFFFT_ERR_WORKSPACE;
   prm.ld = log_decay; prm.len = lengths;
   prm.ntask = 3; prm.B = p->B; prm.H = p->H; prm.L = p->L; prm.sms = f.sms;
-  char* w = (char*)work;
   for (int i = 0; i < 3; i++) {
-    prm.task[i].loc = (float*)w;
     prm.task[i].scale = p->scale;
     prm.task[i].s0_mul = prm.task[i].s1_mul = 1.f;
-    w += sz.loc[i];
   }
   const int share = p->H / p->Hkv;
-  float *wk = (float*)w, *wv = (float*)(w + sz.grad_k);
+  // the workspace begins with the query heads' gradients, whose size does not depend on the kernel
+  const Sizes whole = sizes(p, 1, 1);
+  if (whole.total && (!work || work_bytes < whole.total)) return SFFFT_ERR_WORKSPACE;
+  float *wk = (float*)work, *wv = (float*)((char*)work + whole.grad_k);
   LaTask& a = prm.task[0];   // dq
   a.q = dy; a.k = v; a.v = k; a.y = dq;
   copy3(a.qs, g->dy_stride); copy3(a.ks, p->v_stride); copy3(a.vs, p->k_stride); copy3(a.ys, g->dq_stride);
@@ -339,8 +371,9 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
   if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
   const bool bf = p->io == SFFFT_IO_BF16;
   const cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t ce = launch_la_general(prm, bf, st);
-  if (ce == cudaSuccess && share > 1) {
+  if ((rc = run(p, 1, &prm, f, (char*)work + whole.total, work_bytes - whole.total, st))) return rc;
+  cudaError_t ce = cudaSuccess;
+  if (share > 1) {
     LaReduceParams r = {wk, dk, {}, p->B, p->Hkv, share, p->L, p->D};
     copy3(r.os, g->dk_stride);
     ce = bf ? reduce_t<__nv_bfloat16>(r, f.sms, st) : reduce_t<float>(r, f.sms, st);
@@ -351,6 +384,15 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
     }
   }
   return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
+}
+
+int sffft_linear_attention_check(int device) {
+  if (device < 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  DeviceScope scope(device);
+  if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
+  int status = 0;
+  const cudaError_t ce = la_tc_status(&status);
+  return ce == cudaSuccess ? status : sffft_note_cuda_error(ce);
 }
 
 int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const void* q, const void* k, const void* v,

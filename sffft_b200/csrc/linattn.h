@@ -60,11 +60,22 @@ struct LaDecay {
     const float e = fmaf(hi, x, -p) + lo * x;
     return exp2f(p) * fmaf(e, 0.69314718f, 1.f);
   }
+  // what the float `r` = pow(n) leaves of lambda^n
+  __device__ __forceinline__ float pow_rest(int n, float r) const {
+    if (n <= 0 || r == 0.f) return 0.f;
+    return (float)(exp2(((double)hi + (double)lo) * n) - (double)r);
+  }
 };
 
 // fp32 on CUDA cores: any type, strides and head sizes up to 256 (launches: G > 1 two, else one).
 cudaError_t launch_la_general(const LaParams& prm, bool bf16, cudaStream_t st);
 // positions in a chunk of the general kernel for head sizes up to dmax
 inline int la_general_chunk(int dmax) { return dmax > 128 ? 32 : 64; }
+
+// bf16 on the tensor cores: head sizes up to 128 in multiples of 8, 16-byte aligned rows (la_tc_takes), any length.
+bool la_tc_takes(const LaParams& prm);
+cudaError_t launch_la_tc(const LaParams& prm, cudaStream_t st);
+cudaError_t la_tc_status(int* status);   // waits for the current device; reads and clears its status word
+constexpr int kLaTcChunk = 128;
 
 }  // namespace sffft

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
   const int ps = min(g * prm.seg, n), pe = min((g + 1) * prm.seg, n);
   const LaDecay dec(prm.ld[h]);
   for (int i = tid; i <= C; i += kThreads) pw[i] = dec.pow(i);
+  const float whole_lo = dec.pow_rest(C, dec.pow(C));
 
   const T* q = (const T*)tk.q + b * tk.qs[0] + (h / tk.qdiv) * tk.qs[1];
   const T* k = (const T*)tk.k + b * tk.ks[0] + (h / tk.kdiv) * tk.ks[1];
@@ -166,7 +167,8 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
       for (int e = tid; e < DM * C; e += kThreads) Kt[(e % DM) * PT + e / DM] *= pw[max(m - 1 - e / DM, 0)];
       __syncthreads();
     }
-    const float ws = pw[m - off];
+    // lambda^C as a sum of two floats: its rounding would come back with every chunk
+    const float ws = pw[m - off], ws_lo = m - off == C ? whole_lo : 0.f;
     for (int d0 = ty * 4; d0 < D; d0 += 64) {
       float acc[4][4];
 #pragma unroll
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
 #pragma unroll
         for (int y = 0; y < 4; y++) {
           float& s = S[(d0 + x) * kCols + tx * 4 + y];
-          s = fmaf(ws, s, acc[x][y]);
+          s = fmaf(ws, s, fmaf(ws_lo, s, acc[x][y]));
         }
     }
     __syncthreads();
