@@ -48,12 +48,13 @@ struct __align__(64) LaTcParams {
 
 template <int DQ, int DV>
 struct Shape {
-  static constexpr int NB = DV / 64;                    // state warpgroups
-  static constexpr int threads = 128 + 128 * NB + 64;
+  static constexpr int NB = DV / 64, NW = DV / 32;      // 64-column tiles of v; state warpgroups, 32 columns each
+  static constexpr int threads = 128 + 128 * NW + 64;
   static constexpr bool alias = DQ == 64 && DV == 64;   // two CTAs on an SM: 256 columns each, O lies in S's upper half
-  static constexpr uint32_t q_bytes = DQ / 64 * kBlk, v_bytes = DV / 64 * kBlk, stage = 2 * q_bytes + v_bytes;
-  static constexpr uint32_t off_s = 2 * stage, off_tab = off_s + NB * kBlk, off_bar = off_tab + 544;
-  static constexpr uint32_t smem = off_bar + 16 * 8 + 16;
+  static constexpr bool out_q = DQ >= DV;               // O is staged where Q was, else where V was
+  static constexpr uint32_t q_bytes = DQ / 64 * kBlk, v_bytes = NB * kBlk, stage = 2 * q_bytes + v_bytes;
+  static constexpr uint32_t off_s = 2 * stage, off_tab = off_s + NB * kBlk, off_bar = off_tab + 4 * 160;
+  static constexpr uint32_t smem = off_bar + 17 * 8 + 8;
   static constexpr uint32_t cols = alias ? 256 : 512;
   // TMEM columns: products Q K^T (P over their first half), O, increment of S, X
   static constexpr uint32_t c_p = 0, c_o = alias ? 64 : 128, c_kv = alias ? 128 : 128 + DV, c_x = c_kv + DV;
@@ -61,7 +62,17 @@ struct Shape {
   static_assert(c_x + x_cols <= cols, "TMEM");
 };
 
-enum { B_FULL0, B_FULL1, B_S, B_P, B_O1, B_OS, B_O, B_OOUT, B_OFREE, B_X, B_KV, B_X2, B_KV2, B_ST, B_FIN, B_COUNT };
+// Barriers; each completes once a chunk (the first two pairs once for every other chunk).
+enum {
+  B_KV0, B_KV1, B_Q0, B_Q1,   // K and V, Q loaded
+  B_S, B_P,                   // products ready; P ready
+  B_O1, B_OS, B_O,            // Q S taken; scaled; O complete
+  B_OOUT, B_OFREE,            // O staged; O's TMEM read
+  B_X, B_INC, B_X2, B_INC2,   // X ready, its product taken; third part ready, its product taken
+  B_ST,                       // S published (once more before the first chunk)
+  B_FIN, B_COUNT
+};
+static_assert(B_COUNT <= 17, "barriers");
 
 __host__ __device__ constexpr uint32_t idesc_bf16(int N, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -123,15 +134,19 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* m, uint32_t src, in
                : "memory");
 }
 
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
+// Four 8 x 8 tiles of 16-bit values, transposed: lane l gives the address of row l % 8 of tile l / 8, and gets of each tile
+// rows 2 (l % 4) and 2 (l % 4) + 1 of column l / 4, in one word.
+__device__ __forceinline__ void ldsm_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
 }
-__device__ __forceinline__ float lds32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
+// 16 lanes x 16 columns: word 2 i + k of lane l goes to TMEM lane 8 k + l / 4, column 4 i + l % 4.
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t t, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -147,8 +162,58 @@ __device__ __forceinline__ float hi_f(uint32_t u) { return __uint_as_float(u & 0
 
 // among the 128 threads of a state warpgroup
 __device__ __forceinline__ void wg_sync(int wg) {
-  if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-  else asm volatile("bar.sync 2, 128;" ::: "memory");
+  switch (wg) {
+    case 0: asm volatile("bar.sync 1, 128;" ::: "memory"); break;
+    case 1: asm volatile("bar.sync 2, 128;" ::: "memory"); break;
+    case 2: asm volatile("bar.sync 3, 128;" ::: "memory"); break;
+    default: asm volatile("bar.sync 4, 128;" ::: "memory");
+  }
+}
+
+// two floats in one instruction
+struct F2 {
+  float a, b;
+};
+__device__ __forceinline__ F2 mul2(F2 x, F2 y) {
+  F2 r;
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(r.a), "=f"(r.b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 c) {
+  F2 r;
+  asm("{\n\t.reg .b64 p, q, m;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 m, {%6, %7};\n\t"
+      "fma.rn.f32x2 p, p, q, m;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(r.a), "=f"(r.b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b), "f"(c.a), "f"(c.b));
+  return r;
+}
+__device__ __forceinline__ F2 sub2(F2 x, F2 y) {   // x + (-y)
+  F2 r;
+  asm("{\n\t.reg .b64 p, q, m;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 m, 0xbf800000bf800000;\n\t"
+      "fma.rn.f32x2 p, q, m, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(r.a), "=f"(r.b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b));
+  return r;
+}
+// cut off behind bf16's eighth bit; the same packed
+__device__ __forceinline__ F2 cut2(F2 x) {
+  return {__uint_as_float(__float_as_uint(x.a) & 0xffff0000u), __uint_as_float(__float_as_uint(x.b) & 0xffff0000u)};
+}
+__device__ __forceinline__ uint32_t upper2(F2 x) { return __byte_perm(__float_as_uint(x.a), __float_as_uint(x.b), 0x7632); }
+
+// Waits asleep for up to about a millisecond.
+__device__ __forceinline__ bool try_wait_for(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P1;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, P1;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
 }
 
 struct Waiter {
@@ -156,12 +221,12 @@ struct Waiter {
   volatile int* stop;
   // false: the CTA gives up
   __device__ __forceinline__ bool operator()(int b, uint32_t parity) const {
-    if (mbar_try_wait(bars + b, parity)) return true;
+    if (try_wait_for(bars + b, parity)) return true;
     return slow(b, parity);
   }
   __device__ __noinline__ bool slow(int b, uint32_t parity) const {
     const uint64_t t0 = global_ns();
-    while (!mbar_try_wait(bars + b, parity)) {
+    while (!try_wait_for(bars + b, parity)) {
       if (*stop) return false;
       if (global_ns() - t0 > kWaitLimit) {
         *stop = 1;
@@ -189,13 +254,16 @@ template <int DQ, int DV, bool LOCAL>
 __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ? 2 : 1)
     la_tc_kernel(const __grid_constant__ LaTcParams prm) {
   using SH = Shape<DQ, DV>;
-  constexpr int NB = SH::NB;
+  constexpr int NB = SH::NB, NW = SH::NW;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t sm = smem_u32(smem);
-  float* tab = (float*)(smem + SH::off_tab);   // lambda^0 .. lambda^128
+  // Powers of lambda in the order in which they are wanted, so that a loop over positions has fixed offsets.  Forward:
+  // lambda^127 .. lambda^0 and 32 zeros; in reverse: 32 zeros, lambda^0 .. lambda^127.  The zeros are the masked side of a
+  // diagonal block.
+  float* tab = (float*)(smem + SH::off_tab);
   uint64_t* bars = (uint64_t*)(smem + SH::off_bar);
-  volatile int* stop = (volatile int*)(smem + SH::off_bar + 16 * 8);
-  uint32_t* slot = (uint32_t*)(smem + SH::off_bar + 16 * 8 + 4);
+  volatile int* stop = (volatile int*)(smem + SH::off_bar + 17 * 8);
+  uint32_t* slot = (uint32_t*)(smem + SH::off_bar + 17 * 8 + 4);
 
   const LaParams& lp = prm.p;
   const int ti = blockIdx.x % lp.ntask, u = blockIdx.x / lp.ntask;
@@ -215,13 +283,18 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   const bool fresh = !LOCAL && before == 0 && !tk.s0;
 
   if (threadIdx.x == 0) {
-    const int count[B_COUNT] = {1, 1, 1, 128, 1, 128, 1, 128, 128, 128 * NB, 1, 128 * NB, 1, 128 * NB, 1};
-    for (int i = 0; i < B_COUNT; i++) mbar_init(bars + i, (uint32_t)count[i]);
+    for (int i = 0; i < B_COUNT; i++) {
+      const bool a = i == B_P || i == B_OS || i == B_OOUT || i == B_OFREE, x = i == B_X || i == B_X2 || i == B_ST;
+      mbar_init(bars + i, a ? 128u : x ? 128u * NW : 1u);
+    }
     *stop = (sm & 1023u) != 0;   // swizzled tiles need the alignment that the launch gives
     if (*stop) atomicExch(&g_la_status, SFFFT_ERR_DEVICE);
     fence_mbar_init();
   }
-  for (int i = threadIdx.x; i <= kTok; i += blockDim.x) tab[i] = dec.pow(i);
+  for (int i = threadIdx.x; i < 160; i += blockDim.x) {
+    const int e = rev ? i - 32 : 127 - i;
+    tab[i] = e >= 0 ? dec.pow(e) : 0.f;
+  }
   if (warp == SH::threads / 32 - 1) {
     tmem_alloc(slot, SH::cols);
     tmem_relinquish();
@@ -232,7 +305,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   const uint32_t tm = *slot;
   const Waiter wait{bars, stop};
   const WarpWaiter wwait{wait};
-  const uint32_t tabs = sm + SH::off_tab;
+  auto power = [&](int e) { return tab[rev ? 32 + e : 127 - e]; };   // 0 <= e < 128
 
   auto tokens = [&](int c) {   // of chunk c0 + c
     const int blk = rev ? nblk - 1 - (c0 + c) : c0 + c;
@@ -246,80 +319,118 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     if (lane == 0) {
       const CUtensorMap* m = prm.map[ti];
       const int hq = h / tk.qdiv, hk = h / tk.kdiv, hv = h / tk.vdiv;
-      auto load = [&](int c) {
+      auto load_kv = [&](int c) {
         const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage;
-        uint64_t* bar = bars + B_FULL0 + (c & 1);
+        uint64_t* bar = bars + B_KV0 + (c & 1);
         const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
-        mbar_expect(bar, (LOCAL ? SH::q_bytes : 2 * SH::q_bytes) + SH::v_bytes);
+        mbar_expect(bar, SH::q_bytes + SH::v_bytes);
         for (int i = 0; i < DQ / 64; i++) tma_load(st + SH::q_bytes + i * kBlk, m + 1, i * 64, t, hk, b, bar);
-        if (!LOCAL)
-          for (int i = 0; i < DQ / 64; i++) tma_load(st + i * kBlk, m + 0, i * 64, t, hq, b, bar);
         for (int i = 0; i < NB; i++) tma_load(st + 2 * SH::q_bytes + i * kBlk, m + 2, i * 64, t, hv, b, bar);
       };
-      int issued = 0;
-      for (; issued < min(nc, 2); issued++) load(issued);
-      for (int c = 0; c < nc; c++) {
-        if (!wait(LOCAL ? B_ST : B_OOUT, c & 1)) break;
-        if (!LOCAL && !tk.y_f32) {
-          const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage + 2 * SH::q_bytes;
+      auto load_q = [&](int c) {
+        const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage;
+        uint64_t* bar = bars + B_Q0 + (c & 1);
+        const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
+        mbar_expect(bar, SH::q_bytes);
+        for (int i = 0; i < DQ / 64; i++) tma_load(st + i * kBlk, m + 0, i * 64, t, hq, b, bar);
+      };
+      int kv = 0, qs = 0;   // loads issued
+      for (; kv < min(nc, 2); kv++) load_kv(kv);
+      if (!LOCAL)
+        for (; qs < min(nc, 2); qs++) load_q(qs);
+      // a parity names the phase that follows a completed one: the first publication goes by before the loop
+      const bool go = LOCAL || nc == 0 || wait(B_ST, 0);
+      for (int c = 0; go && c < nc; c++) {
+        // K and V have been read: by X and its products, and by P V
+        if (!wait(B_ST, (LOCAL ? c : c + 1) & 1) || (!LOCAL && !wait(B_O, c & 1))) break;
+        if ((LOCAL || SH::out_q) && c + 2 < nc) load_kv(kv++);
+        if (LOCAL) continue;
+        if (!wait(B_OOUT, c & 1)) break;
+        if (!tk.y_f32) {
+          const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage + (SH::out_q ? 0 : 2 * SH::q_bytes);
           const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
           for (int i = 0; i < NB; i++) tma_store(m + 3, st + i * kBlk, i * 64, t, h, b);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          if (c + 2 < nc || c + 1 == nc) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          if (c + 2 < nc) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
-        if (c + 2 < nc) load(issued++);
+        if (c + 2 < nc) {
+          if (!SH::out_q) load_kv(kv++);
+          load_q(qs++);
+        }
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      if (*stop)   // copies in flight end before the block does
-        for (int c = max(0, issued - 2); c < issued; c++) mbar_wait_bounded(bars + B_FULL0 + (c & 1), (c >> 1) & 1, kWaitLimit);
+      if (*stop) {   // copies in flight end before the block does
+        for (int c = max(0, kv - 2); c < kv; c++) mbar_wait_bounded(bars + B_KV0 + (c & 1), (c >> 1) & 1, kWaitLimit);
+        for (int c = max(0, qs - 2); c < qs; c++) mbar_wait_bounded(bars + B_Q0 + (c & 1), (c >> 1) & 1, kWaitLimit);
+      }
     }
   } else if (warp == SH::threads / 32 - 1) {
     // ---- products ----
     if (lane == 0) {
       constexpr uint32_t id_s = idesc_bf16(128, false), id_v = idesc_bf16(DV, true);
-      for (int c = 0; c < nc; c++) {
+      auto at = [](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
+      auto kstep = [](int k) { return (uint32_t)(k >> 2) * kBlk + (uint32_t)(k & 3) * 32; };   // K-major: 16 values on
+      const uint64_t sd = make_sdesc(sm + SH::off_s, kBlk, 1024, LT_SW128);
+      bool ok = true;
+      for (int c = 0; ok && c < nc; c++) {
         const uint32_t ph = c & 1, st = sm + (uint32_t)(c & 1) * SH::stage;
-        if (!wait(B_FULL0 + (c & 1), (c >> 1) & 1)) break;
+        if (!wait(B_KV0 + (c & 1), (c >> 1) & 1)) break;
         const uint64_t qd = make_sdesc(st, 16, 1024, LT_SW128), kd = make_sdesc(st + SH::q_bytes, 16, 1024, LT_SW128);
         const uint64_t vd = make_sdesc(st + 2 * SH::q_bytes, kBlk, 1024, LT_SW128);
-        const uint64_t sd = make_sdesc(sm + SH::off_s, kBlk, 1024, LT_SW128);
-        auto at = [](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
-        auto kstep = [](int k) { return (uint32_t)(k >> 2) * kBlk + (uint32_t)(k & 3) * 32; };   // K-major: 16 values on
         if (!LOCAL) {
+          if (!wait(B_Q0 + (c & 1), (c >> 1) & 1)) break;
           if (SH::alias && c > 0 && !wait(B_OFREE, ph ^ 1)) break;
           tc_fence_after();
           for (int k = 0; k < DQ / 16; k++) mma_f16_ss(tm + SH::c_p, at(qd, kstep(k)), at(kd, kstep(k)), id_s, k > 0);
           mma_commit(bars + B_S);
         }
-        if (!wait(B_X, ph)) break;
-        tc_fence_after();
-        for (int part = 0; part < DQ / 64; part++)
-          for (int k = 0; k < 8; k++)
-            mma_ts(tm + SH::c_kv, tm + SH::c_x + part * 64 + k * 8, at(vd, k * 2048), id_v, (part | k) > 0);
-        mma_commit(bars + B_KV);
-        if (!LOCAL) {
-          if (!wait(B_ST, ph)) break;
-          if (!SH::alias && c > 0 && !wait(B_OFREE, ph ^ 1)) break;
-          if (SH::alias && !wait(B_P, ph)) break;
-          tc_fence_after();
-          if (!(fresh && c == 0))
+        // the chunk's other products in the order in which their operands become ready
+        bool inc = false, inc2 = !three, qs = LOCAL, pv = LOCAL;
+        const bool dirty = tokens(c) < kTok && n < lp.L;   // v is cleaned before X arrives
+        uint64_t t0 = 0;
+        uint32_t idle = 0;
+        while (!(inc && inc2 && qs && pv)) {
+          if (!qs && mbar_test_wait(bars + B_ST, ph) &&
+              (SH::alias ? mbar_test_wait(bars + B_P, ph) : c == 0 || mbar_test_wait(bars + B_OFREE, ph ^ 1))) {
+            tc_fence_after();
+            if (!(fresh && c == 0))
+              for (int k = 0; k < 8; k++)
+                mma_f16_ss(tm + SH::c_o, at(qd, kstep(DQ == 64 ? k & 3 : k)), at(sd, k * 2048), id_v, k > 0);
+            mma_commit(bars + B_O1);
+            qs = true;
+          } else if (qs && !pv && (inc || !dirty) && mbar_test_wait(bars + B_OS, ph) && mbar_test_wait(bars + B_P, ph)) {
+            tc_fence_after();
             for (int k = 0; k < 8; k++)
-              mma_f16_ss(tm + SH::c_o, at(qd, kstep(DQ == 64 ? k & 3 : k)), at(sd, k * 2048), id_v, k > 0);
-          mma_commit(bars + B_O1);
-        }
-        if (three) {
-          if (!wait(B_X2, ph)) break;
-          tc_fence_after();
-          for (int k = 0; k < 8; k++) mma_ts(tm + SH::c_kv, tm + SH::c_x + k * 8, at(vd, k * 2048), id_v, 1);
-          mma_commit(bars + B_KV2);
-        }
-        if (!LOCAL) {
-          if (!SH::alias && !wait(B_P, ph)) break;
-          if (!wait(B_OS, ph)) break;
-          tc_fence_after();
-          for (int k = 0; k < 8; k++)
-            mma_ts(tm + SH::c_o, tm + SH::c_p + k * 8, at(vd, k * 2048), id_v, k > 0 || !(fresh && c == 0));
-          mma_commit(bars + B_O);
+              mma_ts(tm + SH::c_o, tm + SH::c_p + k * 8, at(vd, k * 2048), id_v, k > 0 || !(fresh && c == 0));
+            mma_commit(bars + B_O);
+            pv = true;
+          } else if (!inc && mbar_test_wait(bars + B_X, ph)) {
+            tc_fence_after();
+            for (int part = 0; part < DQ / 64; part++)
+              for (int k = 0; k < 8; k++)
+                mma_ts(tm + SH::c_kv, tm + SH::c_x + part * 64 + k * 8, at(vd, k * 2048), id_v, (part | k) > 0);
+            mma_commit(bars + B_INC);
+            inc = true;
+          } else if (inc && !inc2 && mbar_test_wait(bars + B_X2, ph)) {
+            tc_fence_after();
+            for (int k = 0; k < 8; k++) mma_ts(tm + SH::c_kv, tm + SH::c_x + k * 8, at(vd, k * 2048), id_v, 1);
+            mma_commit(bars + B_INC2);
+            inc2 = true;
+          } else {
+            if ((++idle & 63) == 0) {
+              const uint64_t now = global_ns();
+              if (!t0) t0 = now;
+              if (now - t0 > kWaitLimit) {
+                *stop = 1;
+                atomicExch(&g_la_status, SFFFT_ERR_TIMEOUT);
+              }
+              if (*stop) {
+                ok = false;
+                break;
+              }
+            }
+            __nanosleep(20);
+          }
         }
       }
       if (*stop) {   // products in flight end before TMEM is given back
@@ -332,6 +443,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     if (!LOCAL) {
       const int i = threadIdx.x;   // position in the chunk
       const uint32_t tl = tm + ((uint32_t)(warp * 32) << 16);
+      const float whole = dec.pow(kTok);
       for (int c = 0; c < nc; c++) {
         const uint32_t ph = c & 1;
         const int m = tokens(c), blk = rev ? nblk - 1 - (c0 + c) : c0 + c;
@@ -341,52 +453,43 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
 #pragma unroll 1
         for (int jb = 0; jb < 4; jb++) {
           uint32_t r[32], o[16];
-          const bool some = rev ? jb >= warp : jb <= warp;
-          if (some) {
-            tmem_ld32(tl + SH::c_p + jb * 32, r);
-            // lambda^|i-j|: within the diagonal block the other side is masked, and its table index held in range
-            const int d0 = rev ? jb * 32 - i : i - jb * 32;   // |i - j| = d0 -+ jj
-            tmem_wait_ld();
-            if (rev) {
-#pragma unroll
-              for (int jj = 0; jj < 32; jj++) {
-                const int d = d0 + jj;
-                const float w = lds32(tabs + 4u * (uint32_t)max(d, 0));
-                const float x = __uint_as_float(r[jj]) * w;
-                r[jj] = __float_as_uint(d >= 0 && jb * 32 + jj < m ? x : 0.f);
-              }
-            } else {
-#pragma unroll
-              for (int jj = 0; jj < 32; jj++) {
-                const int d = d0 - jj;
-                const float w = lds32(tabs + 4u * (uint32_t)max(d, 0));
-                const float x = __uint_as_float(r[jj]) * w;
-                r[jj] = __float_as_uint(d >= 0 && i < m ? x : 0.f);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[e] = pack_bf16(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-          } else {
+          if (rev ? jb < warp : jb > warp) {   // a block on the masked side of the diagonal
 #pragma unroll
             for (int e = 0; e < 16; e++) o[e] = 0;
+          } else {
+            tmem_ld32(tl + SH::c_p + jb * 32, r);
+            const float* w = tab + (rev ? 32 + jb * 32 - i : 127 - i + jb * 32);
+            tmem_wait_ld();
+            if (m < kTok) {   // products with what k holds behind the last token may not be finite
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (jb * 32 + e >= m) r[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+              o[e] = pack_bf16(__uint_as_float(r[2 * e]) * w[2 * e], __uint_as_float(r[2 * e + 1]) * w[2 * e + 1]);
           }
           tmem_st16(tl + SH::c_p + jb * 16, o);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bars + B_P);
-        // lambda^(i+1) Q S (in reverse lambda^(m-i)); rows behind the last token hold whatever q holds: zero
+        // lambda^(i+1) Q S, in reverse lambda^(m-i)
         if (!wwait(B_O1, ph)) break;
         tc_fence_after();
         if (!(fresh && c == 0)) {
-          const float w = i < m ? tab[(rev ? m - i : i + 1) - off] : 0.f;
+          const int e = (rev ? m - i : i + 1) - off;
+          const float w = e < 0 ? 0.f : e < kTok ? power(e) : whole;
 #pragma unroll 1
           for (int q = 0; q < DV / 32; q++) {
             uint32_t r[32];
             tmem_ld32(tl + SH::c_o + q * 32, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) r[e] = __float_as_uint(i < m ? __uint_as_float(r[e]) * w : 0.f);
+            for (int x = 0; x < 32; x += 2) {
+              const F2 z = mul2({__uint_as_float(r[x]), __uint_as_float(r[x + 1])}, {w, w});
+              r[x] = __float_as_uint(z.a), r[x + 1] = __float_as_uint(z.b);
+            }
             tmem_st32(tl + SH::c_o + q * 32, r);
           }
           tmem_wait_st();
@@ -395,19 +498,27 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
         mbar_arrive(bars + B_OS);
         if (!wwait(B_O, ph)) break;
         tc_fence_after();
-        const uint32_t out = sm + (uint32_t)(c & 1) * SH::stage + 2 * SH::q_bytes + (uint32_t)i * 128;
+        if (!SH::out_q && !wwait(three ? B_INC2 : B_INC, ph)) break;   // V's last reader
+        const uint32_t out = sm + (uint32_t)(c & 1) * SH::stage + (SH::out_q ? 0 : 2 * SH::q_bytes) + (uint32_t)i * 128;
 #pragma unroll 1
         for (int q = 0; q < DV / 32; q++) {
           uint32_t r[32];
           tmem_ld32(tl + SH::c_o + q * 32, r);
           tmem_wait_ld();
+          // rows behind the last token: whatever q holds has come through
+          if (m < kTok && i >= m) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) r[e] = 0;
+          }
           if (!tk.y_f32) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               uint32_t w[4];
 #pragma unroll
-              for (int x = 0; x < 4; x++)
-                w[x] = pack_bf16(tk.scale * __uint_as_float(r[8 * e + 2 * x]), tk.scale * __uint_as_float(r[8 * e + 2 * x + 1]));
+              for (int x = 0; x < 4; x++) {
+                const F2 z = mul2({__uint_as_float(r[8 * e + 2 * x]), __uint_as_float(r[8 * e + 2 * x + 1])}, {tk.scale, tk.scale});
+                w[x] = pack_bf16(z.a, z.b);
+              }
               const uint32_t chunk = (uint32_t)((q & 1) * 4 + e);
               sts128(out + (uint32_t)(q >> 1) * kBlk + ((chunk ^ (uint32_t)(i & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
@@ -444,11 +555,12 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     const uint32_t tl = tm + ((uint32_t)((warp & 3) * 32) << 16);
     const int d = DQ == 64 ? t & 63 : t;        // the thread's row of the state
     const bool main_part = DQ == 128 || t < 64; // lanes 64-127 hold the second part where the head size is 64
-    float s[64];
+    float s[32];                                // columns 32 wg ..
+    const int col = wg * 32;
 #pragma unroll
-    for (int e = 0; e < 64; e++) s[e] = 0.f;
+    for (int e = 0; e < 32; e++) s[e] = 0.f;
     if (!LOCAL && main_part && d < tk.D) {
-      const float* loc = tk.loc + ((long long)bh * lp.G * tk.D + d) * tk.Dv + wg * 64;
+      const float* loc = tk.loc + ((long long)bh * lp.G * tk.D + d) * tk.Dv + col;
       const long long step = (long long)tk.D * tk.Dv;
       for (int gg = 0; gg < g; gg++) {
         const int a = tokens_before(min(gg * prm.blocks, nblk), n, nblk, rev);
@@ -456,23 +568,37 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
         if (z == a) break;
         const float w = dec.pow(z - a);
 #pragma unroll
-        for (int e = 0; e < 64; e++)
-          if (wg * 64 + e < tk.Dv) s[e] = fmaf(w, s[e], loc[gg * step + e]);
+        for (int e = 0; e < 32; e += 4)   // Dv is a multiple of 8
+          if (col + e < tk.Dv) {
+            const float4 x = *(const float4*)(loc + gg * step + e);
+            s[e] = fmaf(w, s[e], x.x), s[e + 1] = fmaf(w, s[e + 1], x.y);
+            s[e + 2] = fmaf(w, s[e + 2], x.z), s[e + 3] = fmaf(w, s[e + 3], x.w);
+          }
       }
       if (tk.s0) {
         const float w = dec.pow(before - (tk.off && before > 0));
-        const float* s0 = tk.s0 + b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + (long long)(wg * 64) * tk.s0s[3];
+        const float* s0 = tk.s0 + b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + (long long)col * tk.s0s[3];
 #pragma unroll
-        for (int e = 0; e < 64; e++)
-          if (wg * 64 + e < tk.Dv) s[e] = fmaf(w, s0[e * tk.s0s[3]] * tk.s0_mul, s[e]);
+        for (int e = 0; e < 32; e++)
+          if (col + e < tk.Dv) s[e] = fmaf(w, s0[e * tk.s0s[3]] * tk.s0_mul, s[e]);
       }
     }
-    const uint32_t srow = sm + SH::off_s + (uint32_t)wg * kBlk + (uint32_t)t * 128;
+    const uint32_t srow = sm + SH::off_s + (uint32_t)(wg >> 1) * kBlk + (uint32_t)t * 128;
     auto publish = [&]() {   // S in bf16 for the next chunk's product
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        sts128(srow + (((uint32_t)e ^ (uint32_t)(t & 7)) << 4), pack_bf16(s[8 * e], s[8 * e + 1]), pack_bf16(s[8 * e + 2], s[8 * e + 3]),
-               pack_bf16(s[8 * e + 4], s[8 * e + 5]), pack_bf16(s[8 * e + 6], s[8 * e + 7]));
+      for (int e = 0; e < 4; e++)
+        sts128(srow + (((uint32_t)(4 * (wg & 1) + e) ^ (uint32_t)(t & 7)) << 4), pack_bf16(s[8 * e], s[8 * e + 1]),
+               pack_bf16(s[8 * e + 2], s[8 * e + 3]), pack_bf16(s[8 * e + 4], s[8 * e + 5]), pack_bf16(s[8 * e + 6], s[8 * e + 7]));
+      fence_async_smem();
+    };
+    // Zeroes v behind the last token of the chunk, where it may hold anything, and 0 * NaN is NaN.  Products with v wait
+    // for X in such a chunk.
+    auto clean_v = [&](int c) {
+      const int m = tokens(c);
+      if (m == kTok || n == lp.L) return;
+      const uint32_t v = sm + (uint32_t)(c & 1) * SH::stage + 2 * SH::q_bytes + (uint32_t)(wg >> 1) * kBlk;
+      for (int e = t; e < (kTok - m) * 4; e += 128)
+        sts128(v + (uint32_t)(m + (e >> 2)) * 128 + (uint32_t)(4 * (wg & 1) + (e & 3)) * 16, 0, 0, 0, 0);
       fence_async_smem();
     };
     if (!LOCAL) {
@@ -481,109 +607,137 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     }
     // lambda^128 as a sum of two floats: its rounding would come back with every chunk
     const float whole = dec.pow(kTok), whole_lo = dec.pow_rest(kTok, whole);
-    constexpr int TPW = kTok / NB;   // positions whose X this warpgroup makes
-    const uint32_t kcol = (uint32_t)(d >> 6) * kBlk + (uint32_t)(d & 7) * 2;
-    const uint32_t cd = (uint32_t)(d & 63) >> 3;
+    constexpr int TPW = kTok / NW;   // positions whose X this warpgroup makes
+    // Address of the lane's row of the K tiles of the warp's first 16 rows d and first 16 positions: tiles (d, position) are
+    // (0-7, 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15); 16 rows d on is two 16-byte pieces on, under the swizzle.
+    const int dw = DQ == 64 ? (warp & 1) * 32 : (warp & 3) * 32;
+    const uint32_t kaddr = SH::q_bytes + (uint32_t)(dw >> 6) * kBlk + (uint32_t)(((lane >> 4) & 1) * 8 + (lane & 7)) * 128 +
+                           ((((uint32_t)(dw & 63) >> 3) + ((uint32_t)(lane >> 3) & 1)) ^ (uint32_t)(lane & 7)) * 16;
     for (int c = 0; c < nc; c++) {
       const uint32_t ph = c & 1, st = sm + (uint32_t)(c & 1) * SH::stage;
       const int m = tokens(c);
       const int off = tk.off && before == 0 && c == 0;
-      if (!wwait(B_FULL0 + (c & 1), (c >> 1) & 1)) break;
-      if (m < kTok && n < lp.L) {   // v behind the last token may hold anything, and 0 * NaN is NaN
-        const uint32_t v = st + 2 * SH::q_bytes + (uint32_t)wg * kBlk;
-        for (int e = t; e < (kTok - m) * 8; e += 128) sts128(v + (uint32_t)m * 128 + (uint32_t)e * 16, 0, 0, 0, 0);
-        fence_async_smem();
-      }
-      // the first two parts of X, or the third
+      if (!wwait(B_KV0 + (c & 1), (c >> 1) & 1)) break;
+      clean_v(c);
+      // The first two parts of X, or the third.  Lanes of X are rows d of the state, its columns pairs of positions: K's
+      // tiles come transposed from shared memory in the very arrangement that the 16 x 128b store takes.
       auto make_x = [&](bool third) {
-        const uint32_t kb = st + SH::q_bytes + kcol;
 #pragma unroll 1
         for (int j0 = wg * TPW; j0 < (wg + 1) * TPW; j0 += 32) {
-          uint32_t a[16], z[16];
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            float x[2];
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-              const int jj = 2 * e + q, j = j0 + jj;
-              const uint32_t raw = lds16(kb + (uint32_t)j0 * 128 + (uint32_t)jj * 128 + ((cd ^ (uint32_t)(jj & 7)) << 4));
-              const float w = lds32(tabs + 4u * (uint32_t)(rev ? j : max(m - 1 - j, 0)));
-              const float y = __uint_as_float(raw << 16) * w;
-              x[q] = j < m ? y : 0.f;
-            }
-            const uint32_t p1 = pack_bf16(x[0], x[1]);
-            const float r0 = x[0] - lo_f(p1), r1 = x[1] - hi_f(p1);
-            const uint32_t p2 = pack_bf16(r0, r1);
-            if (third) {
-              a[e] = main_part ? pack_bf16(r0 - lo_f(p2), r1 - hi_f(p2)) : 0u;
-            } else if (DQ == 64) {
-              a[e] = t < 64 ? p1 : p2;
-            } else {
-              a[e] = p1;
-              z[e] = p2;
-            }
+          if (DQ == 64 && third && (j0 < kTok / 2) != (t < 64)) {   // each half of the lanes takes half the positions
+            const uint32_t none[8] = {};
+            tmem_st_16x128b_x4(tl + SH::c_x + j0 / 2, none);
+            tmem_st_16x128b_x4(tl + (16u << 16) + SH::c_x + j0 / 2, none);
+            continue;
           }
-          tmem_st16(tl + SH::c_x + j0 / 2, a);
-          if (DQ == 128 && !third) tmem_st16(tl + SH::c_x + 64 + j0 / 2, z);
+          float w[8];   // of positions j0 + 8 i + 2 (lane % 4) + {0, 1}
+          const int wi = (rev ? 32 : kTok - m) + j0 + 2 * (lane & 3);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float* at = tab + min(wi + 8 * i, 158);   // behind the last token: the zeros
+            w[2 * i] = at[0], w[2 * i + 1] = at[1];
+          }
+#pragma unroll 1
+          for (int half = 0; half < 2; half++) {   // 16 rows each
+            uint32_t r[8], z[8];
+            const uint32_t addr = (kaddr + st + (uint32_t)j0 * 128) ^ (uint32_t)(32 * half);
+            ldsm_t(addr, *(uint32_t(*)[4]) & r[0]);
+            ldsm_t(addr + 16 * 128, *(uint32_t(*)[4]) & r[4]);
+            if (m < kTok) {   // behind the last token k may hold anything
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int j = j0 + 8 * i + 2 * (lane & 3);
+                const uint32_t mask = (j < m ? 0xffffu : 0u) | (j + 1 < m ? 0xffff0000u : 0u);
+                r[2 * i] &= mask;
+                r[2 * i + 1] &= mask;
+              }
+            }
+            const uint32_t to = tl + ((uint32_t)(16 * half) << 16) + SH::c_x + j0 / 2;
+            // each part but the last is cut off, so that what is left is exact
+            if (DQ == 64 && !third && t < 64) {
+#pragma unroll
+              for (int i = 0; i < 8; i++) r[i] = upper2(mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]}));
+            } else if (!third) {
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
+                if (DQ == 128) z[i] = upper2(x);
+                x = sub2(x, cut2(x));
+                r[i] = pack_bf16(x.a, x.b);
+              }
+              if (DQ == 128) tmem_st_16x128b_x4(to, z);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
+                x = sub2(x, cut2(x));
+                x = sub2(x, cut2(x));
+                r[i] = pack_bf16(x.a, x.b);
+              }
+            }
+            tmem_st_16x128b_x4(DQ == 128 && !third ? to + 64 : to, r);
+          }
         }
         tmem_wait_st();
         tc_fence_before();
       };
       make_x(false);
       mbar_arrive(bars + B_X);
-      if (!wwait(B_KV, ph)) break;
+      if (!wwait(B_INC, ph)) break;
+      tc_fence_after();
       if (three) {
-        tc_fence_after();
         make_x(true);
         mbar_arrive(bars + B_X2);
-        if (!wwait(B_KV2, ph)) break;
+        if (!wwait(B_INC2, ph)) break;
       }
       if (!LOCAL && !wwait(B_O1, ph)) break;   // the product with the old S has been taken
       tc_fence_after();
       float w = whole, w_lo = whole_lo;
-      if (m - off < kTok) w = tab[m - off], w_lo = 0.f;
+      if (m - off < kTok) w = power(m - off), w_lo = 0.f;
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
+      for (int q = 0; q < 2; q++) {
         uint32_t r[16];
-        tmem_ld16(tl + SH::c_kv + wg * 64 + q * 16, r);
+        tmem_ld16(tl + SH::c_kv + col + q * 16, r);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float& x = s[q * 16 + e];
-          x = fmaf(w, x, fmaf(w_lo, x, __uint_as_float(r[e])));
+        for (int e = 0; e < 16; e += 2) {
+          float &x = s[q * 16 + e], &y = s[q * 16 + e + 1];
+          const F2 z = fma2({w, w}, {x, y}, fma2({w_lo, w_lo}, {x, y}, {__uint_as_float(r[e]), __uint_as_float(r[e + 1])}));
+          x = z.a, y = z.b;
         }
       }
       tc_fence_before();
-      if (!LOCAL) publish();
+      if (!LOCAL && c + 1 < nc) publish();
       mbar_arrive(bars + B_ST);
     }
     // the state that the segment leaves (after a wait that gave up: whatever it is, but every thread comes by)
     if (LOCAL || (tk.s1 && g == lp.G - 1)) {
       if constexpr (DQ == 64) {   // add the two parts; S's shared memory is free: nothing reads it any more
-        wg_sync(wg);
-        float* x = (float*)(smem + SH::off_s + wg * kBlk);
+        // every warpgroup is behind its last use of the tile
+        asm volatile("bar.sync 5, %0;" ::"n"(128 * SH::NW) : "memory");
+        float* x = (float*)(smem + SH::off_s + wg * (kBlk / 2));
         if (t >= 64) {
 #pragma unroll
-          for (int e = 0; e < 64; e++) x[e * 64 + d] = s[e];
+          for (int e = 0; e < 32; e++) x[e * 64 + d] = s[e];
         }
         wg_sync(wg);
         if (t < 64) {
 #pragma unroll
-          for (int e = 0; e < 64; e++) s[e] += x[e * 64 + d];
+          for (int e = 0; e < 32; e++) s[e] += x[e * 64 + d];
         }
       }
       if (main_part && d < tk.D) {
         if (LOCAL) {
-          float* out = tk.loc + (((long long)bh * lp.G + g) * tk.D + d) * tk.Dv + wg * 64;
+          float* out = tk.loc + (((long long)bh * lp.G + g) * tk.D + d) * tk.Dv + col;
 #pragma unroll
-          for (int e = 0; e < 64; e++)
-            if (wg * 64 + e < tk.Dv) out[e] = s[e];
+          for (int e = 0; e < 32; e += 4)
+            if (col + e < tk.Dv) *(float4*)(out + e) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
         } else {
-          const float w = tk.s1_mul * (tk.s1_decay && n > 0 ? tab[1] : 1.f);
-          float* out = tk.s1 + b * tk.s1s[0] + h * tk.s1s[1] + d * tk.s1s[2] + (long long)(wg * 64) * tk.s1s[3];
+          const float w = tk.s1_mul * (tk.s1_decay && n > 0 ? power(1) : 1.f);
+          float* out = tk.s1 + b * tk.s1s[0] + h * tk.s1s[1] + d * tk.s1s[2] + (long long)col * tk.s1s[3];
 #pragma unroll
-          for (int e = 0; e < 64; e++)
-            if (wg * 64 + e < tk.Dv) out[e * tk.s1s[3]] = w * s[e];
+          for (int e = 0; e < 32; e++)
+            if (col + e < tk.Dv) out[e * tk.s1s[3]] = w * s[e];
         }
       }
     }
