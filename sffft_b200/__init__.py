@@ -10,7 +10,10 @@ fallback: if ``lib/libsffft.so`` is missing or the device is not a B200, calls f
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -514,6 +517,32 @@ def emu_conv(config: str, u, Kf, io: str = "fp32", acc: str = "fp32"):
 # Linear attention with a decay for each head, and the norms that join a block to the residual stream
 # ---------------------------------------------------------------------------------------------------------------
 
+# The descriptors as the C structs lie in memory; a call's own is packed, which takes a tenth of filling a ctypes object.
+_LA_DESC, _LA_GRADS = struct.Struct("@8if12q"), struct.Struct("@12q")
+_LA_STEP, _BN_DESC = struct.Struct("@8if9q"), struct.Struct("@q8i2fi3q")
+
+
+def _on_stream(f):
+    """Adds `stream`: the call and its buffers belong to that stream (torch's, or a raw handle), as under torch.cuda.stream."""
+    @functools.wraps(f)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return f(*args, **kw)
+        import torch
+        if isinstance(stream, int):
+            lead = next(a for a in (*args, *kw.values()) if isinstance(a, torch.Tensor))
+            stream = torch.cuda.ExternalStream(stream, device=lead.device)
+        with torch.cuda.stream(stream):
+            return f(*args, **kw)
+    return call
+
+
+def _current(index):
+    """The device's current stream, raw."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _io_of(t, what):
     import torch
     if t.dtype == torch.float32:
@@ -523,27 +552,9 @@ def _io_of(t, what):
     raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}")
 
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
-def _call_stream(stream, device):
-    """(raw stream, torch stream) of a call: the given one, or the device's current stream."""
-    import torch
-    if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, None
-    if isinstance(stream, int):
-        return stream, torch.cuda.ExternalStream(stream, device=device)
-    return stream.cuda_stream, stream
-
-
-def _used_on(stream, *tensors):
-    """Tells the allocator that buffers this call made are in use on a stream other than the current one."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
+def _need_cuda(t, what):
+    if t.device.type != "cuda":
+        raise ValueError(f"{what} needs CUDA tensors (there is no CPU path)")
 
 
 def _heads_like(like, B, H, L, D, dtype):
@@ -559,103 +570,97 @@ def _unit(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _plain(t):
+    """(contiguous tensor, its address), or None twice."""
+    if t is None:
+        return None, None
+    t = t if t.is_contiguous() else t.contiguous()
+    return t, t.data_ptr()
+
+
 def check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, final_grad=None):
-    """Raises ValueError where the arguments of linear_attention do not fit each other."""
-    import math
-
+    """Raises ValueError where the arguments of linear_attention do not fit each other; else (B, H, L, D, Hkv, Dv, io)."""
     import torch
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k and v must be [B][H][L][D], [B][Hkv][L][D] and [B][Hkv][L][Dv]")
-    B, H, L, D = q.shape
-    Hkv, Dv = k.shape[1], v.shape[3]
-    _need(tuple(k.shape) == (B, Hkv, L, D) and tuple(v.shape) == (B, Hkv, L, Dv),
-          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    _need(H > 0 and Hkv > 0 and H % Hkv == 0, f"{H} query heads cannot share {Hkv} key and value heads evenly")
-    _need(D > 0 and Dv > 0, "head sizes must be positive")
-    _io_of(q, "q")
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type")
-    _need(tuple(log_decay.shape) == (H,) and log_decay.dtype == torch.float32, f"log_decay must be a float32 [{H}] tensor")
-    _need(not log_decay.requires_grad, "log_decay is a constant: it has no gradient (pass log_decay.detach())")
-    _need(math.isfinite(scale) and scale != 0, "scale must be finite and not 0")
-    state = (B, H, D, Dv)
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k and v must be [B][H][L][D], [B][Hkv][L][D] and [B][Hkv][L][Dv]")
+    (B, H, L, D), Hkv, Dv = q.shape, k.shape[1], v.shape[3]
+    if k.shape != (B, Hkv, L, D) or v.shape != (B, Hkv, L, Dv):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} key and value heads evenly")
+    if D < 1 or Dv < 1:
+        raise ValueError("head sizes must be positive")
+    io = _io_of(q, "q")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one type")
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+        raise ValueError(f"log_decay must be a float32 [{H}] tensor")
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is a constant: it has no gradient (pass log_decay.detach())")
+    if not math.isfinite(scale) or scale == 0:
+        raise ValueError("scale must be finite and not 0")
     for t, what in ((initial_state, "initial_state"), (final_grad, "the final state's gradient")):
-        _need(t is None or (tuple(t.shape) == state and t.dtype == torch.float32), f"{what} must be a float32 {list(state)} tensor")
-    _need(lengths is None or (tuple(lengths.shape) == (B,) and lengths.dtype == torch.int32), f"lengths must be an int32 [{B}] tensor")
-    for t in (k, v, log_decay, initial_state, lengths):
-        _need(t is None or t.device == q.device, "all tensors must be on one device")
-
-
-def _la_desc(q, k, v, scale, y_stride):
-    B, H, L, D = q.shape
-    d = LinearAttentionDesc(B, H, k.shape[1], L, D, v.shape[3], _io_of(q, "q"), q.device.index, scale)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    d.y_stride[:] = y_stride
-    return d
+        if t is not None and (t.shape != (B, H, D, Dv) or t.dtype != torch.float32):
+            raise ValueError(f"{what} must be a float32 {[B, H, D, Dv]} tensor")
+    if lengths is not None and (lengths.shape != (B,) or lengths.dtype != torch.int32):
+        raise ValueError(f"lengths must be an int32 [{B}] tensor")
+    for t in (k, v, log_decay, initial_state, lengths, final_grad):
+        if t is not None and t.device != q.device:
+            raise ValueError("all tensors must be on one device")
+    return B, H, L, D, Hkv, Dv, io
 
 
 def _la_workspace(desc, backward, device):
     import torch
     need = ctypes.c_size_t()
-    _check(lib().sffft_linear_attention_workspace_bytes(ctypes.byref(desc), int(backward), ctypes.byref(need)),
-           "linear_attention_workspace_bytes")
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _check(lib().sffft_linear_attention_workspace_bytes(desc, backward, ctypes.byref(need)), "linear_attention_workspace_bytes")
+    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    return work, _ptr(work), need.value
 
 
-def linear_attention(q, k, v, log_decay, scale=1.0, initial_state=None, lengths=None, stream=None):
-    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n with lambda = exp(log_decay) for each head.
+@_on_stream
+def linear_attention(q, k, v, log_decay, scale=1.0, initial_state=None, lengths=None):
+    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n, lambda = exp(log_decay) for each head.
 
     q [B][H][L][D], k [B][Hkv][L][D], v [B][Hkv][L][Dv], float32 or bfloat16; log_decay [H] float32, <= 0;
     initial_state and final_state [B][H][D][Dv] float32; lengths [B] int32: tokens of each row (default L).  y has
     q's type and order of axes, and is zero behind a row's last token.  Runs on `stream` (default: the current one)."""
     import torch
-    check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
-    _need(q.device.type == "cuda", "linear_attention needs CUDA tensors (there is no CPU path)")
-    q, k, v = _unit(q), _unit(k), _unit(v)
-    B, H, L, D = q.shape
-    Dv = v.shape[3]
-    raw, side = _call_stream(stream, q.device)
+    B, H, L, D, Hkv, Dv, io = check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+    _need_cuda(q, "linear_attention")
+    q, k, v, dev = _unit(q), _unit(k), _unit(v), q.device
     y = _heads_like(q, B, H, L, Dv, q.dtype)
-    s1 = torch.empty((B, H, D, Dv), dtype=torch.float32, device=q.device)
-    desc = _la_desc(q, k, v, scale, y.stride()[:3])
-    work = _la_workspace(desc, False, q.device)
-    ld = log_decay.contiguous()
-    s0 = None if initial_state is None else initial_state.contiguous()
-    ln = None if lengths is None else lengths.contiguous()
-    _check(lib().sffft_linear_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(), _ptr(ln),
-                                        _ptr(s0), y.data_ptr(), s1.data_ptr(), _ptr(work), 0 if work is None else work.numel(),
-                                        raw), f"linear_attention(q {list(q.shape)}, v {list(v.shape)})")
-    _used_on(side, q, k, v, ld, s0, ln, y, s1, work)
+    s1 = torch.empty((B, H, D, Dv), dtype=torch.float32, device=dev)
+    desc = _LA_DESC.pack(B, H, Hkv, L, D, Dv, io, dev.index, scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                         *y.stride()[:3])
+    work, wp, wn = _la_workspace(desc, 0, dev)
+    (ld, ldp), (s0, s0p), (ln, lnp) = _plain(log_decay), _plain(initial_state), _plain(lengths)
+    _check(lib().sffft_linear_attention(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldp, lnp, s0p, y.data_ptr(),
+                                        s1.data_ptr(), wp, wn, _current(dev.index)), "linear_attention")
     return y, s1
 
 
-def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1.0, initial_state=None, lengths=None,
-                              stream=None):
+@_on_stream
+def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1.0, initial_state=None, lengths=None):
     """(dq, dk, dv, dinitial_state) of linear_attention; dinitial_state is None where there was no initial state."""
     import torch
-    check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, dfinal_state)
-    _need(q.device.type == "cuda", "linear_attention_backward needs CUDA tensors (there is no CPU path)")
-    B, H, L, D = q.shape
-    Hkv, Dv = k.shape[1], v.shape[3]
-    _need(tuple(dy.shape) == (B, H, L, Dv) and dy.dtype == q.dtype and dy.device == q.device,
-          f"dy must be a {q.dtype} {[B, H, L, Dv]} tensor on q's device")
-    _need(dfinal_state is None or dfinal_state.device == q.device, "all tensors must be on one device")
-    q, k, v = _unit(q), _unit(k), _unit(v)
-    dy = dy if dy.stride(-1) == 1 and 0 not in dy.stride() else dy.contiguous()   # a sum's gradient comes expanded
-    raw, side = _call_stream(stream, q.device)
-    dq, dk, dv = _heads_like(q, B, H, L, D, q.dtype), _heads_like(k, B, Hkv, L, D, q.dtype), _heads_like(v, B, Hkv, L, Dv, q.dtype)
-    ds0 = None if initial_state is None else torch.empty((B, H, D, Dv), dtype=torch.float32, device=q.device)
-    desc = _la_desc(q, k, v, scale, (0, 0, 0))
-    grads = LinearAttentionGrads()
-    grads.dy_stride[:], grads.dq_stride[:], grads.dk_stride[:], grads.dv_stride[:] = (t.stride()[:3] for t in (dy, dq, dk, dv))
-    work = _la_workspace(desc, True, q.device)
-    ld = log_decay.contiguous()
-    s0 = None if initial_state is None else initial_state.contiguous()
-    ds1 = None if dfinal_state is None else dfinal_state.contiguous()
-    ln = None if lengths is None else lengths.contiguous()
+    B, H, L, D, Hkv, Dv, io = check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, dfinal_state)
+    _need_cuda(q, "linear_attention_backward")
+    if dy.shape != (B, H, L, Dv) or dy.dtype != q.dtype or dy.device != q.device:
+        raise ValueError(f"dy must be a {q.dtype} {[B, H, L, Dv]} tensor on q's device")
+    q, k, v, dev = _unit(q), _unit(k), _unit(v), q.device
+    if dy.stride(-1) != 1 or 0 in dy.stride():   # a sum's gradient comes expanded
+        dy = dy.contiguous()
+    dq, dk = _heads_like(q, B, H, L, D, q.dtype), _heads_like(k, B, Hkv, L, D, q.dtype)
+    dv = _heads_like(v, B, Hkv, L, Dv, q.dtype)
+    ds0 = None if initial_state is None else torch.empty((B, H, D, Dv), dtype=torch.float32, device=dev)
+    desc = _LA_DESC.pack(B, H, Hkv, L, D, Dv, io, dev.index, scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], 0, 0, 0)
+    grads = _LA_GRADS.pack(*dy.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])
+    work, wp, wn = _la_workspace(desc, 1, dev)
+    (ld, ldp), (s0, s0p), (ln, lnp), (ds1, ds1p) = (_plain(t) for t in (log_decay, initial_state, lengths, dfinal_state))
     _check(lib().sffft_linear_attention_backward(
-        ctypes.byref(desc), ctypes.byref(grads), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(), _ptr(ln), _ptr(s0),
-        dy.data_ptr(), _ptr(ds1), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ds0), _ptr(work),
-        0 if work is None else work.numel(), raw), f"linear_attention_backward(q {list(q.shape)}, v {list(v.shape)})")
-    _used_on(side, q, k, v, ld, s0, ln, dy, ds1, dq, dk, dv, ds0, work)
+        desc, grads, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldp, lnp, s0p, dy.data_ptr(), ds1p, dq.data_ptr(), dk.data_ptr(),
+        dv.data_ptr(), _ptr(ds0), wp, wn, _current(dev.index)), "linear_attention_backward")
     return dq, dk, dv, ds0
 
 
@@ -664,93 +669,122 @@ def linear_attention_check(device: int = 0):
     _check(lib().sffft_linear_attention_check(device), "device status")
 
 
-def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=1.0, stream=None):
+@_on_stream
+def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=1.0):
     """One token for each row: state[slot] <- lambda state[slot] + k v^T in place, y = scale state[slot]^T q.
 
     q [B][H][D], k [B][Hkv][D], v [B][Hkv][Dv]; state [pool][H][D][Dv] float32, of which only the slots' axis may have a
     stride of its own; slots [B] int32 (default: row b uses slot b).  A slot outside the pool marks a padded row, whose
     y is zero; so does a slot that an earlier row of the call has."""
-    import math
-
     import torch
-    _need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be [B][H][D], [B][Hkv][D] and [B][Hkv][Dv]")
-    B, H, D = q.shape
-    Hkv, Dv = k.shape[1], v.shape[2]
-    _need(tuple(k.shape) == (B, Hkv, D) and tuple(v.shape) == (B, Hkv, Dv),
-          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    _need(H > 0 and Hkv > 0 and H % Hkv == 0, f"{H} query heads cannot share {Hkv} key and value heads evenly")
-    _need(D > 0 and Dv > 0, "head sizes must be positive")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k and v must be [B][H][D], [B][Hkv][D] and [B][Hkv][Dv]")
+    (B, H, D), Hkv, Dv = q.shape, k.shape[1], v.shape[2]
+    if k.shape != (B, Hkv, D) or v.shape != (B, Hkv, Dv):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} key and value heads evenly")
+    if D < 1 or Dv < 1:
+        raise ValueError("head sizes must be positive")
     io = _io_of(q, "q")
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type")
-    _need(tuple(log_decay.shape) == (H,) and log_decay.dtype == torch.float32, f"log_decay must be a float32 [{H}] tensor")
-    _need(math.isfinite(scale), "scale must be finite")
-    _need(state.dim() == 4 and tuple(state.shape[1:]) == (H, D, Dv) and state.dtype == torch.float32,
-          f"state must be a float32 [pool, {H}, {D}, {Dv}] tensor")
-    _need(state.stride()[1:] == (D * Dv, Dv, 1) and (state.stride(0) >= H * D * Dv or state.shape[0] <= 1),
-          "a slot's state must be contiguous and slots must not overlap")
-    _need(slots is None or (tuple(slots.shape) == (B,) and slots.dtype == torch.int32), f"slots must be an int32 [{B}] tensor")
-    _need(slots is not None or state.shape[0] >= B, f"{B} rows need {B} slots")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one type")
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+        raise ValueError(f"log_decay must be a float32 [{H}] tensor")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if state.dim() != 4 or state.shape[1:] != (H, D, Dv) or state.dtype != torch.float32:
+        raise ValueError(f"state must be a float32 [pool, {H}, {D}, {Dv}] tensor")
+    pool, stride = state.shape[0], state.stride()
+    if not state[0:1].is_contiguous() or (pool > 1 and stride[0] < H * D * Dv):
+        raise ValueError("a slot's state must be contiguous and slots must not overlap")
+    if slots is not None and (slots.shape != (B,) or slots.dtype != torch.int32):
+        raise ValueError(f"slots must be an int32 [{B}] tensor")
+    if slots is None and pool < B:
+        raise ValueError(f"{B} rows need {B} slots")
+    dev = q.device
     for t in (k, v, log_decay, state, slots):
-        _need(t is None or t.device == q.device, "all tensors must be on one device")
-    _need(q.device.type == "cuda", "linear_attention_step needs CUDA tensors (there is no CPU path)")
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
+    _need_cuda(q, "linear_attention_step")
     q, k, v = _unit(q), _unit(k), _unit(v)
-    raw, side = _call_stream(stream, q.device)
-    y = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
-    d = LinearAttentionStepDesc(B, H, Hkv, D, Dv, state.shape[0], io, q.device.index, scale)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:], d.y_stride[:] = (t.stride()[:2] for t in (q, k, v, y))
-    d.state_stride = state.stride(0)
-    ld = log_decay.contiguous()
-    sl = None if slots is None else slots.contiguous()
-    _check(lib().sffft_linear_attention_step(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(),
-                                             state.data_ptr(), _ptr(sl), y.data_ptr(), raw),
-           f"linear_attention_step(q {list(q.shape)}, v {list(v.shape)})")
-    _used_on(side, q, k, v, ld, sl, state, y)
+    y = torch.empty((B, H, Dv), dtype=q.dtype, device=dev)
+    d = _LA_STEP.pack(B, H, Hkv, D, Dv, pool, io, dev.index, scale, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], H * Dv, Dv,
+                      stride[0])
+    (ld, ldp), (sl, slp) = _plain(log_decay), _plain(slots)
+    _check(lib().sffft_linear_attention_step(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldp, state.data_ptr(), slp,
+                                             y.data_ptr(), _current(dev.index)), "linear_attention_step")
     return y
 
 
 def check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
-    """(channels, kind of gate) of a block_norm call; raises ValueError where its arguments do not fit each other."""
-    import math
-
+    """Raises ValueError where the arguments of block_norm do not fit each other; else (channels, kind of gate, whether the
+    layout is [B][C][L])."""
     import torch
     lead = y if y is not None else x
-    _need(lead is not None, "block_norm needs x or y")
-    _need(dim in (-1, 1, lead.dim() - 1), "dim must be -1, or 1 for [B][C][L] tensors")
-    first = dim == 1 and lead.dim() != 2
-    _need(not first or lead.dim() == 3, "dim 1 is for [B][C][L] tensors")
-    _need(lead.dim() >= 1 and lead.shape[dim] > 0, "there must be channels")
-    C = lead.shape[dim]
+    if lead is None:
+        raise ValueError("block_norm needs x or y")
+    nd = lead.dim()
+    if dim not in (-1, 1, nd - 1):
+        raise ValueError("dim must be -1, or 1 for [B][C][L] tensors")
+    first = dim == 1 and nd != 2
+    if first and nd != 3:
+        raise ValueError("dim 1 is for [B][C][L] tensors")
+    if nd < 1 or lead.shape[dim] < 1:
+        raise ValueError("there must be channels")
+    C, dt, dev = lead.shape[dim], lead.dtype, lead.device
     if y is None:
-        _need(gate is None and post_weight is None, "a gate and post_weight act on y")
-        _need(weight is not None, "without y there must be a weight to norm x with")
-    io = _io_of(lead, "x" if y is None else "y")
+        if gate is not None or post_weight is not None:
+            raise ValueError("a gate and post_weight act on y")
+        if weight is None:
+            raise ValueError("without y there must be a weight to norm x with")
+    if dt != torch.float32 and dt != torch.bfloat16:
+        raise ValueError(f"the tensors must be float32 or bfloat16, not {dt}")
     if x is not None and y is not None:
-        _need(x.shape == y.shape, f"x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
-        _need(x.dtype == y.dtype or (x.dtype == torch.float32 and io == 1), "x must have y's type, or be float32 beside bfloat16")
+        if x.shape != y.shape:
+            raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
+        if x.dtype != dt and x.dtype != torch.float32:
+            raise ValueError("x must have y's type, or be float32 beside bfloat16")
+        if x.device != dev:
+            raise ValueError("all tensors must be on one device")
     kind = "none"
     if gate is not None:
-        kind = "full" if gate.shape == y.shape and gate.dim() > 1 or (gate.dim() == 1 and y.dim() == 1) else "channel"
-        _need(kind == "full" or tuple(gate.shape) == (C,), f"gate must be shaped like y or [{C}]")
-        _need(gate.dtype == y.dtype, "gate must have y's type")
+        kind = "full" if gate.shape == y.shape else "channel"
+        if kind == "channel" and gate.shape != (C,):
+            raise ValueError(f"gate must be shaped like y or [{C}]")
+        if gate.dtype != dt:
+            raise ValueError("gate must have y's type")
+        if gate.device != dev:
+            raise ValueError("all tensors must be on one device")
     for w, what in ((post_weight, "post_weight"), (weight, "weight")):
         if w is not None:
-            _need(tuple(w.shape) == (C,), f"{what} must be [{C}]")
-            _io_of(w, what)
-    _need(post_weight is None or weight is None or post_weight.dtype == weight.dtype, "the weights must have one type")
-    _need(groups >= 1 and C % groups == 0, f"{C} channels do not fall into {groups} groups")
-    _need(groups == 1 or post_weight is not None, "groups are those of the norm with post_weight")
-    _need(act in ACT, f"act must be one of {sorted(ACT)}")
-    _need(math.isfinite(scale), "scale must be finite")
-    _need(math.isfinite(eps) and eps >= 0, "eps must be finite and not negative")
-    for t in (x, gate, post_weight, weight):
-        _need(t is None or t.device == lead.device, "all tensors must be on one device")
+            if w.shape != (C,):
+                raise ValueError(f"{what} must be [{C}]")
+            if w.dtype != torch.float32 and w.dtype != torch.bfloat16:
+                raise ValueError(f"{what} must be float32 or bfloat16, not {w.dtype}")
+            if w.device != dev:
+                raise ValueError("all tensors must be on one device")
+    if post_weight is not None and weight is not None and post_weight.dtype != weight.dtype:
+        raise ValueError("the weights must have one type")
+    if groups < 1 or C % groups:
+        raise ValueError(f"{C} channels do not fall into {groups} groups")
+    if groups > 1 and post_weight is None:
+        raise ValueError("groups are those of the norm with post_weight")
+    if act not in ACT:
+        raise ValueError(f"act must be one of {sorted(ACT)}")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not math.isfinite(eps) or eps < 0:
+        raise ValueError("eps must be finite and not negative")
     return C, kind, first
 
 
 def _as_rows(t, C):
     """(tensor, stride of a row) of a [..., C] tensor whose rows are evenly spaced (a copy where they are not)."""
+    if t.is_contiguous():
+        return t, C
     if t.shape[-1] > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
+        return t.contiguous(), C
     step, rows = None, 1
     for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if n == 1:
@@ -758,88 +792,96 @@ def _as_rows(t, C):
         if step is None:
             step = s
         elif s != step * rows:
-            t = t.contiguous()
-            return t, C
+            return t.contiguous(), C
         rows *= n
     return t, C if step is None else step
 
 
 def _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
+    """(descriptor, x, y, gate, weights, the tensor that the outputs are like, kind of gate, rows)"""
+    import torch
     C, kind, first = check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     lead = y if y is not None else x
-    _need(lead.device.type == "cuda", "block_norm needs CUDA tensors (there is no CPU path)")
-    strides = [0, 0, 0]
-    ts = [x, y, gate]
-    for i, t in enumerate(ts):
-        if t is None or (i == 2 and kind == "channel"):
-            ts[i] = None if t is None else t.contiguous()
-        elif first:
-            ts[i] = t.contiguous()
-        else:
-            ts[i], strides[i] = _as_rows(t, C)
-    pw, w = (None if t is None else t.contiguous() for t in (post_weight, weight))
-    wio = _io_of(pw if pw is not None else w, "weight") if pw is not None or w is not None else 0
+    _need_cuda(lead, "block_norm")
+    xs = ys = gs = 0
+    if first:
+        x, y, gate = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, y, gate))
+    else:
+        if x is not None:
+            x, xs = _as_rows(x, C)
+        if y is not None:
+            y, ys = _as_rows(y, C)
+        if kind == "full":
+            gate, gs = _as_rows(gate, C)
+        elif gate is not None and not gate.is_contiguous():
+            gate = gate.contiguous()
+    pw, w = (t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, weight))
+    some = pw if pw is not None else w
+    bf = torch.bfloat16
     rows = lead.numel() // C
-    inner = lead.shape[2] if first else 0
-    d = BlockNormDesc(rows, C, inner, groups, _io_of(lead, "y"), _io_of(x if x is not None else lead, "x"), wio, GATE[kind],
-                      ACT[act], scale, eps, lead.device.index, *strides)
-    return d, ts, pw, w, lead, kind
+    d = _BN_DESC.pack(rows, C, lead.shape[2] if first else 0, groups, lead.dtype == bf, (lead if x is None else x).dtype == bf,
+                      some is not None and some.dtype == bf, GATE[kind], ACT[act], scale, eps, lead.device.index, xs, ys, gs)
+    return d, x, y, gate, pw, w, lead, kind, rows
 
 
+@_on_stream
 def block_norm(x=None, y=None, gate=None, post_weight=None, weight=None, scale=1.0, eps=1e-6, groups=1, act="none", dim=-1,
-               stats=False, stream=None):
+               stats=False):
     """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight, each part only where its
     tensor is given; rstd(z) = (mean z^2 + eps)^-1/2 over the channels (over each of `groups` runs of them for y).
 
     The channels are the last axis, or axis 1 of [B][C][L] tensors (`dim=1`, the layout of the convolution).  gate: shaped
     like y, or [C]; act: "none", "silu" or "sigmoid".  y, gate and n have one type (float32 or bfloat16); x and h have it
     too, or are float32.  Without y, h is x; without weight, n is None.  `stats=True` also returns the rstd of y's groups
-    and of h, for block_norm_backward."""
+    and of h, for block_norm_backward.  Runs on `stream` (default: the current one)."""
     import torch
-    d, (x, y, gate), pw, w, lead, _ = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
-    raw, side = _call_stream(stream, lead.device)
-    h = x if y is None else torch.empty(lead.shape, dtype=lead.dtype if x is None else x.dtype, device=lead.device)
-    n = None if w is None else torch.empty(lead.shape, dtype=lead.dtype, device=lead.device)
-    r1 = torch.empty((d.rows, groups), dtype=torch.float32, device=lead.device) if stats and pw is not None else None
-    r2 = torch.empty((d.rows,), dtype=torch.float32, device=lead.device) if stats and w is not None else None
-    if lead.numel():
-        _check(lib().sffft_block_norm(ctypes.byref(d), _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(h), _ptr(n),
-                                      _ptr(r1), _ptr(r2), raw), f"block_norm({list(lead.shape)})")
-    _used_on(side, x, y, gate, pw, w, h, n, r1, r2)
+    given = x
+    d, x, y, gate, pw, w, lead, _, rows = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    dev = lead.device
+    h = given if y is None else torch.empty(lead.shape, dtype=lead.dtype if x is None else x.dtype, device=dev)
+    n = None if w is None else torch.empty(lead.shape, dtype=lead.dtype, device=dev)
+    r1 = torch.empty((rows, groups), dtype=torch.float32, device=dev) if stats and pw is not None else None
+    r2 = torch.empty((rows,), dtype=torch.float32, device=dev) if stats and w is not None else None
+    if rows:
+        _check(lib().sffft_block_norm(d, _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(h), _ptr(n), _ptr(r1), _ptr(r2),
+                                      _current(dev.index)), "block_norm")
     return (h, n, r1, r2) if stats else (h, n)
 
 
-def block_norm_backward(dh, dn, x=None, y=None, gate=None, post_weight=None, weight=None, rstd_post=None, rstd=None, scale=1.0,
-                        eps=1e-6, groups=1, act="none", dim=-1, stream=None):
+@_on_stream
+def block_norm_backward(dh, dn, x=None, y=None, gate=None, post_weight=None, weight=None, rstd_post=None, rstd=None,
+                        scale=1.0, eps=1e-6, groups=1, act="none", dim=-1):
     """(dx, dy, dgate, dpost_weight, dweight) of block_norm from the gradients of h (None: zero) and n; None where the tensor
     was not given."""
     import torch
-    d, (x, y, gate), pw, w, lead, kind = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
-    _need(w is None or dn is not None, "dn is needed where there is a weight")
-    _need(dn is None or (dn.shape == lead.shape and dn.dtype == lead.dtype and w is not None), "dn must be like n")
-    ht = lead.dtype if x is None else x.dtype
-    _need(dh is None or (dh.shape == lead.shape and dh.dtype == ht), "dh must be like h")
-    _need(dh is not None or w is not None, "dh or dn is needed")
-    _need(pw is None or rstd_post is not None, "rstd_post of the forward pass is needed")
-    _need(w is None or rstd is not None, "rstd of the forward pass is needed")
+    d, x, y, gate, pw, w, lead, kind, rows = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    if (dn is None) != (w is None):
+        raise ValueError("dn is needed where there is a weight, and only there")
+    if dn is not None and (dn.shape != lead.shape or dn.dtype != lead.dtype):
+        raise ValueError("dn must be like n")
+    if dh is not None and (dh.shape != lead.shape or dh.dtype != (lead if x is None else x).dtype):
+        raise ValueError("dh must be like h")
+    if dh is None and w is None:
+        raise ValueError("dh or dn is needed")
+    for t, w_, n, what in ((rstd_post, pw, rows * groups, "rstd_post"), (rstd, w, rows, "rstd")):
+        if w_ is not None and (t is None or t.numel() != n or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{what} must be the forward pass's")
     for t in (dh, dn, rstd_post, rstd):
-        _need(t is None or t.device == lead.device, "all tensors must be on one device")
-    for t, n in ((rstd_post, d.rows * groups), (rstd, d.rows)):
-        _need(t is None or (t.numel() == n and t.dtype == torch.float32 and t.is_contiguous()), "rstd must be the forward pass's")
-    raw, side = _call_stream(stream, lead.device)
-    dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
-    new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)  # noqa: E731
-    dx, dy, dgate, dpw, dw = new(x), new(y), new(gate), new(pw), new(w)
-    need = ctypes.c_size_t()
-    _check(lib().sffft_block_norm_workspace_bytes(ctypes.byref(d), ctypes.byref(need)), "block_norm_workspace_bytes")
-    work = torch.empty(need.value, dtype=torch.uint8, device=lead.device) if need.value else None
-    if not lead.numel():   # no rows: empty buffers have no address to pass
+        if t is not None and t.device != lead.device:
+            raise ValueError("all tensors must be on one device")
+    dh, dn = (t if t is None or t.is_contiguous() else t.contiguous() for t in (dh, dn))
+    dev = lead.device
+    dx, dy, dgate, dpw, dw = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+                              for t in (x, y, gate, pw, w))
+    if not rows:   # empty buffers have no address to pass
         for t in (dgate if kind == "channel" else None, dpw, dw):
             if t is not None:
                 t.zero_()
         return dx, dy, dgate, dpw, dw
+    need = ctypes.c_size_t()
+    _check(lib().sffft_block_norm_workspace_bytes(d, ctypes.byref(need)), "block_norm_workspace_bytes")
+    work = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
     _check(lib().sffft_block_norm_backward(
-        ctypes.byref(d), _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(rstd_post), _ptr(rstd), _ptr(dh), _ptr(dn),
-        _ptr(dx), _ptr(dy), _ptr(dgate), _ptr(dpw), _ptr(dw), _ptr(work), need.value, raw), f"block_norm_backward({list(lead.shape)})")
-    _used_on(side, x, y, gate, pw, w, rstd_post, rstd, dh, dn, dx, dy, dgate, dpw, dw, work)
+        d, _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(rstd_post), _ptr(rstd), _ptr(dh), _ptr(dn), _ptr(dx), _ptr(dy),
+        _ptr(dgate), _ptr(dpw), _ptr(dw), _ptr(work), need.value, _current(dev.index)), "block_norm_backward")
     return dx, dy, dgate, dpw, dw

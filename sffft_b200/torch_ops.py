@@ -14,9 +14,10 @@
     h, n = sffft_b200.torch_ops.block_norm(x, y, gate, post_weight, weight)   # norms, gate, residual; with gradients
 
 All run on the current CUDA stream of the tensors' device through the C ABI, so they order with surrounding
-PyTorch work and can be captured in CUDA graphs once a first call has created the plan (plan creation allocates).  Fake implementations give output shapes and types without running
-anything, so the operators trace under torch.compile.  The convolution and the FFTs are forward only (the path has
-no backward kernel); linear_attention and block_norm have first derivatives.
+PyTorch work and can be captured in CUDA graphs (the convolution once a first call has created the plan: plan
+creation allocates).  Fake implementations give output shapes and types without running anything, so the operators
+trace under torch.compile.  The convolution and the FFTs are forward only (the path has no backward kernel);
+linear_attention and block_norm have first derivatives.
 
 `acc` is "fp32" or "fp16" (accumulation mode); `config` names a catalog plan ("" = the default for L).
 filter_spectrum and conv must use the same config: the spectrum is in that plan's digit order.
@@ -202,13 +203,34 @@ def _la_backward(ctx, dy, dfinal_state):
 _linear_attention.register_autograd(_la_backward, setup_context=_la_setup)
 
 
-def _plain_call(*tensors) -> bool:
-    """Whether the call needs neither a gradient nor a trace, so that the operator's dispatch can be left out."""
+def _eager(*tensors) -> bool:
+    """Whether the tensors are plain CUDA tensors outside of any trace: the call then goes straight to the C ABI, which saves
+    the operator's dispatch (tens of microseconds, and some hundreds with a gradient)."""
     if torch.compiler.is_compiling():
         return False
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return False
-    return all(t is None or type(t) in (Tensor, torch.nn.Parameter) and t.device.type == "cuda" for t in tensors)
+    return all(t is None or type(t) in (Tensor, torch.nn.Parameter) and t.is_cuda for t in tensors)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale):
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal_state):
+        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+        if dy is None:
+            dy = q.new_zeros((*q.shape[:3], v.shape[3]))
+        dq, dk, dv, ds = sf.linear_attention_backward(q, k, v, log_decay, dy, dfinal_state, ctx.scale, initial_state, lengths)
+        return dq, dk, dv, None, ds, None, None
 
 
 def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: float = 1.0,
@@ -217,7 +239,9 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: 
     head (see sffft_b200.linear_attention).  Differentiable in q, k, v and initial_state."""
     if log_decay.requires_grad:
         raise ValueError("log_decay is a constant: it has no gradient (pass log_decay.detach())")
-    if _plain_call(q, k, v, log_decay, initial_state, lengths):
+    if _eager(q, k, v, log_decay, initial_state, lengths):
+        if _wants_grad(q, k, v, initial_state):
+            return _LinearAttention.apply(q, k, v, log_decay, initial_state, lengths, scale)
         return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
     return _linear_attention(q, k, v, log_decay, initial_state, lengths, scale)
 
@@ -236,9 +260,9 @@ def _(q, k, v, log_decay, state, slots, scale):
 def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor] = None,
                           scale: float = 1.0) -> Tensor:
     """One token for each row, state[slot] updated in place (see sffft_b200.linear_attention_step).  No gradient."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if _wants_grad(q, k, v, log_decay, state):
         raise ValueError("linear_attention_step updates its state in place and has no gradient: use linear_attention, or no_grad")
-    if _plain_call(q, k, v, log_decay, state, slots):
+    if _eager(q, k, v, log_decay, state, slots):
         return sf.linear_attention_step(q, k, v, log_decay, state, slots, scale)
     return _linear_attention_step(q, k, v, log_decay, state, slots, scale)
 
@@ -309,13 +333,38 @@ def _bn_backward(ctx, grads):
 _block_norm.register_autograd(_bn_backward, setup_context=_bn_setup)
 
 
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, post_weight, weight, *rest):
+        h, n, rstd_post, rstd = sf.block_norm(x, y, gate, post_weight, weight, *rest, stats=True)
+        ctx.save_for_backward(x, y, gate, post_weight, weight, rstd_post, rstd)
+        ctx.rest = rest
+        ctx.set_materialize_grads(False)
+        return None if y is None else h, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dn):
+        x, y, gate, post_weight, weight, rstd_post, rstd = ctx.saved_tensors
+        lead = y if y is not None else x
+        if weight is not None and dn is None:
+            dn = torch.zeros_like(lead)
+        if weight is None and dh is None:
+            dh = torch.zeros_like(lead, dtype=lead.dtype if x is None else x.dtype)
+        return (*sf.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, *ctx.rest), *(None,) * 5)
+
+
 def block_norm(x: Optional[Tensor] = None, y: Optional[Tensor] = None, gate: Optional[Tensor] = None,
                post_weight: Optional[Tensor] = None, weight: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6,
                groups: int = 1, act: str = "none", dim: int = -1) -> tuple[Tensor, Optional[Tensor]]:
     """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight: the norms before and after a
     block with its gate and residual scale (see sffft_b200.block_norm).  Differentiable in all its tensors."""
-    if _plain_call(x, y, gate, post_weight, weight):
-        return sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    if _eager(x, y, gate, post_weight, weight):
+        if not _wants_grad(x, y, gate, post_weight, weight):
+            return sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+        if y is None:
+            return x, _BlockNorm.apply(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)[1]
+        return _BlockNorm.apply(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     out = _block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     h = x if y is None else out[0]
     return h, None if weight is None else out[0 if y is None else 1]
