@@ -420,91 +420,124 @@ __global__ void __launch_bounds__(TPR* RPB) norm_rows_bwd_kernel(const __grid_co
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Channels first: [B][C][L].  A block takes kPos positions of one row of the batch, all channels: kPos / VEC threads
-// across the positions, the others down the channels.  The sums over channels are taken by each thread for its own
-// positions and channels, then over the threads that share the positions, through shared memory.
+// Channels first: [B][C][L].  A block takes kPos positions of one row of the batch, all channels: a warp's lanes lie
+// across the positions, VEC each, and down 32 VEC / kPos channels, so that it reads whole 128-byte (bf16: 64-byte) pieces.
+//
+// Sums over a group's channels: each thread adds its own channels, lanes of a position are added by shuffles, warps
+// through shared memory.  With many groups (kManyGroups) each is left to one warp instead.
+//
+// Forward, y's tile is kept in shared memory in fp32 (then h's in its place) as long as it fits, so that y, x and gate are
+// read once.  Backward would have to keep five tiles; instead all three sums that a position needs are taken in one
+// reading,
+//   m = mean(t z),  A_g = sum_g s u (dh + rstd t),  B_g = sum_g s u z   (s = scale f post_weight):  sum_g s u dx = A - m B
+// and the second reading, which writes the results, finds the tile in L2: one block on each SM keeps 148 tiles at work,
+// 71 MB for 768 channels in fp32.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kPos = 32, kFirstThreads = 256;
+constexpr int kPos = 32, kFirstThreads = 512, kFirstWarps = kFirstThreads / 32, kManyGroups = 32;
 
 template <int VEC>
 struct FirstShape {
-  static constexpr int TX = kPos / VEC, TY = kFirstThreads / TX;
+  static constexpr int TX = kPos / VEC, TR = 32 / TX, TY = kFirstWarps * TR;   // lanes across, channels in a warp, in the block
 };
 
-// Sum over ty of each position's value; red: [TY][kPos].
-template <int VEC>
-__device__ __forceinline__ void first_sum(float (&s)[VEC], float* red, int tx, int ty) {
-  constexpr int TY = FirstShape<VEC>::TY;
-  __syncthreads();
+// Sums of N quantities over each group: `add(c, s)` adds channel c's to the thread's s[N][VEC].  out[k]: [groups][kPos].
+// part: [min(groups, kManyGroups - 1)][kFirstWarps][kPos] floats for each quantity.  Ends with the block in step.
+template <int VEC, int N, class F>
+__device__ __forceinline__ void first_sums(int groups, int gc, float* part, float* const (&out)[N], bool in, F add) {
+  using SH = FirstShape<VEC>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = lane % SH::TX, tr = lane / SH::TX;
+  const bool many = groups >= kManyGroups;
+  const int first = many ? tr : warp * SH::TR + tr, step = many ? SH::TR : SH::TY;
+  for (int g = many ? warp : 0; g < groups; g += many ? kFirstWarps : 1) {
+    float s[N][VEC] = {};
+    if (in)
+#pragma unroll 2
+      for (int c = first; c < gc; c += step) add(g * gc + c, s);
 #pragma unroll
-  for (int e = 0; e < VEC; e++) red[ty * kPos + tx * VEC + e] = s[e];
-  __syncthreads();
+    for (int k = 0; k < N; k++) {
 #pragma unroll
-  for (int e = 0; e < VEC; e++) {
-    float z = 0.f;
-    for (int q = 0; q < TY; q++) z += red[q * kPos + tx * VEC + e];
-    s[e] = z;
+      for (int e = 0; e < VEC; e++)
+#pragma unroll
+        for (int o = SH::TX; o < 32; o <<= 1) s[k][e] += __shfl_xor_sync(~0u, s[k][e], o);
+      if (tr == 0) {
+        float* to = many ? out[k] + g * kPos : part + ((k * groups + g) * kFirstWarps + warp) * kPos;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) to[tx * VEC + e] = s[k][e];
+      }
+    }
   }
+  __syncthreads();
+  if (many) return;
+  for (int i = threadIdx.x; i < N * groups * kPos; i += kFirstThreads) {
+    const int k = i / (groups * kPos), gp = i % (groups * kPos);
+    const float* from = part + ((k * groups + gp / kPos) * kFirstWarps) * kPos + gp % kPos;
+    float z = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFirstWarps; w++) z += from[w * kPos];
+    out[k][gp] = z;
+  }
+  __syncthreads();
+}
+
+__host__ __device__ inline int first_part_floats(int groups, int n) {
+  return groups >= kManyGroups ? kFirstWarps * kPos : n * groups * kFirstWarps * kPos;
 }
 
 struct FirstTile {
   long long base;   // element (channel 0, first position of the thread)
   long long row;    // row index of that position
-  int left;         // positions of the thread inside L
+  bool in;          // inside L (VEC 4: L is a multiple of 4)
 };
 
 template <int VEC>
-__device__ __forceinline__ FirstTile first_tile(const NormParams& p, long long tile, int tx) {
+__device__ __forceinline__ FirstTile first_tile(const NormParams& p, long long tile) {
   const int per = (p.inner + kPos - 1) / kPos;
   const long long b = tile / per;
-  const int l = (int)(tile % per) * kPos + tx * VEC;
-  return {b * p.C * p.inner + l, b * p.inner + l, l < p.inner ? min(VEC, p.inner - l) : 0};
+  const int l = (int)(tile % per) * kPos + (int)(threadIdx.x % FirstShape<VEC>::TX) * VEC;
+  return {b * p.C * p.inner + l, b * p.inner + l, l < p.inner};
 }
 
-template <class TX, class TY, int VEC>
+template <class TX, class TY, int VEC, bool KEEP>
 __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_constant__ NormParams p) {
-  constexpr int TXN = FirstShape<VEC>::TX, TYN = FirstShape<VEC>::TY;
+  using SH = FirstShape<VEC>;
   extern __shared__ __align__(16) float dyn[];
-  float* red = dyn;                 // [TYN][kPos]
-  float* r1 = dyn + TYN * kPos;     // [groups][kPos]
-  const int tx = threadIdx.x % TXN, ty = threadIdx.x / TXN;
-  const FirstTile ft = first_tile<VEC>(p, blockIdx.x, tx);
-  const bool in = ft.left > 0;   // VEC 4: L is a multiple of 4
+  float* r1 = dyn;                                     // [groups][kPos]
+  float* r2 = r1 + p.groups * kPos;                    // [kPos]
+  float* part = r2 + kPos;
+  float* tile = part + first_part_floats(p.groups, 1); // KEEP: [C][kPos]
+  const int tx = threadIdx.x % SH::TX, ty = threadIdx.x / SH::TX;
+  const FirstTile ft = first_tile<VEC>(p, blockIdx.x);
   const TY *y = (const TY*)p.y + ft.base, *gate = (const TY*)p.gate;
   const TX* x = (const TX*)p.x + ft.base;
   const long long L = p.inner;
   if (p.pw) {
-    for (int g = 0; g < p.groups; g++) {
-      float s[VEC] = {};
-      if (in)
-        for (int c = g * p.gc + ty; c < (g + 1) * p.gc; c += TYN) {
-          float v[VEC];
-          ldv<VEC>(y + c * L, v);
+    float* const out[1] = {r1};
+    first_sums<VEC, 1>(p.groups, p.gc, part, out, ft.in, [&](int c, float (&s)[1][VEC]) {
+      float v[VEC];
+      ldv<VEC>(y + c * L, v);
+      if (KEEP) stv<VEC>(tile + c * kPos + tx * VEC, v);
 #pragma unroll
-          for (int e = 0; e < VEC; e++) s[e] = fmaf(v[e], v[e], s[e]);
-        }
-      first_sum<VEC>(s, red, tx, ty);
-      if (ty == 0)
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const float rs = rsqrtf(s[e] / (float)p.gc + p.eps);
-          r1[g * kPos + tx * VEC + e] = rs;
-          if (p.r1 && in) p.r1[(ft.row + e) * p.groups + g] = rs;
-        }
-    }
+      for (int e = 0; e < VEC; e++) s[0][e] = fmaf(v[e], v[e], s[0][e]);
+    });
+    for (int i = threadIdx.x; i < p.groups * kPos; i += kFirstThreads) r1[i] = rsqrtf(r1[i] / (float)p.gc + p.eps);
     __syncthreads();
+    if (p.r1 && ft.in)
+      for (int g = ty; g < p.groups; g += SH::TY)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) p.r1[(ft.row + e) * p.groups + g] = r1[g * kPos + tx * VEC + e];
   }
   auto value = [&](int c, float (&h)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; e++) h[e] = 0.f;
     if (p.y) {
-      ldv<VEC>(y + c * L, h);
+      if (KEEP && p.pw) ldv<VEC>(tile + c * kPos + tx * VEC, h);
+      else ldv<VEC>(y + c * L, h);
       if (p.pw) {
         float w[1];
         ldw<1>(p.pw, p.w_bf16, c, w);
-        const int g = c / p.gc;
+        const float* r = r1 + (p.groups > 1 ? c / p.gc : 0) * kPos + tx * VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) h[e] *= r1[g * kPos + tx * VEC + e] * w[0];
+        for (int e = 0; e < VEC; e++) h[e] *= r[e] * w[0];
       }
       if (p.gate_kind) {
         float gv[VEC];
@@ -529,160 +562,159 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
       for (int e = 0; e < VEC; e++) h[e] += xv[e];
     }
   };
-  float s[VEC] = {};
-  if (in)
-    for (int c = ty; c < p.C; c += TYN) {
-      float h[VEC];
-      value(c, h);
-      if (p.h) stv<VEC>((TX*)p.h + ft.base + c * L, h);
+  if (!p.w) {
+    if (ft.in)
+      for (int c = ty; c < p.C; c += SH::TY) {
+        float h[VEC];
+        value(c, h);
+        stv<VEC>((TX*)p.h + ft.base + c * L, h);
+      }
+    return;
+  }
+  float* const out[1] = {r2};
+  first_sums<VEC, 1>(1, p.C, part, out, ft.in, [&](int c, float (&s)[1][VEC]) {
+    float h[VEC];
+    value(c, h);
+    if (p.h) stv<VEC>((TX*)p.h + ft.base + c * L, h);
+    if (KEEP) stv<VEC>(tile + c * kPos + tx * VEC, h);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) s[e] = fmaf(h[e], h[e], s[e]);
-    }
-  if (!p.w) return;
-  first_sum<VEC>(s, red, tx, ty);
-  if (!in) return;
+    for (int e = 0; e < VEC; e++) s[0][e] = fmaf(h[e], h[e], s[0][e]);
+  });
+  if (!ft.in) return;
+  float rs[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; e++) {
-    s[e] = rsqrtf(s[e] / (float)p.C + p.eps);
-    if (p.r2 && ty == 0) p.r2[ft.row + e] = s[e];
+    rs[e] = rsqrtf(r2[tx * VEC + e] / (float)p.C + p.eps);
+    if (p.r2 && ty == 0) p.r2[ft.row + e] = rs[e];
   }
-  for (int c = ty; c < p.C; c += TYN) {
+  for (int c = ty; c < p.C; c += SH::TY) {
     float h[VEC], w[1];
-    value(c, h);
+    if (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, h);
+    else value(c, h);
     ldw<1>(p.w, p.w_bf16, c, w);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) h[e] *= s[e] * w[0];
+    for (int e = 0; e < VEC; e++) h[e] *= rs[e] * w[0];
     stv<VEC>((TY*)p.n + ft.base + c * L, h);
   }
 }
 
 template <class TX, class TY, int VEC>
 __global__ void __launch_bounds__(kFirstThreads) norm_first_bwd_kernel(const __grid_constant__ NormParams p) {
-  constexpr int TXN = FirstShape<VEC>::TX, TYN = FirstShape<VEC>::TY;
+  using SH = FirstShape<VEC>;
   extern __shared__ __align__(16) float dyn[];
-  float* red = dyn;                     // [TYN][kPos]
-  float* m1 = dyn + TYN * kPos;         // [groups][kPos]
-  const int tx = threadIdx.x % TXN, ty = threadIdx.x / TXN;
+  float* sA = dyn;                           // [groups][kPos]
+  float* sB = sA + p.groups * kPos;
+  float* sM = sB + p.groups * kPos;          // [groups][kPos], then [kPos]
+  float* part = sM + p.groups * kPos;
+  const int tx = threadIdx.x % SH::TX, ty = threadIdx.x / SH::TX;
   float* out = p.part + (long long)blockIdx.x * 3 * p.C;   // this block's sums; a channel always belongs to one ty
   const long long L = p.inner;
   const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
   const TY* gate = (const TY*)p.gate;
   bool first = true;
   for (long long tile = blockIdx.x; tile < tiles; tile += p.blocks, first = false) {
-    const FirstTile ft = first_tile<VEC>(p, tile, tx);
-    const bool in = ft.left > 0;
+    const FirstTile ft = first_tile<VEC>(p, tile);
     float r2[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; e++) r2[e] = p.w && in ? p.r2[ft.row + e] : 0.f;
-    // u, a = u * post_weight, gate, z and dh + rstd t of channel c
-    auto load = [&](int c, float (&u)[VEC], float& pw, float (&gv)[VEC], float (&z)[VEC], float (&d)[VEC], float (&tn)[VEC],
-                    float& w, float (&q1)[VEC]) {
+    for (int e = 0; e < VEC; e++) r2[e] = p.w && ft.in ? p.r2[ft.row + e] : 0.f;
+    struct Values {
+      float u[VEC], f[VEC], df[VEC], z[VEC], d[VEC], tn[VEC], q[VEC];   // d: dh + rstd t;  q: rstd of y's group
+      float pw, w;
+    };
+    auto load = [&](int c, Values& v, bool with_df) {
+      float gv[VEC], xv[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) u[e] = z[e] = d[e] = tn[e] = 0.f, gv[e] = 1.f, q1[e] = 1.f;
-      pw = 1.f;
-      w = 0.f;
-      if (p.y) {
-        ldv<VEC>((const TY*)p.y + ft.base + c * L, u);
-        if (p.pw) {
-          float t[1];
-          ldw<1>(p.pw, p.w_bf16, c, t);
-          pw = t[0];
-          const int g = c / p.gc;
+      for (int e = 0; e < VEC; e++) v.u[e] = v.d[e] = v.tn[e] = xv[e] = 0.f, v.f[e] = v.q[e] = 1.f, v.df[e] = 0.f;
+      v.pw = 1.f;
+      v.w = 0.f;
+      float t[1];
+      if (p.y) ldv<VEC>((const TY*)p.y + ft.base + c * L, v.u);
+      if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
+      else if (p.gate_kind == GATE_CHANNEL)
 #pragma unroll
-          for (int e = 0; e < VEC; e++) {
-            q1[e] = p.r1[(ft.row + e) * p.groups + g];
-            u[e] *= q1[e];
-          }
-        }
-        if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
-        else if (p.gate_kind == GATE_CHANNEL)
-#pragma unroll
-          for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
-      }
-      if (p.dh) ldv<VEC>((const TX*)p.dh + ft.base + c * L, d);
+        for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
+      if (p.dh) ldv<VEC>((const TX*)p.dh + ft.base + c * L, v.d);
       if (p.w) {
-        float t[1];
+        if (p.x) ldv<VEC>((const TX*)p.x + ft.base + c * L, xv);
+        ldv<VEC>((const TY*)p.dn + ft.base + c * L, v.tn);
         ldw<1>(p.w, p.w_bf16, c, t);
-        w = t[0];
-        if (p.x) ldv<VEC>((const TX*)p.x + ft.base + c * L, z);
-        ldv<VEC>((const TY*)p.dn + ft.base + c * L, tn);
+        v.w = t[0];
+      }
+      if (p.pw) {
+        ldw<1>(p.pw, p.w_bf16, c, t);
+        v.pw = t[0];
+        const float* r = p.r1 + ft.row * p.groups + (p.groups > 1 ? c / p.gc : 0);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
-          if (p.y) {
-            float f = 1.f;
-            if (p.gate_kind) act_fwd(p.act, gv[e], f);
-            z[e] = fmaf(p.scale * f, u[e] * pw, z[e]);
-          }
-          z[e] *= r2[e];
-          d[e] = fmaf(r2[e], tn[e] * w, d[e]);
+          v.q[e] = r[e * p.groups];
+          v.u[e] *= v.q[e];
         }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        if (p.gate_kind) {
+          if (with_df) act_both(p.act, gv[e], v.f[e], v.df[e]);
+          else act_fwd(p.act, gv[e], v.f[e]);
+        }
+        v.z[e] = (p.y ? fmaf(p.scale * v.f[e], v.u[e] * v.pw, xv[e]) : xv[e]) * r2[e];
+        v.d[e] = fmaf(r2[e], v.tn[e] * v.w, v.d[e]);
       }
     };
-    float u[VEC], gv[VEC], z[VEC], d[VEC], tn[VEC], q1[VEC], pw, w;
-    float m2[VEC] = {};
-    if (p.w) {
-      if (in)
-        for (int c = ty; c < p.C; c += TYN) {
-          load(c, u, pw, gv, z, d, tn, w, q1);
+    if (p.w || p.pw) {
+      float* const sums[3] = {sA, sB, sM};
+      first_sums<VEC, 3>(p.groups, p.gc, part, sums, ft.in, [&](int c, float (&s)[3][VEC]) {
+        Values v;
+        load(c, v, false);
 #pragma unroll
-          for (int e = 0; e < VEC; e++) m2[e] = fmaf(tn[e] * w, z[e], m2[e]);
+        for (int e = 0; e < VEC; e++) {
+          const float su = p.scale * v.f[e] * v.pw * v.u[e];
+          s[0][e] = fmaf(su, v.d[e], s[0][e]);
+          s[1][e] = fmaf(su, v.z[e], s[1][e]);
+          s[2][e] = fmaf(v.tn[e] * v.w, v.z[e], s[2][e]);
         }
-      first_sum<VEC>(m2, red, tx, ty);
-#pragma unroll
-      for (int e = 0; e < VEC; e++) m2[e] *= r2[e] / (float)p.C;
-    }
-    if (p.y && p.pw) {
-      for (int g = 0; g < p.groups; g++) {
-        float s[VEC] = {};
-        if (in)
-          for (int c = g * p.gc + ty; c < (g + 1) * p.gc; c += TYN) {
-            load(c, u, pw, gv, z, d, tn, w, q1);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-              float f = 1.f;
-              if (p.gate_kind) act_fwd(p.act, gv[e], f);
-              s[e] = fmaf(p.scale * f * fmaf(-m2[e], z[e], d[e]) * pw, u[e], s[e]);
-            }
-          }
-        first_sum<VEC>(s, red, tx, ty);
-        if (ty == 0)
-#pragma unroll
-          for (int e = 0; e < VEC; e++) m1[g * kPos + tx * VEC + e] = s[e] / (float)p.gc;
+      });
+      if (p.groups > 1) {
+        float m = 0.f;
+        if (threadIdx.x < kPos)
+          for (int g = 0; g < p.groups; g++) m += sM[g * kPos + threadIdx.x];
+        __syncthreads();
+        if (threadIdx.x < kPos) sM[threadIdx.x] = m;
+        __syncthreads();
       }
-      __syncthreads();
     }
-    for (int c = ty; c < p.C; c += TYN) {
+    float m2[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) m2[e] = p.w ? sM[tx * VEC + e] * r2[e] / (float)p.C : 0.f;
+    for (int c = ty; c < p.C; c += SH::TY) {
       float sw = 0.f, sp = 0.f, sg = 0.f;
-      if (in) {
-        load(c, u, pw, gv, z, d, tn, w, q1);
+      if (ft.in) {
+        Values v;
+        load(c, v, true);
         float dg[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
-          sw = fmaf(tn[e], z[e], sw);
-          d[e] = fmaf(-m2[e], z[e], d[e]);
+          sw = fmaf(v.tn[e], v.z[e], sw);
+          v.d[e] = fmaf(-m2[e], v.z[e], v.d[e]);
         }
-        if (p.dx) stv<VEC>((TX*)p.dx + ft.base + c * L, d);
+        if (p.dx) stv<VEC>((TX*)p.dx + ft.base + c * L, v.d);
         if (p.y) {
-          const int g = c / p.gc;
+          const int g = (p.groups > 1 ? c / p.gc : 0) * kPos + tx * VEC;
 #pragma unroll
           for (int e = 0; e < VEC; e++) {
-            float f = 1.f, df = 0.f;
-            if (p.gate_kind) act_both(p.act, gv[e], f, df);
-            dg[e] = p.scale * d[e] * u[e] * pw * df;
+            dg[e] = p.scale * v.d[e] * v.u[e] * v.pw * v.df[e];
             sg += dg[e];
-            const float da = p.scale * f * d[e];
-            sp = fmaf(da, u[e], sp);
-            d[e] = p.pw ? q1[e] * fmaf(-m1[g * kPos + tx * VEC + e], u[e], da * pw) : da;
+            const float da = p.scale * v.f[e] * v.d[e];
+            sp = fmaf(da, v.u[e], sp);
+            v.d[e] = p.pw ? v.q[e] * fmaf(-fmaf(-m2[e], sB[g + e], sA[g + e]) / (float)p.gc, v.u[e], da * v.pw) : da;
           }
           if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + ft.base + c * L, dg);
-          stv<VEC>((TY*)p.dy + ft.base + c * L, d);
+          stv<VEC>((TY*)p.dy + ft.base + c * L, v.d);
         }
       }
-      // the TXN threads of a channel are neighbouring lanes (TXN divides 32); lanes of a warp whose channel is
-      // beyond C have left the loop together with their whole group
-      const unsigned mask = TXN == 32 ? ~0u : ((1u << TXN) - 1) << ((threadIdx.x & 31) / TXN * TXN);
+      // the TX lanes of a channel are neighbours; lanes of a warp whose channel is beyond C have left together
+      const unsigned mask = SH::TX == 32 ? ~0u : ((1u << SH::TX) - 1) << ((threadIdx.x & 31) / SH::TX * SH::TX);
 #pragma unroll
-      for (int o = TXN / 2; o; o >>= 1) {
+      for (int o = SH::TX / 2; o; o >>= 1) {
         sw += __shfl_xor_sync(mask, sw, o);
         sp += __shfl_xor_sync(mask, sp, o);
         sg += __shfl_xor_sync(mask, sg, o);
@@ -724,6 +756,7 @@ __global__ void __launch_bounds__(256) norm_part_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int kMaxShared = 227 * 1024;
 constexpr int kMaxChannels = 8192;   // what a block's registers hold in the backward pass
 
 template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
@@ -752,10 +785,15 @@ cudaError_t rows_v(const NormParams& p, bool bwd, cudaStream_t st) {
 
 template <class TX, class TY, int VEC>
 cudaError_t first_v(const NormParams& p, bool bwd, cudaStream_t st) {
-  const int smem = 4 * (FirstShape<VEC>::TY * kPos + p.groups * kPos);
   const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
-  if (bwd) return launch(norm_first_bwd_kernel<TX, TY, VEC>, dim3((unsigned)p.blocks), kFirstThreads, smem, st, p);
-  return launch(norm_first_kernel<TX, TY, VEC>, dim3((unsigned)tiles), kFirstThreads, smem, st, p);
+  if (bwd) {
+    const int smem = 4 * (3 * p.groups * kPos + first_part_floats(p.groups, 3));
+    return launch(norm_first_bwd_kernel<TX, TY, VEC>, dim3((unsigned)p.blocks), kFirstThreads, smem, st, p);
+  }
+  const int smem = 4 * ((p.groups + 1) * kPos + first_part_floats(p.groups, 1)), kept = smem + 4 * p.C * kPos;
+  if (kept <= kMaxShared)
+    return launch(norm_first_kernel<TX, TY, VEC, true>, dim3((unsigned)tiles), kFirstThreads, kept, st, p);
+  return launch(norm_first_kernel<TX, TY, VEC, false>, dim3((unsigned)tiles), kFirstThreads, smem, st, p);
 }
 
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -803,7 +841,7 @@ int check(const sffft_block_norm_t* d, const void* x, const void* y, const void*
 
 int backward_blocks(const sffft_block_norm_t* d, int sms) {
   const long long units = d->inner ? (d->rows / d->inner) * ((d->inner + kPos - 1) / kPos) : d->rows;
-  const long long most = 4ll * sms;
+  const long long most = d->inner ? sms : 4ll * sms;
   return (int)(units < most ? units : most);
 }
 
