@@ -30,6 +30,8 @@ int sffft_note_cuda_error(cudaError_t e);
 namespace sffft {
 namespace {
 
+constexpr int kMaxChannels = 8192;   // what a block's registers hold in the backward pass
+
 enum { GATE_NONE = 0, GATE_FULL = 1, GATE_CHANNEL = 2 };
 
 struct NormParams {
@@ -124,126 +126,182 @@ __device__ __forceinline__ void act_both(int act, float g, float& f, float& df) 
   }
 }
 
-// Sum over the threads of a row: a warp (TPR = 32), or the block.  `red` holds a float for each warp.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float s, float* red) {
+// ---------------------------------------------------------------------------------------------------------------
+// Rows of contiguous channels.  A row's threads (a warp, or a block) hold VEC x NV channels each.  Bound by memory; what
+// costs is latency: a row is a chain of loads, sums over its threads and stores.  So all of a row's loads are issued before
+// the first use (they are kept as they come, RawV), backward also the next row's before this one's arithmetic, and the sums
+// that backward needs are taken together: with s = scale f post_weight,
+//   m = sum t z,  A_g = sum_g s u (dh + rstd t),  B_g = sum_g s u z   give   sum_g s u dx = A_g - rstd m / C * B_g.
+// ---------------------------------------------------------------------------------------------------------------
+template <class T, int VEC>
+struct RawV {
+  static constexpr int bytes = VEC * (int)sizeof(T);
+  uint32_t w[(bytes + 3) / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (bytes >= 16) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  if constexpr (TPR > 32) {
-    __syncthreads();   // earlier readers of red
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = red[threadIdx.x & (TPR / 32 - 1)];
-#pragma unroll
-    for (int o = TPR / 64; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+      for (int i = 0; i < bytes / 16; i++) {
+        const uint4 a = ((const uint4*)p)[i];
+        w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
+      }
+    } else if constexpr (bytes == 4) {
+      w[0] = *(const uint32_t*)p;
+    } else {
+      w[0] = (uint32_t) * (const uint16_t*)p << 16;
+    }
   }
-  return s;
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& x : w) x = 0;
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[i] = __uint_as_float(w[i]);
+    } else if constexpr (VEC == 1) {
+      v[0] = __uint_as_float(w[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) unpack(w[i / 2], v[i], v[i + 1]);
+    }
+  }
+};
+
+// N sums over the threads of a row: a warp, or (BLOCK) the nw warps of the block, through red[2][N][32], whose halves take
+// turns (`turn`), so that one barrier does.
+template <bool BLOCK, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float* red, int nw, int& turn) {
+#pragma unroll
+  for (int k = 0; k < N; k++)
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s[k] += __shfl_xor_sync(~0u, s[k], o);
+  if constexpr (BLOCK) {
+    float* r = red + turn * N * 32;
+    turn ^= 1;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+      for (int k = 0; k < N; k++) r[k * 32 + (threadIdx.x >> 5)] = s[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      s[k] = lane < nw ? r[k * 32 + lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s[k] += __shfl_xor_sync(~0u, s[k], o);
+    }
+  }
 }
 
-template <int TPR>
+template <bool BLOCK>
 __device__ __forceinline__ void row_sync() {
-  if constexpr (TPR > 32) __syncthreads();
+  if constexpr (BLOCK) __syncthreads();
   else __syncwarp();
 }
 
-// Sums over the groups of channels: v[j] is the sum over the thread's j-th vector, replaced by its group's sum.  Where
+// Sums over several groups of channels: v[j] is the sum over the thread's j-th vector, replaced by its group's sum.  Where
 // a group is a power of two of at most 32 vectors its vectors lie in neighbouring lanes (a row's threads start at a
 // multiple of 32); otherwise the vectors' sums go through shared memory, one warp adding up a group.
-template <int TPR, int NV>
-__device__ __forceinline__ void group_sums(float (&v)[NV], int nvec, int per, int groups, float* vec, float* grp, float* red,
-                                           int t) {
-  if (groups == 1) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; j++) s += v[j];
-    s = row_sum<TPR>(s, red);
-#pragma unroll
-    for (int j = 0; j < NV; j++) v[j] = s;
-    return;
-  }
+template <bool BLOCK, int NV>
+__device__ __forceinline__ void group_sums(float (&v)[NV], int nvec, int per, int groups, float* vec, int t, int tpr) {
   if (per <= 32 && (per & (per - 1)) == 0) {
 #pragma unroll
     for (int j = 0; j < NV; j++)
       for (int o = per >> 1; o; o >>= 1) v[j] += __shfl_xor_sync(~0u, v[j], o);
     return;
   }
-  row_sync<TPR>();
+  float* grp = vec + nvec;
+  row_sync<BLOCK>();
 #pragma unroll
   for (int j = 0; j < NV; j++)
-    if (j * TPR + t < nvec) vec[j * TPR + t] = v[j];
-  row_sync<TPR>();
-  for (int g = t >> 5; g < groups; g += TPR / 32) {
+    if (j * tpr + t < nvec) vec[j * tpr + t] = v[j];
+  row_sync<BLOCK>();
+  for (int g = t >> 5; g < groups; g += tpr >> 5) {
     float s = 0.f;
     for (int e = t & 31; e < per; e += 32) s += vec[g * per + e];
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if ((t & 31) == 0) grp[g] = s;
   }
-  row_sync<TPR>();
+  row_sync<BLOCK>();
 #pragma unroll
-  for (int j = 0; j < NV; j++) v[j] = j * TPR + t < nvec ? grp[(j * TPR + t) / per] : 0.f;
+  for (int j = 0; j < NV; j++) v[j] = j * tpr + t < nvec ? grp[(j * tpr + t) / per] : 0.f;
 }
 
-// Shared memory of a block's rows: vector sums and group sums (only where group_sums needs them), 32 floats for row_sum.
+// Shared memory of a row: vector sums and group sums (only where group_sums needs them).
 __host__ __device__ inline int rows_smem_floats(int nvec, int groups) { return groups > 1 ? nvec + groups : 0; }
 
-template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
-__global__ void __launch_bounds__(TPR* RPB) norm_rows_kernel(const __grid_constant__ NormParams p) {
+constexpr int kRowsPerBlock = 4;   // where a row is a warp's
+
+template <class TX, class TY, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 32 * kRowsPerBlock) norm_rows_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) float dyn[];
-  __shared__ float red[32];
-  const int t = threadIdx.x % TPR, nvec = p.C / VEC;
-  float* vec = dyn + (threadIdx.x / TPR) * rows_smem_floats(nvec, p.groups);
-  float* grp = vec + nvec;
-  const long long r = blockIdx.x * (long long)RPB + threadIdx.x / TPR;
-  if (r >= p.rows) return;   // whole warps (RPB > 1 only with TPR = 32)
-  float v[NV][VEC], a[NV][VEC];
-  const TY* y = (const TY*)p.y + r * p.ys;
+  __shared__ float red[2 * 32];
+  const int tpr = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nvec = p.C / VEC;
+  const int sub = BLOCK ? 0 : threadIdx.x >> 5, nw = tpr >> 5, per = p.gc / VEC;
+  float* vec = dyn + sub * rows_smem_floats(nvec, p.groups);
+  const long long r = BLOCK ? (long long)blockIdx.x : blockIdx.x * (long long)kRowsPerBlock + sub;
+  if (r >= p.rows) return;   // whole warps
+  int turn = 0;
+  RawV<TY, VEC> ry[NV], rg[NV];
+  RawV<TX, VEC> rx[NV];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    const int i = j * TPR + t;
-#pragma unroll
-    for (int e = 0; e < VEC; e++) v[j][e] = 0.f;
-    if (p.y && i < nvec) ldv<VEC>(y + i * VEC, v[j]);
-  }
-  if (p.x) {
-    const TX* x = (const TX*)p.x + r * p.xs;
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-      const int i = j * TPR + t;
-      if (i < nvec) ldv<VEC>(x + i * VEC, a[j]);
+    const int i = j * tpr + t;
+    ry[j].zero(), rg[j].zero(), rx[j].zero();
+    if (i < nvec) {
+      if (p.y) ry[j].load((const TY*)p.y + r * p.ys + i * VEC);
+      if (p.x) rx[j].load((const TX*)p.x + r * p.xs + i * VEC);
+      if (p.gate_kind) rg[j].load((const TY*)p.gate + r * p.gs + i * VEC);
     }
   }
+  float v[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; j++) ry[j].get(v[j]);
   if (p.pw) {
-    float s[NV];
+    float s[NV], all[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       s[j] = 0.f;
 #pragma unroll
       for (int e = 0; e < VEC; e++) s[j] = fmaf(v[j][e], v[j][e], s[j]);
+      all[0] += s[j];
     }
-    const int per = p.gc / VEC;
-    group_sums<TPR, NV>(s, nvec, per, p.groups, vec, grp, red, t);
+    if (p.groups == 1) {
+      row_sums<BLOCK, 1>(all, red, nw, turn);
+#pragma unroll
+      for (int j = 0; j < NV; j++) s[j] = all[0];
+    } else {
+      group_sums<BLOCK, NV>(s, nvec, per, p.groups, vec, t, tpr);
+    }
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = j * TPR + t;
+      const int i = j * tpr + t;
       if (i >= nvec) continue;
       const float rs = rsqrtf(s[j] / (float)p.gc + p.eps);
-      if (p.r1 && i % per == 0) p.r1[r * p.groups + i / per] = rs;
+      if (p.r1) {
+        if (p.groups == 1) {
+          if (i == 0) p.r1[r] = rs;
+        } else if (i % per == 0) {
+          p.r1[r * p.groups + i / per] = rs;
+        }
+      }
       float w[VEC];
       ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
 #pragma unroll
       for (int e = 0; e < VEC; e++) v[j][e] *= rs * w[e];
     }
   }
-  float ss = 0.f;
+  float ss[1] = {0.f};
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    const int i = j * TPR + t;
+    const int i = j * tpr + t;
     if (i >= nvec) continue;
+    float a[VEC];
+    rx[j].get(a);
     if (p.y) {
       if (p.gate_kind) {
         float g[VEC];
-        ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
+        rg[j].get(g);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
           float f;
@@ -252,22 +310,22 @@ __global__ void __launch_bounds__(TPR* RPB) norm_rows_kernel(const __grid_consta
         }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v[j][e] = p.x ? fmaf(p.scale, v[j][e], a[j][e]) : p.scale * v[j][e];
-      if (p.h) stv<VEC>((TX*)p.h + r * p.C + i * VEC, v[j]);
+      for (int e = 0; e < VEC; e++) v[j][e] = fmaf(p.scale, v[j][e], a[e]);
+      stv<VEC>((TX*)p.h + r * p.C + i * VEC, v[j]);
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v[j][e] = a[j][e];
+      for (int e = 0; e < VEC; e++) v[j][e] = a[e];
     }
 #pragma unroll
-    for (int e = 0; e < VEC; e++) ss = fmaf(v[j][e], v[j][e], ss);
+    for (int e = 0; e < VEC; e++) ss[0] = fmaf(v[j][e], v[j][e], ss[0]);
   }
   if (!p.w) return;
-  ss = row_sum<TPR>(ss, red);
-  const float rs = rsqrtf(ss / (float)p.C + p.eps);
+  row_sums<BLOCK, 1>(ss, red, nw, turn);
+  const float rs = rsqrtf(ss[0] / (float)p.C + p.eps);
   if (p.r2 && t == 0) p.r2[r] = rs;
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    const int i = j * TPR + t;
+    const int i = j * tpr + t;
     if (i >= nvec) continue;
     float w[VEC];
     ldw<VEC>(p.w, p.w_bf16, i * VEC, w);
@@ -277,134 +335,153 @@ __global__ void __launch_bounds__(TPR* RPB) norm_rows_kernel(const __grid_consta
   }
 }
 
-template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
-__global__ void __launch_bounds__(TPR* RPB) norm_rows_bwd_kernel(const __grid_constant__ NormParams p) {
+template <class TX, class TY, int VEC, int NV>
+struct RawRow {
+  RawV<TY, VEC> y[NV], g[NV], dn[NV];
+  RawV<TX, VEC> x[NV], dh[NV];
+  float r1[NV], r2;
+  __device__ __forceinline__ void load(const NormParams& p, long long r, int t, int tpr, int nvec, const int (&grp)[NV]) {
+    r2 = p.w ? p.r2[r] : 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = j * tpr + t;
+      y[j].zero(), g[j].zero(), dn[j].zero(), x[j].zero(), dh[j].zero();
+      r1[j] = 1.f;
+      if (i >= nvec) continue;
+      if (p.y) y[j].load((const TY*)p.y + r * p.ys + i * VEC);
+      if (p.gate_kind == GATE_FULL) g[j].load((const TY*)p.gate + r * p.gs + i * VEC);
+      if (p.dh) dh[j].load((const TX*)p.dh + r * p.C + i * VEC);
+      if (p.w) {
+        if (p.x) x[j].load((const TX*)p.x + r * p.xs + i * VEC);
+        dn[j].load((const TY*)p.dn + r * p.C + i * VEC);
+      }
+      if (p.pw) r1[j] = p.r1[r * p.groups + grp[j]];
+    }
+  }
+};
+
+// Threads of a row in the backward pass: 512 at most, which leaves each 128 registers.
+template <class TX, class TY, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr bool AHEAD = NV == 1;   // registers for the next row
   extern __shared__ __align__(16) float dyn[];
-  __shared__ float red[32];
-  const int t = threadIdx.x % TPR, nvec = p.C / VEC, per = p.gc / VEC, sub = threadIdx.x / TPR;
+  __shared__ float red[2 * 3 * 32];
+  const int tpr = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nvec = p.C / VEC;
+  const int sub = BLOCK ? 0 : threadIdx.x >> 5, nw = tpr >> 5, per = p.gc / VEC;
   float* vec = dyn + sub * rows_smem_floats(nvec, p.groups);
-  float* grp = vec + nvec;
+  int turn = 0, grp[NV];
   float sw[NV][VEC], sp[NV][VEC], sg[NV][VEC];
 #pragma unroll
-  for (int j = 0; j < NV; j++)
+  for (int j = 0; j < NV; j++) {
+    grp[j] = p.groups > 1 ? min((j * tpr + t) / per, p.groups - 1) : 0;
 #pragma unroll
     for (int e = 0; e < VEC; e++) sw[j][e] = sp[j][e] = sg[j][e] = 0.f;
+  }
+  const long long step = BLOCK ? (long long)p.blocks : (long long)p.blocks * kRowsPerBlock;
+  long long r = BLOCK ? (long long)blockIdx.x : blockIdx.x * (long long)kRowsPerBlock + sub;
+  RawRow<TX, TY, VEC, NV> now, next;
+  if (r < p.rows) now.load(p, r, t, tpr, nvec, grp);
+  const float inv_c = 1.f / (float)p.C, inv_g = 1.f / (float)p.gc;
 
-  for (long long r = blockIdx.x * (long long)RPB + sub; r < p.rows; r += (long long)p.blocks * RPB) {
-    const float r2 = p.w ? p.r2[r] : 0.f;
-    float u[NV][VEC], z[NV][VEC], d[NV][VEC];   // u, then s u's parts; h, then z; dx
-    float s = 0.f;
+  for (; r < p.rows; r += step) {
+    if (AHEAD && r + step < p.rows) next.load(p, r + step, t, tpr, nvec, grp);
+    float u[NV][VEC], z[NV][VEC], d[NV][VEC], s[NV][VEC];   // d: dh + rstd t, then dx;  s: scale f post_weight
+    float A[NV], B[NV], sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = j * TPR + t;
+      const int i = j * tpr + t;
+      float x[VEC], tn[VEC], w[VEC], pw[VEC], g[VEC];
+      now.y[j].get(u[j]);
+      now.x[j].get(x);
+      now.dn[j].get(tn);
+      now.dh[j].get(d[j]);
+      now.g[j].get(g);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) d[j][e] = z[j][e] = u[j][e] = 0.f;
-      if (i >= nvec) continue;
-      float a[VEC], f[VEC];
-      if (p.y) {
-        ldv<VEC>((const TY*)p.y + r * p.ys + i * VEC, u[j]);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) a[e] = u[j][e];
-        if (p.pw) {
-          const float r1 = p.r1[r * p.groups + i / per];
-          float w[VEC];
-          ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
-#pragma unroll
-          for (int e = 0; e < VEC; e++) {
-            u[j][e] *= r1;
-            a[e] = u[j][e] * w[e];
-          }
-        }
-        if (p.gate_kind) {
-          float g[VEC];
-          ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
-#pragma unroll
-          for (int e = 0; e < VEC; e++) act_fwd(p.act, g[e], f[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; e++) f[e] = 1.f;
-        }
+      for (int e = 0; e < VEC; e++) w[e] = 0.f, pw[e] = 1.f;
+      if (i < nvec) {
+        if (p.w) ldw<VEC>(p.w, p.w_bf16, i * VEC, w);
+        if (p.pw) ldw<VEC>(p.pw, p.w_bf16, i * VEC, pw);
+        if (p.gate_kind == GATE_CHANNEL) ldv<VEC>((const TY*)p.gate + i * VEC, g);
       }
-      if (p.dh) ldv<VEC>((const TX*)p.dh + r * p.C + i * VEC, d[j]);
+      A[j] = B[j] = 0.f;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        u[j][e] *= now.r1[j];
+        float f = 1.f;
+        if (p.gate_kind) act_fwd(p.act, g[e], f);
+        s[j][e] = p.scale * f * pw[e];
+        z[j][e] = fmaf(p.y ? s[j][e] : 0.f, u[j][e], x[e]) * now.r2;
+        sw[j][e] = fmaf(tn[e], z[j][e], sw[j][e]);
+        const float tt = tn[e] * w[e], su = s[j][e] * u[j][e];
+        d[j][e] = fmaf(now.r2, tt, d[j][e]);
+        sum[0] = fmaf(tt, z[j][e], sum[0]);
+        A[j] = fmaf(su, d[j][e], A[j]);
+        B[j] = fmaf(su, z[j][e], B[j]);
+      }
+    }
+    if (p.pw && p.groups == 1) {
+#pragma unroll
+      for (int j = 0; j < NV; j++) sum[1] += A[j], sum[2] += B[j];
+      row_sums<BLOCK, 3>(sum, red, nw, turn);
+#pragma unroll
+      for (int j = 0; j < NV; j++) A[j] = sum[1], B[j] = sum[2];
+    } else {
       if (p.w) {
-        float tn[VEC], w[VEC];
-        if (p.x) ldv<VEC>((const TX*)p.x + r * p.xs + i * VEC, z[j]);
-        ldv<VEC>((const TY*)p.dn + r * p.C + i * VEC, tn);
-        ldw<VEC>(p.w, p.w_bf16, i * VEC, w);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          if (p.y) z[j][e] = fmaf(p.scale * f[e], a[e], z[j][e]);
-          z[j][e] *= r2;
-          sw[j][e] = fmaf(tn[e], z[j][e], sw[j][e]);
-          const float tt = tn[e] * w[e];
-          s = fmaf(tt, z[j][e], s);
-          d[j][e] = fmaf(r2, tt, d[j][e]);
-        }
+        float one[1] = {sum[0]};
+        row_sums<BLOCK, 1>(one, red, nw, turn);
+        sum[0] = one[0];
+      }
+      if (p.pw) {
+        group_sums<BLOCK, NV>(A, nvec, per, p.groups, vec, t, tpr);
+        group_sums<BLOCK, NV>(B, nvec, per, p.groups, vec, t, tpr);
       }
     }
-    if (p.w) {
-      s = row_sum<TPR>(s, red) / (float)p.C * r2;
-#pragma unroll
-      for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int e = 0; e < VEC; e++) d[j][e] = fmaf(-s, z[j][e], d[j][e]);
-    }
-    float gs[NV];
+    const float m = sum[0] * now.r2 * inv_c;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = j * TPR + t;
-      gs[j] = 0.f;
+      const int i = j * tpr + t;
       if (i >= nvec) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) d[j][e] = fmaf(-m, z[j][e], d[j][e]);
       if (p.dx) stv<VEC>((TX*)p.dx + r * p.C + i * VEC, d[j]);
       if (!p.y) continue;
-      float w[VEC];
+      float pw[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) w[e] = 1.f;
-      if (p.pw) ldw<VEC>(p.pw, p.w_bf16, i * VEC, w);
-      float f[VEC], g[VEC];
+      for (int e = 0; e < VEC; e++) pw[e] = 1.f;
+      if (p.pw) ldw<VEC>(p.pw, p.w_bf16, i * VEC, pw);
       if (p.gate_kind) {
-        ldv<VEC>((const TY*)p.gate + (p.gate_kind == GATE_FULL ? r * p.gs : 0) + i * VEC, g);
+        float g[VEC];
+        if (p.gate_kind == GATE_FULL) now.g[j].get(g);
+        else ldv<VEC>((const TY*)p.gate + i * VEC, g);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
-          float df;
-          act_both(p.act, g[e], f[e], df);
-          g[e] = p.scale * d[j][e] * u[j][e] * w[e] * df;
+          float f, df;
+          act_both(p.act, g[e], f, df);
+          const float du = p.scale * d[j][e] * u[j][e];
+          sp[j][e] = fmaf(f, du, sp[j][e]);
+          g[e] = du * pw[e] * df;
           sg[j][e] += g[e];
         }
         if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + r * p.C + i * VEC, g);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) f[e] = 1.f;
+        for (int e = 0; e < VEC; e++) sp[j][e] = fmaf(p.scale * d[j][e], u[j][e], sp[j][e]);
       }
+      const float mu = p.pw ? fmaf(-m, B[j], A[j]) * inv_g : 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const float da = p.scale * f[e] * d[j][e];
-        if (p.pw) sp[j][e] = fmaf(da, u[j][e], sp[j][e]);
-        d[j][e] = da * w[e];
-        gs[j] = fmaf(d[j][e], u[j][e], gs[j]);
-      }
-    }
-    if (!p.y) continue;
-    if (p.pw) group_sums<TPR, NV>(gs, nvec, per, p.groups, vec, grp, red, t);
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-      const int i = j * TPR + t;
-      if (i >= nvec) continue;
-      if (p.pw) {
-        const float r1 = p.r1[r * p.groups + i / per], m = gs[j] / (float)p.gc;
-#pragma unroll
-        for (int e = 0; e < VEC; e++) d[j][e] = r1 * fmaf(-m, u[j][e], d[j][e]);
-      }
+      for (int e = 0; e < VEC; e++) d[j][e] = now.r1[j] * fmaf(-mu, u[j][e], s[j][e] * d[j][e]);
       stv<VEC>((TY*)p.dy + r * p.C + i * VEC, d[j]);
     }
+    if (AHEAD) now = next;
+    else if (r + step < p.rows) now.load(p, r + step, t, tpr, nvec, grp);
   }
   // this block's sums over its rows, its warps' one after the other
   float* out = p.part + (long long)blockIdx.x * 3 * p.C;
-  for (int q = 0; q < RPB; q++) {
+  for (int q = 0; q < (BLOCK ? 1 : kRowsPerBlock); q++) {
     if (q == sub) {
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int i = j * TPR + t;
+        const int i = j * tpr + t;
         if (i >= nvec) continue;
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
@@ -757,30 +834,42 @@ __global__ void __launch_bounds__(256) norm_part_kernel(const __grid_constant__ 
 // Launches
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxShared = 227 * 1024;
-constexpr int kMaxChannels = 8192;   // what a block's registers hold in the backward pass
 
-template <class TX, class TY, int VEC, int TPR, int NV, int RPB>
-cudaError_t rows_t(const NormParams& p, bool bwd, cudaStream_t st) {
-  const int smem = 4 * RPB * rows_smem_floats(p.C / VEC, p.groups);
-  if (bwd) return launch(norm_rows_bwd_kernel<TX, TY, VEC, TPR, NV, RPB>, dim3((unsigned)p.blocks), TPR * RPB, smem, st, p);
-  return launch(norm_rows_kernel<TX, TY, VEC, TPR, NV, RPB>, dim3((unsigned)((p.rows + RPB - 1) / RPB)), TPR * RPB, smem, st, p);
+template <class TX, class TY, int VEC, int NV, bool BLOCK>
+cudaError_t rows_fwd(const NormParams& p, cudaStream_t st) {
+  const int nvec = p.C / VEC, tpr = BLOCK ? ((nvec + NV - 1) / NV + 31) / 32 * 32 : 32, rpb = BLOCK ? 1 : kRowsPerBlock;
+  return launch(norm_rows_kernel<TX, TY, VEC, NV, BLOCK>, dim3((unsigned)((p.rows + rpb - 1) / rpb)), tpr * rpb,
+                4 * rpb * rows_smem_floats(nvec, p.groups), st, p);
+}
+template <class TX, class TY, int VEC, int NV, bool BLOCK>
+cudaError_t rows_bwd(const NormParams& p, cudaStream_t st) {
+  const int nvec = p.C / VEC, tpr = BLOCK ? ((nvec + NV - 1) / NV + 31) / 32 * 32 : 32, rpb = BLOCK ? 1 : kRowsPerBlock;
+  return launch(norm_rows_bwd_kernel<TX, TY, VEC, NV, BLOCK>, dim3((unsigned)p.blocks), tpr * rpb,
+                4 * rpb * rows_smem_floats(nvec, p.groups), st, p);
 }
 
-// Threads for a row: a warp holds up to 4 vectors a thread; wider rows take a block, of which NV vectors a thread.
+// Vectors of a thread: one, as long as a block's threads do.
 template <class TX, class TY, int VEC>
 cudaError_t rows_v(const NormParams& p, bool bwd, cudaStream_t st) {
+  constexpr int kVecs = kMaxChannels / VEC;   // the most of a row
   const int nvec = p.C / VEC;
-  if (nvec <= 32) return rows_t<TX, TY, VEC, 32, 1, 4>(p, bwd, st);
-  if (nvec <= 64) return rows_t<TX, TY, VEC, 32, 2, 4>(p, bwd, st);
-  if (nvec <= 128) return rows_t<TX, TY, VEC, 128, 1, 1>(p, bwd, st);
-  if (nvec <= 256) return rows_t<TX, TY, VEC, 256, 1, 1>(p, bwd, st);
-  if (nvec <= 512) return rows_t<TX, TY, VEC, 512, 1, 1>(p, bwd, st);
-  if constexpr (VEC == 8) return rows_t<TX, TY, VEC, 512, 2, 1>(p, bwd, st);
-  else {
-    if (nvec <= 1024) return rows_t<TX, TY, VEC, 512, 2, 1>(p, bwd, st);
-    if constexpr (VEC > 1) return rows_t<TX, TY, VEC, 512, 4, 1>(p, bwd, st);
-    else return rows_t<TX, TY, 1, 1024, 8, 1>(p, bwd, st);
+  if (bwd) {
+    if (nvec <= 32) return rows_bwd<TX, TY, VEC, 1, false>(p, st);
+    if (nvec <= 512) return rows_bwd<TX, TY, VEC, 1, true>(p, st);
+    if (nvec <= 1024) return rows_bwd<TX, TY, VEC, 2, true>(p, st);
+    if constexpr (kVecs > 1024) {
+      if (nvec <= 2048) return rows_bwd<TX, TY, VEC, 4, true>(p, st);
+      if constexpr (kVecs > 2048) return rows_bwd<TX, TY, VEC, 16, true>(p, st);
+    }
+    return cudaErrorInvalidValue;
   }
+  if (nvec <= 32) return rows_fwd<TX, TY, VEC, 1, false>(p, st);
+  if (nvec <= 1024) return rows_fwd<TX, TY, VEC, 1, true>(p, st);
+  if constexpr (kVecs > 1024) {
+    if (nvec <= 2048) return rows_fwd<TX, TY, VEC, 2, true>(p, st);
+    if constexpr (kVecs > 2048) return rows_fwd<TX, TY, VEC, 8, true>(p, st);
+  }
+  return cudaErrorInvalidValue;
 }
 
 template <class TX, class TY, int VEC>
@@ -841,7 +930,10 @@ int check(const sffft_block_norm_t* d, const void* x, const void* y, const void*
 
 int backward_blocks(const sffft_block_norm_t* d, int sms) {
   const long long units = d->inner ? (d->rows / d->inner) * ((d->inner + kPos - 1) / kPos) : d->rows;
-  const long long most = d->inner ? sms : 4ll * sms;
+  // rows: as many blocks of a row's threads as an SM's registers hold at 128 each; channels first: one
+  const int threads = (d->channels / (d->io == SFFFT_IO_BF16 ? 8 : 4) + 31) / 32 * 32;
+  const int per_sm = d->inner || threads > 256 ? 1 : threads <= 32 ? 4 : 512 / threads;
+  const long long most = (long long)per_sm * sms;
   return (int)(units < most ? units : most);
 }
 
