@@ -25,10 +25,10 @@ class DeviceScope {
  public:
   explicit DeviceScope(int device) {
     err = cudaGetDevice(&prev_);
-    if (err == cudaSuccess && prev_ != device) {
-      err = cudaSetDevice(device);
-      back_ = err == cudaSuccess;
-    }
+    // Also where it is current already: on a thread of its own that is where the device's context is bound, and a driver
+    // call such as the encoding of a tensor map needs it.
+    if (err == cudaSuccess) err = cudaSetDevice(device);
+    back_ = err == cudaSuccess && prev_ != device;
   }
   ~DeviceScope() {
     if (back_) cudaSetDevice(prev_);

@@ -156,20 +156,20 @@ void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G
   *G = chunks ? (int)((chunks + per - 1) / per) : 1;
 }
 
-// Segments for the tensor-core kernel.  An SM holds two CTAs of head size 64, else one; a CTA's time is that of its
-// chunks one after the other, so cutting pays until the CTAs fill the SMs, and costs a second reading of k and v
-// (half a chunk's work), a launch and the sum of earlier states (together about kCutCost chunks).
-constexpr double kCutCost = 4.0;
+// Segments for the tensor-core kernel, one CTA on an SM.  A CTA's time is that of its chunks one after the other, so cutting
+// pays until the CTAs fill the SMs; it costs a reading of k and v (about kLocalCost of a chunk's time each) and a launch with
+// the sums of earlier states (about kCutCost chunks).
+constexpr double kCutCost = 3.0, kLocalCost = 0.5;
 
 void plan_tc(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
-  const long long slots = (long long)sms * (D <= 64 && Dv <= 64 ? 2 : 1), units = (long long)B * H * ntask;
+  const long long units = (long long)B * H * ntask * la_tc_slices(D, Dv);
   const int chunks = (L + kLaTcChunk - 1) / kLaTcChunk;
   double best = 0;
   *G = 1;
   for (int g = 1; g <= kMaxSegments && g <= chunks; g++) {
-    const long long waves = (units * g + slots - 1) / slots;
+    const long long waves = (units * g + sms - 1) / sms;
     const int per = (chunks + g - 1) / g;
-    const double cost = (double)waves * per * (g > 1 ? 1.5 : 1.0) + (g > 1 ? kCutCost : 0.0);
+    const double cost = (double)waves * per * (g > 1 ? 1.0 + kLocalCost : 1.0) + (g > 1 ? kCutCost : 0.0);
     if (g == 1 || cost < best) best = cost, *G = g;
   }
   const int per = chunks ? (chunks + *G - 1) / *G : 1;

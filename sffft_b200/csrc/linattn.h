@@ -25,7 +25,7 @@ struct LaTask {
   long long s1s[4];
   float s1_mul;
   int s1_decay;                           // the end state takes one more factor lambda (where there is a token)
-  float* loc;                             // G > 1: state that each segment alone leaves, [B*H][G][D][Dv]
+  float* loc;                             // G > 1: state that each segment alone leaves, [B*H][G][D Dv] in a kernel's own order
   int D, Dv;
   int rev;                                // tokens are taken from the last one to the first
   int off;                                // the first token takes the start state as it is, without a factor lambda
@@ -72,10 +72,11 @@ cudaError_t launch_la_general(const LaParams& prm, bool bf16, cudaStream_t st);
 // positions in a chunk of the general kernel for head sizes up to dmax
 inline int la_general_chunk(int dmax) { return dmax > 128 ? 32 : 64; }
 
-// bf16 on the tensor cores: head sizes up to 128 in multiples of 8, 16-byte aligned rows (la_tc_takes), any length.
+// bf16 on the tensor cores: D up to 128, D and Dv multiples of 8, 16-byte aligned rows (la_tc_takes), any length.
 bool la_tc_takes(const LaParams& prm);
 cudaError_t launch_la_tc(const LaParams& prm, cudaStream_t st);
 cudaError_t la_tc_status(int* status);   // waits for the current device; reads and clears its status word
 constexpr int kLaTcChunk = 128;
+int la_tc_slices(int D, int Dv);   // CTAs over the columns of v
 
 }  // namespace sffft

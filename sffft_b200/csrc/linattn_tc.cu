@@ -1,23 +1,29 @@
 // Linear attention with a decay for each head on the tensor cores (bf16 operands, fp32 accumulators in TMEM).
 //
-// A CTA takes one head of one row and a segment of its positions, 128 at a time (the MMA's M).  With S the state before the
-// chunk, P = (Q K^T) * lambda^(i-j) for j <= i, m tokens in the chunk:
+// A CTA takes one head of one row, up to 64 or 128 columns of v and a segment of the positions, 128 at a time (the MMA's M).
+// With S the state before the chunk, P = (Q K^T) * lambda^(i-j) for j <= i, m tokens in the chunk:
 //   O = lambda^(i+1) (Q S) + P V              S <- lambda^m S + X^T V,    X_j = lambda^(m-1-j) k_j
-// Four products a chunk; each of 128 x 128 x 128 takes 512 cycles of an SM, while the chunk's 128 KB of q, k, v and y
-// (head size 128) take about 5700 cycles of its share of the memory's bandwidth: the kernel is bound by memory as long as
-// what lies between the products is overlapped with the loads.  So the work is split over warps:
-//   4 warps     P: TMEM -> scale, mask, round -> TMEM;  O: lambda^(i+1) scale between the two products;  output
-//   4 per 64 columns of v   X: shared memory -> TMEM, transposed;  S in fp32 registers -> bf16 in shared memory
-//   1 thread    TMA loads, two stages of (Q, K, V), and the store of O, which is staged where V was
-//   1 thread    tcgen05.mma
+// Four products a chunk.  A chunk's q, k, v and y take about 5700 cycles of an SM's share of the memory's bandwidth at head
+// size 128 (128 KB) and 2850 at 64; the products take 2050 to 2560 and 1020 to 1280.  So the kernel is bound by memory as
+// far as what lies between the products keeps up, and that is spread over warps:
+//   A warpgroups     P: TMEM -> scale, mask, round -> TMEM;  O: lambda^(i+1) between the two products;  output.  One, or
+//                    two that take turns at head size 64, where a chunk has half the time
+//   state warpgroups, one for each 32 columns of v    X: shared memory -> TMEM, transposed;  S: fp32 registers, and in bf16
+//                    in shared memory for the next chunk's product
+//   1 thread         TMA loads, 2 to 6 stages, and the store of O, which is staged where Q was
+//   1 thread         tcgen05.mma, each product as soon as its operands are there
 //
 // Rounding.  y takes P and S rounded to bf16, one rounding beside its own, as any tensor-core product must.  The state is an
-// fp32 result that lives for the whole row, so X is held as a sum of bf16 values: two (2^-17) where only y uses the state,
-// three (2^-25) where it is an output; and S is added up in registers, not in the accumulator, whose additions truncate.
-// With a head size of 64 the first two parts fill the 128 lanes together (lanes 0-63 and 64-127), and so does S, whose two
-// halves the product with Q adds up.
+// fp32 result that lives for the whole row, so X is held as a sum of bf16 values: two (2^-16) where only y uses the state,
+// three (2^-24) where it is an output; and S is added up in registers, not in the accumulator, whose additions truncate.
+//
+// Head size 64 would leave half of the 128 lanes of X^T V idle.  So lanes 0-63 take the chunk's first 64 positions and lanes
+// 64-127 the others, against both halves of V side by side (N = 128): of the four 64 x 64 results the two mixed ones are
+// not looked at, and S is the sum of two halves that Q S adds up, each with its own copy of Q.
 //
 // Time reversal (gradients of k and v): chunks from the last to the first, P and X mirrored.
+//
+// A segment's own contribution to the state (LOCAL) needs X^T V alone.
 //
 // Every wait is bounded: after kWaitLimit ns the waiting role raises the CTA's flag, all roles leave, and the device's
 // status word says so.
@@ -44,35 +50,51 @@ struct __align__(64) LaTcParams {
   CUtensorMap map[kLaMaxTasks][4];   // q, k, v, y
   LaParams p;
   int blocks;   // chunks in a segment
+  int slices;   // CTAs over the columns of v
 };
 
-template <int DQ, int DV>
+template <int DQ, int DV, bool LOCAL>
 struct Shape {
+  static constexpr bool split = DQ == 64;               // positions over the halves of the lanes
+  static_assert(!split || DV == 64, "head size 64 takes 64 columns of v");
   static constexpr int NB = DV / 64, NW = DV / 32;      // 64-column tiles of v; state warpgroups, 32 columns each
-  static constexpr int threads = 128 + 128 * NW + 64;
-  static constexpr bool alias = DQ == 64 && DV == 64;   // two CTAs on an SM: 256 columns each, O lies in S's upper half
-  static constexpr bool out_q = DQ >= DV;               // O is staged where Q was, else where V was
-  static constexpr uint32_t q_bytes = DQ / 64 * kBlk, v_bytes = NB * kBlk, stage = 2 * q_bytes + v_bytes;
-  static constexpr uint32_t off_s = 2 * stage, off_tab = off_s + NB * kBlk, off_bar = off_tab + 4 * 160;
-  static constexpr uint32_t smem = off_bar + 17 * 8 + 8;
-  static constexpr uint32_t cols = alias ? 256 : 512;
-  // TMEM columns: products Q K^T (P over their first half), O, increment of S, X
-  static constexpr uint32_t c_p = 0, c_o = alias ? 64 : 128, c_kv = alias ? 128 : 128 + DV, c_x = c_kv + DV;
-  static constexpr uint32_t x_cols = DQ == 64 ? 64 : 128;
-  static_assert(c_x + x_cols <= cols, "TMEM");
+  static constexpr int NA = LOCAL ? 0 : split ? 2 : 1;
+  static constexpr int NS = LOCAL ? (split ? 6 : 3) : split ? 4 : 2;   // stages: what shared memory holds
+  static constexpr int threads = 128 * NA + 128 * NW + 64;
+  static constexpr uint32_t q_bytes = DQ / 64 * kBlk, v_bytes = NB * kBlk;
+  static constexpr uint32_t off_k = LOCAL ? 0 : q_bytes, off_v = off_k + q_bytes, stage = off_v + v_bytes;
+  static constexpr uint32_t off_s = NS * stage, off_tab = off_s + NB * kBlk, off_bar = off_tab + 4 * 160;
+  static constexpr uint32_t smem = off_bar + 42 * 8 + 8;
+  static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one CTA on an SM: each takes all of TMEM");
+  // TMEM columns.  Products Q K^T (P over their first half) and O of A warpgroup a; the increment of S; X.
+  __host__ __device__ static constexpr uint32_t c_p(int a) { return (uint32_t)a * 128; }
+  __host__ __device__ static constexpr uint32_t c_o(int a) { return split ? (uint32_t)a * 128 + 64 : 128; }
+  static constexpr uint32_t inc_cols = split ? 128 : DV;
+  __host__ __device__ static constexpr uint32_t c_inc(int c) { return LOCAL ? (uint32_t)(c & 1) * 128 : 256; }   // LOCAL: two, in turn
+  static constexpr uint32_t c_x = LOCAL ? 256 : 256 + inc_cols;
+  static constexpr bool whole_x = split || LOCAL;       // all parts of X at once; else the third after the others
+  static constexpr uint32_t part_cols = split ? 32 : 64;
+  static_assert(c_x + part_cols * (whole_x ? 3 : 2) <= 512, "TMEM");
 };
 
-// Barriers; each completes once a chunk (the first two pairs once for every other chunk).
+// Barriers.  A wait names a phase by its parity alone, so whoever waits must not fall two phases behind: that holds where the
+// next phase needs something that the waiting role does after it has seen this one.  The thread that loads is ahead of
+// nothing, so what it waits for has a barrier for each stage, whose next phase needs that thread's own next load.
+// Those of the stages complete once for each NS chunks, those of an A warpgroup once for each NA, the others once a chunk.
 enum {
-  B_KV0, B_KV1, B_Q0, B_Q1,   // K and V, Q loaded
-  B_S, B_P,                   // products ready; P ready
-  B_O1, B_OS, B_O,            // Q S taken; scaled; O complete
-  B_OOUT, B_OFREE,            // O staged; O's TMEM read
-  B_X, B_INC, B_X2, B_INC2,   // X ready, its product taken; third part ready, its product taken
-  B_ST,                       // S published (once more before the first chunk)
+  B_KV = 0, B_Q = 6,          // K and V, Q loaded [stage]
+  B_REL = 10,                 // K and V read by the state warpgroups and X^T V [stage]
+  B_PV = 14,                  // V read by P V; LOCAL: by X^T V [stage]
+  B_OOUT = 20,                // O staged [stage]
+  B_S = 24, B_P = 26,         // products ready; P ready [A]
+  B_O1 = 28, B_OS = 30,       // Q S taken; scaled [A]
+  B_O = 32, B_OFREE = 34,     // O complete; its TMEM read [A]
+  B_X = 36, B_INC,            // X ready, its product taken
+  B_X2, B_INC2,               // third part ready, its product taken
+  B_ST,                       // S taken over and published; once more before the first chunk (not LOCAL)
   B_FIN, B_COUNT
 };
-static_assert(B_COUNT <= 17, "barriers");
+static_assert(B_COUNT <= 42, "barriers");
 
 __host__ __device__ constexpr uint32_t idesc_bf16(int N, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -251,10 +273,9 @@ __device__ __forceinline__ int tokens_before(int c, int n, int nblk, bool rev) {
 }
 
 template <int DQ, int DV, bool LOCAL>
-__global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ? 2 : 1)
-    la_tc_kernel(const __grid_constant__ LaTcParams prm) {
-  using SH = Shape<DQ, DV>;
-  constexpr int NB = SH::NB, NW = SH::NW;
+__global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel(const __grid_constant__ LaTcParams prm) {
+  using SH = Shape<DQ, DV, LOCAL>;
+  constexpr int NB = SH::NB, NW = SH::NW, NA = SH::NA, NS = SH::NS;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t sm = smem_u32(smem);
   // Powers of lambda in the order in which they are wanted, so that a loop over positions has fixed offsets.  Forward:
@@ -262,14 +283,19 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   // diagonal block.
   float* tab = (float*)(smem + SH::off_tab);
   uint64_t* bars = (uint64_t*)(smem + SH::off_bar);
-  volatile int* stop = (volatile int*)(smem + SH::off_bar + 17 * 8);
-  uint32_t* slot = (uint32_t*)(smem + SH::off_bar + 17 * 8 + 4);
+  volatile int* stop = (volatile int*)(smem + SH::off_bar + 42 * 8);
+  uint32_t* slot = (uint32_t*)(smem + SH::off_bar + 42 * 8 + 4);
 
   const LaParams& lp = prm.p;
-  const int ti = blockIdx.x % lp.ntask, u = blockIdx.x / lp.ntask;
+  uint32_t u = blockIdx.x;
+  const int vi = u % prm.slices;   // the CTA's columns of v
+  u /= prm.slices;
+  const int ti = u % lp.ntask;
+  u /= lp.ntask;
   const LaTask& tk = lp.task[ti];
+  const int cb = vi * DV;
   const int g = u % lp.G, bh = u / lp.G, b = bh / lp.H, h = bh % lp.H;
-  if (LOCAL && g == lp.G - 1) return;
+  if (cb >= tk.Dv || (LOCAL && g == lp.G - 1)) return;   // nothing follows the last segment
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n = lp.L;
   if (lp.len) n = min(max(lp.len[b], 0), lp.L);
@@ -278,13 +304,13 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   const int c0 = min(g * prm.blocks, nblk), c1 = min(c0 + prm.blocks, nblk), nc = c1 - c0;
   const int before = tokens_before(c0, n, nblk, rev);
   const LaDecay dec(lp.ld[h]);
-  const bool three = tk.s1 != nullptr;   // the state is an output: three parts of X
-  // the first chunk meets no state
-  const bool fresh = !LOCAL && before == 0 && !tk.s0;
+  const bool three = tk.s1 != nullptr && (LOCAL || g == lp.G - 1);   // the state, or what it is made of, is an output
+  const bool fresh = !LOCAL && before == 0 && !tk.s0;                // the first chunk meets no state
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < B_COUNT; i++) {
-      const bool a = i == B_P || i == B_OS || i == B_OOUT || i == B_OFREE, x = i == B_X || i == B_X2 || i == B_ST;
+      const bool a = (i >= B_OOUT && i < B_S) || (i >= B_P && i < B_O1) || (i >= B_OS && i < B_O) || (i >= B_OFREE && i < B_X);
+      const bool x = (i >= B_REL && i < B_PV) || i == B_X || i == B_X2 || i == B_ST;
       mbar_init(bars + i, a ? 128u : x ? 128u * NW : 1u);
     }
     *stop = (sm & 1023u) != 0;   // swizzled tiles need the alignment that the launch gives
@@ -296,7 +322,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     tab[i] = e >= 0 ? dec.pow(e) : 0.f;
   }
   if (warp == SH::threads / 32 - 1) {
-    tmem_alloc(slot, SH::cols);
+    tmem_alloc(slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -307,157 +333,180 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   const WarpWaiter wwait{wait};
   auto power = [&](int e) { return tab[rev ? 32 + e : 127 - e]; };   // 0 <= e < 128
 
-  auto tokens = [&](int c) {   // of chunk c0 + c
-    const int blk = rev ? nblk - 1 - (c0 + c) : c0 + c;
-    return min(kTok, n - blk * kTok);
-  };
+  auto block = [&](int c) { return rev ? nblk - 1 - (c0 + c) : c0 + c; };
+  auto tokens = [&](int c) { return min(kTok, n - block(c) * kTok); };
+  auto stage_at = [&](int c) { return sm + (uint32_t)(c % NS) * SH::stage; };
+  auto sph = [](int c) { return (uint32_t)(c / NS) & 1; };         // phase of a stage's barrier
+  auto aph = [](int c) { return (uint32_t)(c / (NA ? NA : 1)) & 1; };   // of an A warpgroup's
+  auto grp = [](int c) { return NA ? c % NA : 0; };
 
   if (*stop) {
     // nothing has been started
   } else if (warp == SH::threads / 32 - 2) {
     // ---- loads, stores ----
     if (lane == 0) {
-      const CUtensorMap* m = prm.map[ti];
+      const CUtensorMap* mp = prm.map[ti];
       const int hq = h / tk.qdiv, hk = h / tk.kdiv, hv = h / tk.vdiv;
-      auto load_kv = [&](int c) {
-        const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage;
-        uint64_t* bar = bars + B_KV0 + (c & 1);
-        const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
-        mbar_expect(bar, SH::q_bytes + SH::v_bytes);
-        for (int i = 0; i < DQ / 64; i++) tma_load(st + SH::q_bytes + i * kBlk, m + 1, i * 64, t, hk, b, bar);
-        for (int i = 0; i < NB; i++) tma_load(st + 2 * SH::q_bytes + i * kBlk, m + 2, i * 64, t, hv, b, bar);
-      };
-      auto load_q = [&](int c) {
-        const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage;
-        uint64_t* bar = bars + B_Q0 + (c & 1);
-        const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
-        mbar_expect(bar, SH::q_bytes);
-        for (int i = 0; i < DQ / 64; i++) tma_load(st + i * kBlk, m + 0, i * 64, t, hq, b, bar);
-      };
       int kv = 0, qs = 0;   // loads issued
-      for (; kv < min(nc, 2); kv++) load_kv(kv);
-      if (!LOCAL)
-        for (; qs < min(nc, 2); qs++) load_q(qs);
-      // a parity names the phase that follows a completed one: the first publication goes by before the loop
-      const bool go = LOCAL || nc == 0 || wait(B_ST, 0);
-      for (int c = 0; go && c < nc; c++) {
-        // K and V have been read: by X and its products, and by P V
-        if (!wait(B_ST, (LOCAL ? c : c + 1) & 1) || (!LOCAL && !wait(B_O, c & 1))) break;
-        if ((LOCAL || SH::out_q) && c + 2 < nc) load_kv(kv++);
-        if (LOCAL) continue;
-        if (!wait(B_OOUT, c & 1)) break;
-        if (!tk.y_f32) {
-          const uint32_t st = sm + (uint32_t)(c & 1) * SH::stage + (SH::out_q ? 0 : 2 * SH::q_bytes);
-          const int t = (rev ? nblk - 1 - (c0 + c) : c0 + c) * kTok;
-          for (int i = 0; i < NB; i++) tma_store(m + 3, st + i * kBlk, i * 64, t, h, b);
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          if (c + 2 < nc) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      auto load_kv = [&]() {
+        const int c = kv++;
+        uint64_t* bar = bars + B_KV + c % NS;
+        mbar_expect(bar, SH::q_bytes + SH::v_bytes);
+        for (int i = 0; i < DQ / 64; i++) tma_load(stage_at(c) + SH::off_k + i * kBlk, mp + 1, i * 64, block(c) * kTok, hk, b, bar);
+        for (int i = 0; i < NB; i++) tma_load(stage_at(c) + SH::off_v + i * kBlk, mp + 2, cb + i * 64, block(c) * kTok, hv, b, bar);
+      };
+      auto load_q = [&]() {
+        const int c = qs++;
+        uint64_t* bar = bars + B_Q + c % NS;
+        mbar_expect(bar, SH::q_bytes);
+        for (int i = 0; i < DQ / 64; i++) tma_load(stage_at(c) + i * kBlk, mp + 0, i * 64, block(c) * kTok, hq, b, bar);
+      };
+      while (kv < min(nc, NS)) {
+        load_kv();
+        if (!LOCAL) load_q();
+      }
+      for (int c = 0; c < nc; c++) {
+        const int r = c % NS;
+        if (LOCAL) {
+          if (!wait(B_PV + r, sph(c))) break;
+          if (kv < nc) load_kv();
+          continue;
         }
-        if (c + 2 < nc) {
-          if (!SH::out_q) load_kv(kv++);
-          load_q(qs++);
+        if (!SH::split) {   // with two stages K and V are wanted back before O is staged
+          if (!wait(B_REL + r, sph(c)) || !wait(B_PV + r, sph(c))) break;
+          if (kv < nc) load_kv();
+        }
+        if (!wait(B_OOUT + r, sph(c))) break;
+        if (!tk.y_f32) {
+          for (int i = 0; i < NB; i++) tma_store(mp + 3, stage_at(c) + i * kBlk, cb + i * 64, block(c) * kTok, h, b);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if (qs < nc) {
+          if (SH::split && !wait(B_REL + r, sph(c))) break;   // and P V: O is out
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          if (SH::split) load_kv();
+          load_q();
         }
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (*stop) {   // copies in flight end before the block does
-        for (int c = max(0, kv - 2); c < kv; c++) mbar_wait_bounded(bars + B_KV0 + (c & 1), (c >> 1) & 1, kWaitLimit);
-        for (int c = max(0, qs - 2); c < qs; c++) mbar_wait_bounded(bars + B_Q0 + (c & 1), (c >> 1) & 1, kWaitLimit);
+        for (int c = max(0, kv - NS); c < kv; c++) mbar_wait_bounded(bars + B_KV + c % NS, sph(c), kWaitLimit);
+        for (int c = max(0, qs - NS); c < qs; c++) mbar_wait_bounded(bars + B_Q + c % NS, sph(c), kWaitLimit);
       }
     }
   } else if (warp == SH::threads / 32 - 1) {
     // ---- products ----
     if (lane == 0) {
-      constexpr uint32_t id_s = idesc_bf16(128, false), id_v = idesc_bf16(DV, true);
+      constexpr uint32_t id_s = idesc_bf16(128, false), id_v = idesc_bf16(DV, true), id_inc = idesc_bf16(SH::inc_cols, true);
       auto at = [](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
       auto kstep = [](int k) { return (uint32_t)(k >> 2) * kBlk + (uint32_t)(k & 3) * 32; };   // K-major: 16 values on
+      auto ready = [&](int bar, uint32_t parity) { return mbar_test_wait(bars + bar, parity); };
       const uint64_t sd = make_sdesc(sm + SH::off_s, kBlk, 1024, LT_SW128);
-      bool ok = true;
-      for (int c = 0; ok && c < nc; c++) {
-        const uint32_t ph = c & 1, st = sm + (uint32_t)(c & 1) * SH::stage;
-        if (!wait(B_KV0 + (c & 1), (c >> 1) & 1)) break;
-        const uint64_t qd = make_sdesc(st, 16, 1024, LT_SW128), kd = make_sdesc(st + SH::q_bytes, 16, 1024, LT_SW128);
-        const uint64_t vd = make_sdesc(st + 2 * SH::q_bytes, kBlk, 1024, LT_SW128);
-        if (!LOCAL) {
-          if (!wait(B_Q0 + (c & 1), (c >> 1) & 1)) break;
-          if (SH::alias && c > 0 && !wait(B_OFREE, ph ^ 1)) break;
-          tc_fence_after();
-          for (int k = 0; k < DQ / 16; k++) mma_f16_ss(tm + SH::c_p, at(qd, kstep(k)), at(kd, kstep(k)), id_s, k > 0);
-          mma_commit(bars + B_S);
-        }
-        // the chunk's other products in the order in which their operands become ready
-        bool inc = false, inc2 = !three, qs = LOCAL, pv = LOCAL;
-        const bool dirty = tokens(c) < kTok && n < lp.L;   // v is cleaned before X arrives
-        uint64_t t0 = 0;
-        uint32_t idle = 0;
-        while (!(inc && inc2 && qs && pv)) {
-          if (!qs && mbar_test_wait(bars + B_ST, ph) &&
-              (SH::alias ? mbar_test_wait(bars + B_P, ph) : c == 0 || mbar_test_wait(bars + B_OFREE, ph ^ 1))) {
+      // X^T V: parts first .. last - 1 of X.  Split: 64 positions against both halves of V, 64 rows of 128 bytes apart.
+      auto increment = [&](int c, int first, int last, bool keep) {
+        const uint64_t vd = make_sdesc(stage_at(c) + SH::off_v, SH::split ? kBlk / 2 : kBlk, 1024, LT_SW128);
+        for (int part = first; part < last; part++)
+          for (int k = 0; k < (SH::split ? 4 : 8); k++)
+            mma_ts(tm + SH::c_inc(c), tm + SH::c_x + part * SH::part_cols + k * 8, at(vd, k * 2048), id_inc, keep || part > first || k > 0);
+      };
+      int i_s = 0, i_q = 0, i_v = 0, i_k = 0, i_k2 = 0;   // chunks whose products Q K^T, Q S, P V, X^T V (third part) are issued
+      const bool later = three && !SH::whole_x;
+      uint64_t t0 = 0;
+      uint32_t idle = 0;
+      while (LOCAL ? i_k < nc : i_v < nc || i_k < nc || (later && i_k2 < nc)) {
+        bool some = false;
+        if constexpr (!LOCAL) {
+          if (i_q < i_s && ready(B_ST, i_q & 1) &&
+              (SH::split ? ready(B_P + grp(i_q), aph(i_q)) : i_q == 0 || ready(B_OFREE, (i_q - 1) & 1))) {
+            const int c = i_q++;
+            const uint64_t qd = make_sdesc(stage_at(c), 16, 1024, LT_SW128);
             tc_fence_after();
             if (!(fresh && c == 0))
               for (int k = 0; k < 8; k++)
-                mma_f16_ss(tm + SH::c_o, at(qd, kstep(DQ == 64 ? k & 3 : k)), at(sd, k * 2048), id_v, k > 0);
-            mma_commit(bars + B_O1);
-            qs = true;
-          } else if (qs && !pv && (inc || !dirty) && mbar_test_wait(bars + B_OS, ph) && mbar_test_wait(bars + B_P, ph)) {
+                mma_f16_ss(tm + SH::c_o(grp(c)), at(qd, kstep(SH::split ? k & 3 : k)), at(sd, k * 2048), id_v, k > 0);
+            mma_commit(bars + B_O1 + grp(c));
+            some = true;
+          }
+          if (i_v < i_q && ready(B_OS + grp(i_v), aph(i_v)) && ready(B_P + grp(i_v), aph(i_v)) &&
+              (i_k > i_v || tokens(i_v) == kTok || n == lp.L)) {   // v is cleaned before X arrives
+            const int c = i_v++;
+            const uint64_t vd = make_sdesc(stage_at(c) + SH::off_v, kBlk, 1024, LT_SW128);
             tc_fence_after();
             for (int k = 0; k < 8; k++)
-              mma_ts(tm + SH::c_o, tm + SH::c_p + k * 8, at(vd, k * 2048), id_v, k > 0 || !(fresh && c == 0));
-            mma_commit(bars + B_O);
-            pv = true;
-          } else if (!inc && mbar_test_wait(bars + B_X, ph)) {
-            tc_fence_after();
-            for (int part = 0; part < DQ / 64; part++)
-              for (int k = 0; k < 8; k++)
-                mma_ts(tm + SH::c_kv, tm + SH::c_x + part * 64 + k * 8, at(vd, k * 2048), id_v, (part | k) > 0);
-            mma_commit(bars + B_INC);
-            inc = true;
-          } else if (inc && !inc2 && mbar_test_wait(bars + B_X2, ph)) {
-            tc_fence_after();
-            for (int k = 0; k < 8; k++) mma_ts(tm + SH::c_kv, tm + SH::c_x + k * 8, at(vd, k * 2048), id_v, 1);
-            mma_commit(bars + B_INC2);
-            inc2 = true;
-          } else {
-            if ((++idle & 63) == 0) {
-              const uint64_t now = global_ns();
-              if (!t0) t0 = now;
-              if (now - t0 > kWaitLimit) {
-                *stop = 1;
-                atomicExch(&g_la_status, SFFFT_ERR_TIMEOUT);
-              }
-              if (*stop) {
-                ok = false;
-                break;
-              }
-            }
-            __nanosleep(20);
+              mma_ts(tm + SH::c_o(grp(c)), tm + SH::c_p(grp(c)) + k * 8, at(vd, k * 2048), id_v, k > 0 || !(fresh && c == 0));
+            mma_commit(bars + B_O + grp(c));
+            if (!SH::split) mma_commit(bars + B_PV + c % NS);
+            some = true;
           }
         }
+        if (i_k < nc && ready(B_KV + i_k % NS, sph(i_k)) && ready(B_X, i_k & 1)) {   // LOCAL: X of a chunk
+          // comes after the state of the last but one has been taken over from these columns
+          const int c = i_k++;
+          tc_fence_after();
+          increment(c, 0, SH::whole_x && three ? 3 : 2, false);
+          mma_commit(bars + B_INC);
+          if (LOCAL) mma_commit(bars + B_PV + c % NS);
+          some = true;
+        }
+        if (later && i_k2 < i_k && ready(B_X2, i_k2 & 1)) {
+          const int c = i_k2++;
+          tc_fence_after();
+          increment(c, 0, 1, true);
+          mma_commit(bars + B_INC2);
+          some = true;
+        }
+        if constexpr (!LOCAL) {
+          if (i_s < nc && ready(B_KV + i_s % NS, sph(i_s)) && ready(B_Q + i_s % NS, sph(i_s)) &&
+              (SH::split ? i_s < NA || ready(B_OFREE + grp(i_s), aph(i_s - NA)) : i_v == i_s)) {   // P has been read
+            const int c = i_s++;
+            const uint64_t qd = make_sdesc(stage_at(c), 16, 1024, LT_SW128);
+            const uint64_t kd = make_sdesc(stage_at(c) + SH::off_k, 16, 1024, LT_SW128);
+            tc_fence_after();
+            for (int k = 0; k < DQ / 16; k++) mma_f16_ss(tm + SH::c_p(grp(c)), at(qd, kstep(k)), at(kd, kstep(k)), id_s, k > 0);
+            mma_commit(bars + B_S + grp(c));
+            some = true;
+          }
+        }
+        if (some) {
+          t0 = 0;
+          continue;
+        }
+        if ((++idle & 63) == 0) {
+          const uint64_t now = global_ns();
+          if (!t0) t0 = now;
+          if (now - t0 > kWaitLimit) {
+            *stop = 1;
+            atomicExch(&g_la_status, SFFFT_ERR_TIMEOUT);
+          }
+          if (*stop) break;
+        }
+        __nanosleep(20);
       }
       if (*stop) {   // products in flight end before TMEM is given back
         mma_commit(bars + B_FIN);
         mbar_wait_bounded(bars + B_FIN, 0, kWaitLimit);
       }
     }
-  } else if (warp < 4) {
+  } else if (warp < 4 * NA) {
     // ---- P and O ----
-    if (!LOCAL) {
-      const int i = threadIdx.x;   // position in the chunk
-      const uint32_t tl = tm + ((uint32_t)(warp * 32) << 16);
+    if constexpr (!LOCAL) {
+      const int i = threadIdx.x & 127, a = warp >> 2, quad = warp & 3;   // position in the chunk
+      const uint32_t tl = tm + ((uint32_t)(quad * 32) << 16), tp = tl + SH::c_p(a), to = tl + SH::c_o(a);
       const float whole = dec.pow(kTok);
-      for (int c = 0; c < nc; c++) {
-        const uint32_t ph = c & 1;
-        const int m = tokens(c), blk = rev ? nblk - 1 - (c0 + c) : c0 + c;
+      for (int c = a; c < nc; c += NA) {
+        const uint32_t ph = aph(c);
+        const int m = tokens(c), blk = block(c);
         const int off = tk.off && before == 0 && c == 0;
-        if (!wwait(B_S, ph)) break;
+        if (!wwait(B_S + a, ph)) break;
         tc_fence_after();
 #pragma unroll 1
         for (int jb = 0; jb < 4; jb++) {
           uint32_t r[32], o[16];
-          if (rev ? jb < warp : jb > warp) {   // a block on the masked side of the diagonal
+          if (rev ? jb < quad : jb > quad) {   // a block on the masked side of the diagonal
 #pragma unroll
             for (int e = 0; e < 16; e++) o[e] = 0;
           } else {
-            tmem_ld32(tl + SH::c_p + jb * 32, r);
+            tmem_ld32(tp + jb * 32, r);
             const float* w = tab + (rev ? 32 + jb * 32 - i : 127 - i + jb * 32);
             tmem_wait_ld();
             if (m < kTok) {   // products with what k holds behind the last token may not be finite
@@ -469,13 +518,13 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
             for (int e = 0; e < 16; e++)
               o[e] = pack_bf16(__uint_as_float(r[2 * e]) * w[2 * e], __uint_as_float(r[2 * e + 1]) * w[2 * e + 1]);
           }
-          tmem_st16(tl + SH::c_p + jb * 16, o);
+          tmem_st16(tp + jb * 16, o);
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bars + B_P);
+        mbar_arrive(bars + B_P + a);
         // lambda^(i+1) Q S, in reverse lambda^(m-i)
-        if (!wwait(B_O1, ph)) break;
+        if (!wwait(B_O1 + a, ph)) break;
         tc_fence_after();
         if (!(fresh && c == 0)) {
           const int e = (rev ? m - i : i + 1) - off;
@@ -483,27 +532,26 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
 #pragma unroll 1
           for (int q = 0; q < DV / 32; q++) {
             uint32_t r[32];
-            tmem_ld32(tl + SH::c_o + q * 32, r);
+            tmem_ld32(to + q * 32, r);
             tmem_wait_ld();
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
               const F2 z = mul2({__uint_as_float(r[x]), __uint_as_float(r[x + 1])}, {w, w});
               r[x] = __float_as_uint(z.a), r[x + 1] = __float_as_uint(z.b);
             }
-            tmem_st32(tl + SH::c_o + q * 32, r);
+            tmem_st32(to + q * 32, r);
           }
           tmem_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(bars + B_OS);
-        if (!wwait(B_O, ph)) break;
+        mbar_arrive(bars + B_OS + a);
+        if (!wwait(B_O + a, ph)) break;
         tc_fence_after();
-        if (!SH::out_q && !wwait(three ? B_INC2 : B_INC, ph)) break;   // V's last reader
-        const uint32_t out = sm + (uint32_t)(c & 1) * SH::stage + (SH::out_q ? 0 : 2 * SH::q_bytes) + (uint32_t)i * 128;
+        const uint32_t out = stage_at(c) + (uint32_t)i * 128;   // Q has been read: its products are complete
 #pragma unroll 1
         for (int q = 0; q < DV / 32; q++) {
           uint32_t r[32];
-          tmem_ld32(tl + SH::c_o + q * 32, r);
+          tmem_ld32(to + q * 32, r);
           tmem_wait_ld();
           // rows behind the last token: whatever q holds has come through
           if (m < kTok && i >= m) {
@@ -523,24 +571,24 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
               sts128(out + (uint32_t)(q >> 1) * kBlk + ((chunk ^ (uint32_t)(i & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
           } else if (blk * kTok + i < lp.L) {
-            float* y = (float*)tk.y + b * tk.ys[0] + h * tk.ys[1] + (long long)(blk * kTok + i) * tk.ys[2] + q * 32;
+            float* y = (float*)tk.y + b * tk.ys[0] + h * tk.ys[1] + (long long)(blk * kTok + i) * tk.ys[2] + cb + q * 32;
 #pragma unroll
             for (int e = 0; e < 32; e += 4)   // Dv is a multiple of 8
-              if (q * 32 + e < tk.Dv)
+              if (cb + q * 32 + e < tk.Dv)
                 *(float4*)(y + e) = make_float4(tk.scale * __uint_as_float(r[e]), tk.scale * __uint_as_float(r[e + 1]),
                                                 tk.scale * __uint_as_float(r[e + 2]), tk.scale * __uint_as_float(r[e + 3]));
           }
         }
         fence_async_smem();
         tc_fence_before();
-        mbar_arrive(bars + B_OFREE);
-        mbar_arrive(bars + B_OOUT);
+        mbar_arrive(bars + B_OFREE + a);
+        mbar_arrive(bars + B_OOUT + c % NS);
       }
       // chunks of the segment behind the row's last token
       const int z0 = max(g * prm.blocks, nblk) * kTok, z1 = min((long long)(g + 1) * prm.blocks * kTok, (long long)lp.L);
-      const int pieces = tk.Dv / 8;
-      for (long long e = i; e < (long long)(z1 - z0) * pieces; e += 128) {
-        const long long at = b * tk.ys[0] + h * tk.ys[1] + (z0 + e / pieces) * tk.ys[2] + (e % pieces) * 8;
+      const int pieces = min(tk.Dv - cb, DV) / 8;
+      for (long long e = threadIdx.x; e < (long long)(z1 - z0) * pieces; e += 128 * NA) {
+        const long long at = b * tk.ys[0] + h * tk.ys[1] + (z0 + e / pieces) * tk.ys[2] + cb + (e % pieces) * 8;
         if (tk.y_f32) {
           *(float4*)((float*)tk.y + at) = make_float4(0.f, 0.f, 0.f, 0.f);
           *(float4*)((float*)tk.y + at + 4) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -551,16 +599,17 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
     }
   } else {
     // ---- X and S ----
-    const int wg = (warp - 4) >> 2, t = threadIdx.x & 127;
-    const uint32_t tl = tm + ((uint32_t)((warp & 3) * 32) << 16);
-    const int d = DQ == 64 ? t & 63 : t;        // the thread's row of the state
-    const bool main_part = DQ == 128 || t < 64; // lanes 64-127 hold the second part where the head size is 64
-    float s[32];                                // columns 32 wg ..
-    const int col = wg * 32;
+    const int wg = (warp >> 2) - NA, t = threadIdx.x & 127, quad = warp & 3;
+    const uint32_t tl = tm + ((uint32_t)(quad * 32) << 16);
+    const int d = SH::split ? t & 63 : t;         // the thread's row of the state
+    const bool main_part = !SH::split || t < 64;  // split: lanes 64-127 hold the second halves' sum
+    float s[32];                                  // columns 32 wg ..
+    const int col = cb + wg * 32;
 #pragma unroll
     for (int e = 0; e < 32; e++) s[e] = 0.f;
+    const long long mine = (long long)col * tk.D + d;   // of the segments' states, which are kept transposed: lanes are rows
     if (!LOCAL && main_part && d < tk.D) {
-      const float* loc = tk.loc + ((long long)bh * lp.G * tk.D + d) * tk.Dv + col;
+      const float* loc = tk.loc + (long long)bh * lp.G * tk.D * tk.Dv + mine;
       const long long step = (long long)tk.D * tk.Dv;
       for (int gg = 0; gg < g; gg++) {
         const int a = tokens_before(min(gg * prm.blocks, nblk), n, nblk, rev);
@@ -568,19 +617,25 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
         if (z == a) break;
         const float w = dec.pow(z - a);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4)   // Dv is a multiple of 8
-          if (col + e < tk.Dv) {
-            const float4 x = *(const float4*)(loc + gg * step + e);
-            s[e] = fmaf(w, s[e], x.x), s[e + 1] = fmaf(w, s[e + 1], x.y);
-            s[e + 2] = fmaf(w, s[e + 2], x.z), s[e + 3] = fmaf(w, s[e + 3], x.w);
-          }
+        for (int e = 0; e < 32; e++)
+          if (col + e < tk.Dv) s[e] = fmaf(w, s[e], loc[gg * step + (long long)e * tk.D]);
       }
       if (tk.s0) {
         const float w = dec.pow(before - (tk.off && before > 0));
         const float* s0 = tk.s0 + b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + (long long)col * tk.s0s[3];
+        if (tk.s0s[3] == 1 && ((uintptr_t)s0 & 15) == 0) {
 #pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (col + e < tk.Dv) s[e] = fmaf(w, s0[e * tk.s0s[3]] * tk.s0_mul, s[e]);
+          for (int e = 0; e < 32; e += 4)
+            if (col + e < tk.Dv) {
+              const float4 x = *(const float4*)(s0 + e);
+              s[e] = fmaf(w, x.x * tk.s0_mul, s[e]), s[e + 1] = fmaf(w, x.y * tk.s0_mul, s[e + 1]);
+              s[e + 2] = fmaf(w, x.z * tk.s0_mul, s[e + 2]), s[e + 3] = fmaf(w, x.w * tk.s0_mul, s[e + 3]);
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (col + e < tk.Dv) s[e] = fmaf(w, s0[e * tk.s0s[3]] * tk.s0_mul, s[e]);
+        }
       }
     }
     const uint32_t srow = sm + SH::off_s + (uint32_t)(wg >> 1) * kBlk + (uint32_t)t * 128;
@@ -591,113 +646,102 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
                pack_bf16(s[8 * e + 2], s[8 * e + 3]), pack_bf16(s[8 * e + 4], s[8 * e + 5]), pack_bf16(s[8 * e + 6], s[8 * e + 7]));
       fence_async_smem();
     };
-    // Zeroes v behind the last token of the chunk, where it may hold anything, and 0 * NaN is NaN.  Products with v wait
-    // for X in such a chunk.
-    auto clean_v = [&](int c) {
-      const int m = tokens(c);
-      if (m == kTok || n == lp.L) return;
-      const uint32_t v = sm + (uint32_t)(c & 1) * SH::stage + 2 * SH::q_bytes + (uint32_t)(wg >> 1) * kBlk;
-      for (int e = t; e < (kTok - m) * 4; e += 128)
-        sts128(v + (uint32_t)(m + (e >> 2)) * 128 + (uint32_t)(4 * (wg & 1) + (e & 3)) * 16, 0, 0, 0, 0);
-      fence_async_smem();
-    };
     if (!LOCAL) {
       publish();
       mbar_arrive(bars + B_ST);
     }
     // lambda^128 as a sum of two floats: its rounding would come back with every chunk
     const float whole = dec.pow(kTok), whole_lo = dec.pow_rest(kTok, whole);
-    constexpr int TPW = kTok / NW;   // positions whose X this warpgroup makes
     // Address of the lane's row of the K tiles of the warp's first 16 rows d and first 16 positions: tiles (d, position) are
     // (0-7, 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15); 16 rows d on is two 16-byte pieces on, under the swizzle.
-    const int dw = DQ == 64 ? (warp & 1) * 32 : (warp & 3) * 32;
-    const uint32_t kaddr = SH::q_bytes + (uint32_t)(dw >> 6) * kBlk + (uint32_t)(((lane >> 4) & 1) * 8 + (lane & 7)) * 128 +
+    const int dw = SH::split ? (quad & 1) * 32 : quad * 32;
+    const uint32_t kaddr = SH::off_k + (uint32_t)(dw >> 6) * kBlk + (uint32_t)(((lane >> 4) & 1) * 8 + (lane & 7)) * 128 +
                            ((((uint32_t)(dw & 63) >> 3) + ((uint32_t)(lane >> 3) & 1)) ^ (uint32_t)(lane & 7)) * 16;
-    for (int c = 0; c < nc; c++) {
-      const uint32_t ph = c & 1, st = sm + (uint32_t)(c & 1) * SH::stage;
-      const int m = tokens(c);
-      const int off = tk.off && before == 0 && c == 0;
-      if (!wwait(B_KV0 + (c & 1), (c >> 1) & 1)) break;
-      clean_v(c);
-      // The first two parts of X, or the third.  Lanes of X are rows d of the state, its columns pairs of positions: K's
-      // tiles come transposed from shared memory in the very arrangement that the 16 x 128b store takes.
-      auto make_x = [&](bool third) {
+    // Positions whose X the warp makes, and the column of X that the first of them has.
+    constexpr int kMine = SH::split ? 64 / NW : kTok / NW;
+    const int first = SH::split ? (quad >> 1) * 64 + wg * kMine : wg * kMine;
+    const uint32_t xcol = (uint32_t)(wg * kMine) / 2;
+    static_assert(kMine % 32 == 0, "32 positions at a time");
+
+    // Parts of X of chunk c: the first two (and the third, whole_x), or the third alone.  Lanes of X are rows d of the state,
+    // its columns pairs of positions: K's tiles come transposed from shared memory in the very arrangement that the 16 x 128b
+    // store takes.  Each part but the last is cut off, not rounded, so that what is left is exact.
+    auto make_x = [&](int c, int m, bool third) {
+      const uint32_t st = stage_at(c);
 #pragma unroll 1
-        for (int j0 = wg * TPW; j0 < (wg + 1) * TPW; j0 += 32) {
-          if (DQ == 64 && third && (j0 < kTok / 2) != (t < 64)) {   // each half of the lanes takes half the positions
-            const uint32_t none[8] = {};
-            tmem_st_16x128b_x4(tl + SH::c_x + j0 / 2, none);
-            tmem_st_16x128b_x4(tl + (16u << 16) + SH::c_x + j0 / 2, none);
-            continue;
-          }
-          float w[8];   // of positions j0 + 8 i + 2 (lane % 4) + {0, 1}
-          const int wi = (rev ? 32 : kTok - m) + j0 + 2 * (lane & 3);
+      for (int jj = 0; jj < kMine; jj += 32) {
+        const int j0 = first + jj;
+        float w[8];   // of positions j0 + 8 i + 2 (lane % 4) + {0, 1}
+        const int wi = (rev ? 32 : kTok - m) + j0 + 2 * (lane & 3);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float* at = tab + min(wi + 8 * i, 158);   // behind the last token: the zeros
-            w[2 * i] = at[0], w[2 * i + 1] = at[1];
-          }
+        for (int i = 0; i < 4; i++) {
+          const float* at = tab + min(wi + 8 * i, 158);   // behind the last token: the zeros
+          w[2 * i] = at[0], w[2 * i + 1] = at[1];
+        }
 #pragma unroll 1
-          for (int half = 0; half < 2; half++) {   // 16 rows each
-            uint32_t r[8], z[8];
-            const uint32_t addr = (kaddr + st + (uint32_t)j0 * 128) ^ (uint32_t)(32 * half);
-            ldsm_t(addr, *(uint32_t(*)[4]) & r[0]);
-            ldsm_t(addr + 16 * 128, *(uint32_t(*)[4]) & r[4]);
-            if (m < kTok) {   // behind the last token k may hold anything
+        for (int half = 0; half < 2; half++) {   // 16 rows each
+          uint32_t r[8], y[8], z[8];
+          const uint32_t addr = (kaddr + st + (uint32_t)j0 * 128) ^ (uint32_t)(32 * half);
+          ldsm_t(addr, *(uint32_t(*)[4]) & r[0]);
+          ldsm_t(addr + 16 * 128, *(uint32_t(*)[4]) & r[4]);
+          if (m < kTok) {   // behind the last token k may hold anything
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const int j = j0 + 8 * i + 2 * (lane & 3);
-                const uint32_t mask = (j < m ? 0xffffu : 0u) | (j + 1 < m ? 0xffff0000u : 0u);
-                r[2 * i] &= mask;
-                r[2 * i + 1] &= mask;
-              }
+            for (int i = 0; i < 4; i++) {
+              const int j = j0 + 8 * i + 2 * (lane & 3);
+              const uint32_t mask = (j < m ? 0xffffu : 0u) | (j + 1 < m ? 0xffff0000u : 0u);
+              r[2 * i] &= mask;
+              r[2 * i + 1] &= mask;
             }
-            const uint32_t to = tl + ((uint32_t)(16 * half) << 16) + SH::c_x + j0 / 2;
-            // each part but the last is cut off, so that what is left is exact
-            if (DQ == 64 && !third && t < 64) {
+          }
+          const uint32_t to = tl + ((uint32_t)(16 * half) << 16) + SH::c_x + xcol + jj / 2;
+          if (SH::whole_x && three) {
 #pragma unroll
-              for (int i = 0; i < 8; i++) r[i] = upper2(mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]}));
-            } else if (!third) {
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
-                if (DQ == 128) z[i] = upper2(x);
-                x = sub2(x, cut2(x));
-                r[i] = pack_bf16(x.a, x.b);
-              }
-              if (DQ == 128) tmem_st_16x128b_x4(to, z);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
-                x = sub2(x, cut2(x));
-                x = sub2(x, cut2(x));
-                r[i] = pack_bf16(x.a, x.b);
-              }
+            for (int i = 0; i < 8; i++) {
+              F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
+              r[i] = upper2(x);
+              x = sub2(x, cut2(x));
+              y[i] = upper2(x);
+              x = sub2(x, cut2(x));
+              z[i] = pack_bf16(x.a, x.b);
             }
-            tmem_st_16x128b_x4(DQ == 128 && !third ? to + 64 : to, r);
+            tmem_st_16x128b_x4(to, r);
+            tmem_st_16x128b_x4(to + SH::part_cols, y);
+            tmem_st_16x128b_x4(to + 2 * SH::part_cols, z);
+          } else if (!third) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
+              r[i] = upper2(x);
+              x = sub2(x, cut2(x));
+              y[i] = pack_bf16(x.a, x.b);
+            }
+            tmem_st_16x128b_x4(to, r);
+            tmem_st_16x128b_x4(to + SH::part_cols, y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
+              x = sub2(x, cut2(x));
+              x = sub2(x, cut2(x));
+              r[i] = pack_bf16(x.a, x.b);
+            }
+            tmem_st_16x128b_x4(to, r);
           }
         }
-        tmem_wait_st();
-        tc_fence_before();
-      };
-      make_x(false);
-      mbar_arrive(bars + B_X);
-      if (!wwait(B_INC, ph)) break;
-      tc_fence_after();
-      if (three) {
-        make_x(true);
-        mbar_arrive(bars + B_X2);
-        if (!wwait(B_INC2, ph)) break;
       }
-      if (!LOCAL && !wwait(B_O1, ph)) break;   // the product with the old S has been taken
-      tc_fence_after();
+      tmem_wait_st();
+      tc_fence_before();
+    };
+    // S <- lambda^m S + X^T V of chunk c, whose product is complete
+    auto take = [&](int c) {
+      const int m = tokens(c), off = tk.off && before == 0 && c == 0;
       float w = whole, w_lo = whole_lo;
       if (m - off < kTok) w = power(m - off), w_lo = 0.f;
+      const uint32_t from = tl + SH::c_inc(c) + (SH::split ? (uint32_t)(quad >> 1) * 64 : 0) + wg * 32;
 #pragma unroll
       for (int q = 0; q < 2; q++) {
         uint32_t r[16];
-        tmem_ld16(tl + SH::c_kv + col + q * 16, r);
+        tmem_ld16(from + q * 16, r);
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
@@ -707,14 +751,40 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
         }
       }
       tc_fence_before();
-      if (!LOCAL && c + 1 < nc) publish();
+    };
+    for (int c = 0; c < nc; c++) {
+      const uint32_t ph = c & 1;
+      const int m = tokens(c);
+      if (!wwait(B_KV + c % NS, sph(c))) break;
+      if (m < kTok && n < lp.L) {   // v behind the last token may hold anything, and 0 * NaN is NaN
+        const uint32_t v = stage_at(c) + SH::off_v + (uint32_t)(wg >> 1) * kBlk;
+        for (int e = t; e < (kTok - m) * 4; e += 128)
+          sts128(v + (uint32_t)(m + (e >> 2)) * 128 + (uint32_t)(4 * (wg & 1) + (e & 3)) * 16, 0, 0, 0, 0);
+        fence_async_smem();
+      }
+      make_x(c, m, false);
+      mbar_arrive(bars + B_X);
+      if (LOCAL && c > 0) take(c - 1);   // one chunk behind, while this one's product runs
+      if (!wwait(B_INC, ph)) break;
+      tc_fence_after();
+      if (LOCAL) continue;
+      if (three && !SH::whole_x) {
+        make_x(c, m, true);
+        mbar_arrive(bars + B_X2);
+        if (!wwait(B_INC2, ph)) break;
+      }
+      if (!wwait(B_O1 + grp(c), aph(c))) break;   // the product with the old S has been taken
+      tc_fence_after();
+      take(c);
+      if (c + 1 < nc) publish();
       mbar_arrive(bars + B_ST);
+      mbar_arrive(bars + B_REL + c % NS);
     }
+    if (LOCAL && nc > 0) take(nc - 1);
     // the state that the segment leaves (after a wait that gave up: whatever it is, but every thread comes by)
     if (LOCAL || (tk.s1 && g == lp.G - 1)) {
-      if constexpr (DQ == 64) {   // add the two parts; S's shared memory is free: nothing reads it any more
-        // every warpgroup is behind its last use of the tile
-        asm volatile("bar.sync 5, %0;" ::"n"(128 * SH::NW) : "memory");
+      if constexpr (SH::split) {   // add the two halves, in S's shared memory, once all warpgroups are through with it
+        asm volatile("bar.sync 5, %0;" ::"n"(128 * NW) : "memory");
         float* x = (float*)(smem + SH::off_s + wg * (kBlk / 2));
         if (t >= 64) {
 #pragma unroll
@@ -728,16 +798,22 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
       }
       if (main_part && d < tk.D) {
         if (LOCAL) {
-          float* out = tk.loc + (((long long)bh * lp.G + g) * tk.D + d) * tk.Dv + col;
+          float* out = tk.loc + ((long long)bh * lp.G + g) * tk.D * tk.Dv + mine;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (col + e < tk.Dv) *(float4*)(out + e) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+          for (int e = 0; e < 32; e++)
+            if (col + e < tk.Dv) out[(long long)e * tk.D] = s[e];
         } else {
           const float w = tk.s1_mul * (tk.s1_decay && n > 0 ? power(1) : 1.f);
           float* out = tk.s1 + b * tk.s1s[0] + h * tk.s1s[1] + d * tk.s1s[2] + (long long)col * tk.s1s[3];
+          if (tk.s1s[3] == 1 && ((uintptr_t)out & 15) == 0) {
 #pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (col + e < tk.Dv) out[e * tk.s1s[3]] = w * s[e];
+            for (int e = 0; e < 32; e += 4)
+              if (col + e < tk.Dv) *(float4*)(out + e) = make_float4(w * s[e], w * s[e + 1], w * s[e + 2], w * s[e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (col + e < tk.Dv) out[e * tk.s1s[3]] = w * s[e];
+          }
         }
       }
     }
@@ -746,7 +822,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV>::threads, Shape<DQ, DV>::alias ?
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == SH::threads / 32 - 1) tmem_dealloc(tm, SH::cols);
+  if (warp == SH::threads / 32 - 1) tmem_dealloc(tm, 512);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -770,7 +846,7 @@ EncodeFn encode_fn() {
 
 // What a tensor map of [B][H][L][D] bf16 needs: 16-byte aligned rows, and strides of their own.
 bool mappable(const void* p, const long long (&s)[3], int B, int H, int L, int D) {
-  if (((uintptr_t)p & 15) != 0 || D % 8 != 0 || D > 128) return false;
+  if (((uintptr_t)p & 15) != 0 || D % 8 != 0) return false;
   const int n[3] = {B, H, L};
   for (int i = 0; i < 3; i++)
     if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 != 0 || s[i] >= (1ll << 38))) return false;
@@ -787,14 +863,18 @@ bool make_map(CUtensorMap* m, const void* p, const long long (&s)[3], int B, int
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Columns of v in a CTA.
+int tile_v(int D, int Dv) { return D > 64 && Dv > 64 ? 128 : 64; }
+
 template <int DQ, int DV>
 cudaError_t launch_shape(const LaTcParams& prm, cudaStream_t st) {
-  using SH = Shape<DQ, DV>;
-  const dim3 grid((unsigned)(prm.p.B * prm.p.H * prm.p.G * prm.p.ntask));
+  const dim3 grid((unsigned)(prm.p.B * prm.p.H * prm.p.G * prm.p.ntask * prm.slices));
   if (prm.p.G > 1) {
+    using SH = Shape<DQ, DV, true>;
     const cudaError_t ce = launch(la_tc_kernel<DQ, DV, true>, grid, SH::threads, (int)SH::smem, st, prm);
     if (ce != cudaSuccess) return ce;
   }
+  using SH = Shape<DQ, DV, false>;
   return launch(la_tc_kernel<DQ, DV, false>, grid, SH::threads, (int)SH::smem, st, prm);
 }
 
@@ -804,13 +884,14 @@ bool la_tc_takes(const LaParams& p) {
   if (p.L < 1 || !encode_fn()) return false;
   for (int i = 0; i < p.ntask; i++) {
     const LaTask& t = p.task[i];
-    if (!mappable(t.q, t.qs, p.B, p.H / t.qdiv, p.L, t.D) || !mappable(t.k, t.ks, p.B, p.H / t.kdiv, p.L, t.D) ||
-        !mappable(t.v, t.vs, p.B, p.H / t.vdiv, p.L, t.Dv) || t.Dv % 8 != 0)
+    if (t.D > 128 || !mappable(t.q, t.qs, p.B, p.H / t.qdiv, p.L, t.D) || !mappable(t.k, t.ks, p.B, p.H / t.kdiv, p.L, t.D) ||
+        !mappable(t.v, t.vs, p.B, p.H / t.vdiv, p.L, t.Dv) || !mappable(t.y, t.ys, p.B, p.H, p.L, t.Dv))
       return false;
-    if (!mappable(t.y, t.ys, p.B, p.H, p.L, t.Dv)) return false;
   }
   return true;
 }
+
+int la_tc_slices(int D, int Dv) { return (Dv + tile_v(D, Dv) - 1) / tile_v(D, Dv); }
 
 cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
   // tasks of one tile shape go into one launch
@@ -821,21 +902,25 @@ cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
     prm.p = p;
     prm.p.ntask = 0;
     prm.blocks = p.seg / kTok;
-    const bool q2 = p.task[i].D > 64, v2 = p.task[i].Dv > 64;
+    prm.slices = 1;
+    const bool q2 = p.task[i].D > 64;
+    const int dv = tile_v(p.task[i].D, p.task[i].Dv);
     for (int j = i; j < p.ntask; j++) {
       const LaTask& t = p.task[j];
-      if (done[j] || (t.D > 64) != q2 || (t.Dv > 64) != v2) continue;
+      if (done[j] || (t.D > 64) != q2 || tile_v(t.D, t.Dv) != dv) continue;
       done[j] = true;
       const int k = prm.p.ntask++;
       prm.p.task[k] = t;
+      const int sl = la_tc_slices(t.D, t.Dv);
+      if (sl > prm.slices) prm.slices = sl;
       if (!make_map(&prm.map[k][0], t.q, t.qs, p.B, p.H / t.qdiv, p.L, t.D) ||
           !make_map(&prm.map[k][1], t.k, t.ks, p.B, p.H / t.kdiv, p.L, t.D) ||
           !make_map(&prm.map[k][2], t.v, t.vs, p.B, p.H / t.vdiv, p.L, t.Dv) ||
           (!t.y_f32 && !make_map(&prm.map[k][3], t.y, t.ys, p.B, p.H, p.L, t.Dv)))
         return cudaErrorInvalidValue;
     }
-    const cudaError_t ce = q2 ? (v2 ? launch_shape<128, 128>(prm, st) : launch_shape<128, 64>(prm, st))
-                              : (v2 ? launch_shape<64, 128>(prm, st) : launch_shape<64, 64>(prm, st));
+    const cudaError_t ce = !q2 ? launch_shape<64, 64>(prm, st) : dv == 128 ? launch_shape<128, 128>(prm, st)
+                                                                           : launch_shape<128, 64>(prm, st);
     if (ce != cudaSuccess) return ce;
   }
   return cudaSuccess;

@@ -54,6 +54,7 @@ def check(t, ld, scale, lengths=None, backward=True):
         assert torch.isfinite(x).all(), name
         bad = off > tol
         assert not bad.any(), (name, off[bad].max().item(), (off / tol).max().item(), bad.nonzero()[0].tolist())
+    sf.linear_attention_check()
     return got
 
 
@@ -266,6 +267,35 @@ def test_streams_graphs_and_compile():
     compiled = torch.compile(lambda q, k, v, s: ops.linear_attention(q, k, v, ld, 0.125, s), fullgraph=True)
     assert all(torch.equal(a, b) for a, b in zip(compiled(t["q"], t["k"], t["v"], t["s0"]), want))
     del back
+
+
+def test_threads_of_their_own():
+    """Calls from threads that have made no CUDA call yet (autograd's are such), while others call too."""
+    import threading
+    t = make(2, 4, 4, 500, 64, 64, BF, 14)
+    ld = decays(4, "cuda")
+    want = sf.linear_attention(t["q"], t["k"], t["v"], ld, 0.125, t["s0"])
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [sf.linear_attention(t["q"], t["k"], t["v"], ld, 0.125, t["s0"]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    for n in (1, 4):      # the second time with memory at hand, so that nothing else touches CUDA first
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(n)]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+        assert len(got) == n
+        assert all(torch.equal(a, b) for runs in got.values() for o in runs for a, b in zip(o, want))
+        got.clear()
+    q = t["q"].clone().requires_grad_()
+    y, _ = ops.linear_attention(q, t["k"], t["v"], ld, 0.125, t["s0"])
+    y.backward(t["dy"])
+    assert torch.equal(q.grad, sf.linear_attention_backward(t["q"], t["k"], t["v"], ld, t["dy"], None, 0.125, t["s0"])[0])
 
 
 def test_offsets_beyond_32_bits():
