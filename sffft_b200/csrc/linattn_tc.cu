@@ -30,6 +30,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "../../include/sffft.h"
 #include "launch.h"
 #include "linattn.h"
@@ -472,8 +474,9 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
                  keep || part > first || k > 0);
     };
     auto x_v = [&](int c) {
-      // LOCAL: X of a chunk comes after the state of the last but one has been taken over from these columns
-      if (!wwait(B_KV + c % NS, sph(c)) || !wwait(B_X, c & 1)) return false;
+      // The increment's columns have been taken over: from the last chunk, once its state is published; LOCAL, from the last
+      // but one, before X of this one came.
+      if (!wwait(B_KV + c % NS, sph(c)) || !wwait(B_X, c & 1) || (!LOCAL && !wwait(B_ST, c & 1))) return false;
       const bool all = any(SH::whole_x && three);
       tc_fence_after();
       if (elect_one()) {
@@ -496,15 +499,14 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       return true;
     };
     // The order in which operands become ready (asking for whichever is took 10 questions a product, 500 cycles and more).
-    // Split: from the publication of S on, X of a chunk takes about 1150 cycles, in which Q S and the next chunk's Q K^T run
-    // (the other A warpgroup's O has been read by then); then the state's product, which the next chunk waits for.
+    // The state's product goes first: the chain from one to the next (X, and taking the state over) is the longest.
     if constexpr (LOCAL) {
       for (int c = 0; any(c < nc); c++)
         if (!x_v(c)) break;
     } else if constexpr (SH::split) {
       if (any(nc > 0) && q_k(0))
         for (int c = 0; any(c < nc); c++)
-          if (!q_s(c) || (any(c + 1 < nc) && !q_k(c + 1)) || !x_v(c) || !p_v(c)) break;
+          if (!x_v(c) || !q_s(c) || (any(c + 1 < nc) && !q_k(c + 1)) || !p_v(c)) break;
     } else {
       for (int c = 0; any(c < nc); c++)
         if (!q_k(c) || !x_v(c) || !q_s(c) || !p_v(c) || (any(later) && !x_v_third(c))) break;
@@ -638,33 +640,16 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
     for (int e = 0; e < 32; e++) s[e] = 0.f;
     const long long mine = (long long)col * tk.D + d;   // of the segments' states, which are kept transposed: lanes are rows
     if (!LOCAL && main_part && d < tk.D) {
-      const float* loc = tk.loc + (long long)bh * lp.G * tk.D * tk.Dv + mine;
-      const long long step = (long long)tk.D * tk.Dv;
-      for (int gg = 0; gg < g; gg++) {
-        const int a = tokens_before(min(gg * prm.blocks, nblk), n, nblk, rev);
-        const int z = tokens_before(min((gg + 1) * prm.blocks, nblk), n, nblk, rev);
-        if (z == a) break;
-        const float w = dec.pow(z - a);
+      if (g > 0) {   // what the earlier segments leave, s0 included
+        const float* in = tk.loc + ((long long)bh * lp.G + g - 1) * tk.D * tk.Dv + mine;
 #pragma unroll
         for (int e = 0; e < 32; e++)
-          if (col + e < tk.Dv) s[e] = fmaf(w, s[e], loc[gg * step + (long long)e * tk.D]);
-      }
-      if (tk.s0) {
-        const float w = dec.pow(before - (tk.off && before > 0));
+          if (col + e < tk.Dv) s[e] = in[(long long)e * tk.D];
+      } else if (tk.s0) {
         const float* s0 = tk.s0 + b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + (long long)col * tk.s0s[3];
-        if (tk.s0s[3] == 1 && ((uintptr_t)s0 & 15) == 0) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (col + e < tk.Dv) {
-              const float4 x = *(const float4*)(s0 + e);
-              s[e] = fmaf(w, x.x * tk.s0_mul, s[e]), s[e + 1] = fmaf(w, x.y * tk.s0_mul, s[e + 1]);
-              s[e + 2] = fmaf(w, x.z * tk.s0_mul, s[e + 2]), s[e + 3] = fmaf(w, x.w * tk.s0_mul, s[e + 3]);
-            }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (col + e < tk.Dv) s[e] = fmaf(w, s0[e * tk.s0s[3]] * tk.s0_mul, s[e]);
-        }
+        for (int e = 0; e < 32; e++)
+          if (col + e < tk.Dv) s[e] = s0[e * tk.s0s[3]] * tk.s0_mul;
       }
     }
     const uint32_t srow = sm + SH::off_s + (uint32_t)(wg >> 1) * kBlk + (uint32_t)t * 128;
@@ -767,24 +752,20 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       float w = whole, w_lo = whole_lo;
       if (m - off < kTok) w = power(m - off), w_lo = 0.f;
       const uint32_t from = tl + SH::c_inc(c) + (SH::split ? (uint32_t)(quad >> 1) * 64 : 0) + wg * 32;
+      uint32_t r[32];
+      tmem_ld32(from, r);
+      tmem_wait_ld();
 #pragma unroll
-      for (int q = 0; q < 2; q++) {
-        uint32_t r[16];
-        tmem_ld16(from + q * 16, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float &x = s[q * 16 + e], &y = s[q * 16 + e + 1];
-          const F2 z = fma2({w, w}, {x, y}, fma2({w_lo, w_lo}, {x, y}, {__uint_as_float(r[e]), __uint_as_float(r[e + 1])}));
-          x = z.a, y = z.b;
-        }
+      for (int e = 0; e < 32; e += 2) {
+        const F2 z = fma2({w, w}, {s[e], s[e + 1]}, fma2({w_lo, w_lo}, {s[e], s[e + 1]}, {__uint_as_float(r[e]), __uint_as_float(r[e + 1])}));
+        s[e] = z.a, s[e + 1] = z.b;
       }
       tc_fence_before();
     };
-    for (int c = 0; c < nc; c++) {
-      const uint32_t ph = c & 1;
+    // X of chunk c, once its tiles are there
+    auto give_x = [&](int c) {
       const int m = tokens(c);
-      if (!wwait(B_KV + c % NS, sph(c))) break;
+      if (!wwait(B_KV + c % NS, sph(c))) return false;
       if (m < kTok && n < lp.L) {   // v behind the last token may hold anything, and 0 * NaN is NaN
         const uint32_t v = stage_at(c) + SH::off_v + (uint32_t)(wg >> 1) * kBlk;
         for (int e = t; e < (kTok - m) * 4; e += 128)
@@ -793,23 +774,27 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       }
       make_x(c, m, false);
       mbar_arrive(bars + B_X);
-      if (LOCAL && c > 0) take(c - 1);   // one chunk behind, while this one's product runs
-      if (!wwait(B_INC, ph)) break;
-      tc_fence_after();
-      if (LOCAL) continue;
-      if (three && !SH::whole_x) {
-        make_x(c, m, true);
-        mbar_arrive(bars + B_X2);
-        if (!wwait(B_INC2, ph)) break;
+      return true;
+    };
+    // X of the next chunk goes before this one's state: it needs only the columns that this one's product has read.
+    if (nc > 0 && give_x(0))
+      for (int c = 0; c < nc; c++) {
+        if (!wwait(B_INC, c & 1)) break;
+        tc_fence_after();
+        if (three && !SH::whole_x) {
+          make_x(c, tokens(c), true);
+          mbar_arrive(bars + B_X2);
+          if (!wwait(B_INC2, c & 1)) break;
+          tc_fence_after();
+        }
+        if (c + 1 < nc && !give_x(c + 1)) break;
+        if (!LOCAL && !wwait(B_O1 + grp(c), aph(c))) break;   // the product with the old S has been taken
+        take(c);
+        if (LOCAL) continue;
+        if (c + 1 < nc) publish();
+        mbar_arrive(bars + B_ST);
+        mbar_arrive(bars + B_REL + c % NS);
       }
-      if (!wwait(B_O1 + grp(c), aph(c))) break;   // the product with the old S has been taken
-      tc_fence_after();
-      take(c);
-      if (c + 1 < nc) publish();
-      mbar_arrive(bars + B_ST);
-      mbar_arrive(bars + B_REL + c % NS);
-    }
-    if (LOCAL && nc > 0) take(nc - 1);
     // the state that the segment leaves (after a wait that gave up: whatever it is, but every thread comes by)
     if (LOCAL || (tk.s1 && g == lp.G - 1)) {
       if constexpr (SH::split) {   // add the two halves, in S's shared memory, once all warpgroups are through with it
@@ -852,6 +837,38 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   __syncthreads();
   tc_fence_after();
   if (warp == SH::threads / 32 - 1) tmem_dealloc(*slot, 512);
+}
+
+// What the segments up to each one leave, from what each leaves alone, in place; the last one's is not needed.  A thread
+// takes one element of a state; the loads of all segments are independent of the sums.
+__global__ void __launch_bounds__(256) la_prefix_kernel(const __grid_constant__ LaTcParams prm) {
+  const LaParams& lp = prm.p;
+  const LaTask& tk = lp.task[blockIdx.z];
+  const int size = tk.D * tk.Dv, e = blockIdx.y * 256 + threadIdx.x;   // [Dv][D]
+  const int bh = blockIdx.x, b = bh / lp.H, h = bh % lp.H;
+  if (e >= size) return;
+  int n = lp.L;
+  if (lp.len) n = min(max(lp.len[b], 0), lp.L);
+  const int nblk = (n + kTok - 1) / kTok;
+  const LaDecay dec(lp.ld[h]);
+  float s = 0.f;
+  if (tk.s0) s = tk.s0[b * tk.s0s[0] + h * tk.s0s[1] + (e % tk.D) * tk.s0s[2] + (e / tk.D) * tk.s0s[3]] * tk.s0_mul;
+  float* loc = tk.loc + (long long)bh * lp.G * size + e;
+  for (int g0 = 0; g0 < lp.G - 1; g0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (g0 + i < lp.G - 1) x[i] = loc[(long long)(g0 + i) * size];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int g = g0 + i;
+      if (g >= lp.G - 1) break;
+      const int a = tokens_before(min(g * prm.blocks, nblk), n, nblk, tk.rev);
+      const int m = tokens_before(min((g + 1) * prm.blocks, nblk), n, nblk, tk.rev) - a;
+      if (m > 0) s = fmaf(dec.pow(m - (tk.off && a == 0)), s, x[i]);
+      loc[(long long)g * size] = s;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -900,7 +917,11 @@ cudaError_t launch_shape(const LaTcParams& prm, cudaStream_t st) {
   const dim3 grid((unsigned)(prm.p.B * prm.p.H * prm.p.G * prm.p.ntask * prm.slices));
   if (prm.p.G > 1) {
     using SH = Shape<DQ, DV, true>;
-    const cudaError_t ce = launch(la_tc_kernel<DQ, DV, true>, grid, SH::threads, (int)SH::smem, st, prm);
+    cudaError_t ce = launch(la_tc_kernel<DQ, DV, true>, grid, SH::threads, (int)SH::smem, st, prm);
+    if (ce != cudaSuccess) return ce;
+    int size = 0;
+    for (int i = 0; i < prm.p.ntask; i++) size = std::max(size, prm.p.task[i].D * prm.p.task[i].Dv);
+    ce = launch(la_prefix_kernel, dim3((unsigned)(prm.p.B * prm.p.H), (unsigned)((size + 255) / 256), (unsigned)prm.p.ntask), 256, 0, st, prm);
     if (ce != cudaSuccess) return ce;
   }
   using SH = Shape<DQ, DV, false>;
