@@ -559,10 +559,9 @@ def _need_cuda(t, what):
 
 def _heads_like(like, B, H, L, D, dtype):
     """An empty [B][H][L][D] tensor whose memory is ordered like `like`'s: [B][L][H][D] where its positions are outermost."""
-    import torch
     if like.stride(2) > like.stride(1) and H > 1:
-        return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=dtype, device=like.device)
-    return torch.empty((B, H, L, D), dtype=dtype, device=like.device)
+        return like.new_empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=dtype)
+    return like.new_empty((B, H, L, D), dtype=dtype)
 
 
 def _unit(t):
@@ -630,7 +629,7 @@ def linear_attention(q, k, v, log_decay, scale=1.0, initial_state=None, lengths=
     _need_cuda(q, "linear_attention")
     q, k, v, dev = _unit(q), _unit(k), _unit(v), q.device
     y = _heads_like(q, B, H, L, Dv, q.dtype)
-    s1 = torch.empty((B, H, D, Dv), dtype=torch.float32, device=dev)
+    s1 = q.new_empty((B, H, D, Dv), dtype=torch.float32)
     desc = _LA_DESC.pack(B, H, Hkv, L, D, Dv, io, dev.index, scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                          *y.stride()[:3])
     work, wp, wn = _la_workspace(desc, 0, dev)
@@ -653,7 +652,7 @@ def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1
         dy = dy.contiguous()
     dq, dk = _heads_like(q, B, H, L, D, q.dtype), _heads_like(k, B, Hkv, L, D, q.dtype)
     dv = _heads_like(v, B, Hkv, L, Dv, q.dtype)
-    ds0 = None if initial_state is None else torch.empty((B, H, D, Dv), dtype=torch.float32, device=dev)
+    ds0 = None if initial_state is None else q.new_empty((B, H, D, Dv), dtype=torch.float32)
     desc = _LA_DESC.pack(B, H, Hkv, L, D, Dv, io, dev.index, scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], 0, 0, 0)
     grads = _LA_GRADS.pack(*dy.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])
     work, wp, wn = _la_workspace(desc, 1, dev)
@@ -708,7 +707,7 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=1.0):
             raise ValueError("all tensors must be on one device")
     _need_cuda(q, "linear_attention_step")
     q, k, v = _unit(q), _unit(k), _unit(v)
-    y = torch.empty((B, H, Dv), dtype=q.dtype, device=dev)
+    y = q.new_empty((B, H, Dv))
     d = _LA_STEP.pack(B, H, Hkv, D, Dv, pool, io, dev.index, scale, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], H * Dv, Dv,
                       stride[0])
     (ld, ldp), (sl, slp) = _plain(log_decay), _plain(slots)
@@ -779,6 +778,12 @@ def check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, d
     return C, kind, first
 
 
+def _packed_like(t):
+    """An empty contiguous tensor of t's shape and type."""
+    import torch
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _as_rows(t, C):
     """(tensor, stride of a row) of a [..., C] tensor whose rows are evenly spaced (a copy where they are not)."""
     if t.is_contiguous():
@@ -838,10 +843,10 @@ def block_norm(x=None, y=None, gate=None, post_weight=None, weight=None, scale=1
     given = x
     d, x, y, gate, pw, w, lead, _, rows = _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     dev = lead.device
-    h = given if y is None else torch.empty(lead.shape, dtype=lead.dtype if x is None else x.dtype, device=dev)
-    n = None if w is None else torch.empty(lead.shape, dtype=lead.dtype, device=dev)
-    r1 = torch.empty((rows, groups), dtype=torch.float32, device=dev) if stats and pw is not None else None
-    r2 = torch.empty((rows,), dtype=torch.float32, device=dev) if stats and w is not None else None
+    h = given if y is None else _packed_like(lead if x is None else x)
+    n = None if w is None else _packed_like(lead)
+    r1 = lead.new_empty((rows, groups), dtype=torch.float32) if stats and pw is not None else None
+    r2 = lead.new_empty((rows,), dtype=torch.float32) if stats and w is not None else None
     if rows:
         _check(lib().sffft_block_norm(d, _ptr(x), _ptr(y), _ptr(gate), _ptr(pw), _ptr(w), _ptr(h), _ptr(n), _ptr(r1), _ptr(r2),
                                       _current(dev.index)), "block_norm")
@@ -871,8 +876,7 @@ def block_norm_backward(dh, dn, x=None, y=None, gate=None, post_weight=None, wei
             raise ValueError("all tensors must be on one device")
     dh, dn = (t if t is None or t.is_contiguous() else t.contiguous() for t in (dh, dn))
     dev = lead.device
-    dx, dy, dgate, dpw, dw = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
-                              for t in (x, y, gate, pw, w))
+    dx, dy, dgate, dpw, dw = (None if t is None else _packed_like(t) for t in (x, y, gate, pw, w))
     if not rows:   # empty buffers have no address to pass
         for t in (dgate if kind == "channel" else None, dpw, dw):
             if t is not None:

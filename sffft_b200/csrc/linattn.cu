@@ -2,6 +2,7 @@
 // that share a key and value head.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -103,7 +104,9 @@ __global__ void __launch_bounds__(kStepThreads) la_step_kernel(const __grid_cons
   }
 }
 
-// Sum over the query heads that share a key and value head, in head order: out[b][g][t] = sum_r w[b][g R + r][t].
+// Sum over the query heads that share a key and value head, in head order: out[b][g][t] = sum_r w[b][g R + r][t].  Bound by
+// memory: a thread takes VEC values of a position; blockIdx.y is the row and head, so that no index needs a division but
+// that by the D / VEC pieces of a position.
 struct LaReduceParams {
   const float* w;   // [B][G R][L][D]
   void* out;
@@ -111,15 +114,30 @@ struct LaReduceParams {
   int B, G, R, L, D;
 };
 
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(256) la_reduce_kernel(const __grid_constant__ LaReduceParams p) {
-  const long long total = (long long)p.B * p.G * p.L * p.D, plane = (long long)p.L * p.D;
-  for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-    const long long bg = e / plane, at = e % plane, t = at / p.D, d = at % p.D, b = bg / p.G, g = bg % p.G;
-    const float* w = p.w + bg * p.R * plane + at;
-    float s = 0.f;
-    for (int r = 0; r < p.R; r++) s += w[r * plane];
-    stf((T*)p.out + b * p.os[0] + g * p.os[1] + t * p.os[2] + d, s);
+  const long long plane = (long long)p.L * p.D;
+  const int pieces = p.D / VEC;
+  const unsigned total = (unsigned)p.L * (unsigned)pieces;   // below 2^31: D is at most 256 and L 2^30 / 128 or memory ends
+  for (int bg = blockIdx.y; bg < p.B * p.G; bg += gridDim.y) {
+    const float* w = p.w + (long long)bg * p.R * plane;
+    T* out = (T*)p.out + (bg / p.G) * p.os[0] + (bg % p.G) * p.os[1];
+    for (unsigned e = blockIdx.x * 256u + threadIdx.x; e < total; e += gridDim.x * 256u) {
+      const unsigned t = e / (unsigned)pieces, d = (e - t * (unsigned)pieces) * VEC;
+      float s[VEC] = {};
+      for (int r = 0; r < p.R; r++) {
+        const float* x = w + r * plane + (long long)e * VEC;
+        if constexpr (VEC == 8) {
+          const float4 a = *(const float4*)x, c = *(const float4*)(x + 4);
+          s[0] += a.x, s[1] += a.y, s[2] += a.z, s[3] += a.w, s[4] += c.x, s[5] += c.y, s[6] += c.z, s[7] += c.w;
+        } else {
+          s[0] += *x;
+        }
+      }
+      T* to = out + (long long)t * p.os[2] + d;
+#pragma unroll
+      for (int i = 0; i < VEC; i++) stf(to + i, s[i]);
+    }
   }
 }
 
@@ -257,11 +275,12 @@ int start(const sffft_linear_attention_t* p, DeviceFacts* f) {
 
 template <class T>
 cudaError_t reduce_t(const LaReduceParams& r, int sms, cudaStream_t st) {
-  const long long total = (long long)r.B * r.G * r.L * r.D;
-  if (total == 0) return cudaSuccess;
-  long long blocks = (total + 255) / 256;
-  if (blocks > 16ll * sms) blocks = 16ll * sms;
-  return launch(la_reduce_kernel<T>, dim3((unsigned)blocks), 256, 0, st, r);
+  if (r.B == 0 || r.L == 0) return cudaSuccess;
+  const bool vec = r.D % 8 == 0;
+  const long long per = ((long long)r.L * (vec ? r.D / 8 : r.D) + 255) / 256;
+  const long long heads = (long long)r.B * r.G, most = std::max(1ll, 16ll * sms / heads);
+  const dim3 grid((unsigned)std::min(per, most), (unsigned)std::min(heads, 65535ll));
+  return vec ? launch(la_reduce_kernel<T, 8>, grid, 256, 0, st, r) : launch(la_reduce_kernel<T, 1>, grid, 256, 0, st, r);
 }
 
 }  // namespace
