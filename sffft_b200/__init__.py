@@ -19,6 +19,7 @@ from typing import Optional, Sequence
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libsffft.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "lib", "libsffft_torch.so")   # the PyTorch operators (torch_ops)
 EMU_PATH = os.path.join(_HERE, "lib", "libsffft_emu.so")
 CLI_PATH = os.path.join(_HERE, "bin", "sffft")
 

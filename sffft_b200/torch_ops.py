@@ -24,6 +24,7 @@ filter_spectrum and conv must use the same config: the spectrum is in that plan'
 `layout` ("causal", "two_sided", "circular") says which convolution the spectrum makes conv compute; the
 fused kernel is the same for all three.
 """
+import os
 import threading
 from typing import Optional
 
@@ -156,127 +157,38 @@ def _(X: Tensor, config: str = "") -> Tensor:
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# Linear attention and the norms around a block
+# Linear attention and the norms around a block: operators of csrc/torch_binding.cpp (kernels and gradients); here the
+# functions that users call, and shapes for tracing
 # ---------------------------------------------------------------------------------------------------------------
+if not os.path.exists(sf.TORCH_LIB_PATH):
+    raise RuntimeError(f"native library missing: {sf.TORCH_LIB_PATH} (run `make -C sffft_b200`)")
+sf.lib()   # which it is linked with
+torch.ops.load_library(sf.TORCH_LIB_PATH)
+_attention = torch.ops.sffft.linear_attention.default
+_attention_step = torch.ops.sffft.linear_attention_step.default
+_block_norm = torch.ops.sffft.block_norm.default
 
-@torch.library.custom_op("sffft::linear_attention", mutates_args=())
-def _linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
-                      lengths: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor]:
-    return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
 
-
-@_linear_attention.register_fake
+@torch.library.register_fake("sffft::linear_attention")
 def _(q, k, v, log_decay, initial_state, lengths, scale):
     sf.check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
     B, H, L, D = q.shape
     return sf._heads_like(q, B, H, L, v.shape[3], q.dtype), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
 
 
-@torch.library.custom_op("sffft::linear_attention_backward", mutates_args=())
-def _linear_attention_backward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
-                               lengths: Optional[Tensor], scale: float, dy: Tensor,
-                               dfinal_state: Optional[Tensor]) -> list[Tensor]:
-    out = sf.linear_attention_backward(q, k, v, log_decay, dy, dfinal_state, scale, initial_state, lengths)
-    return [t for t in out if t is not None]
-
-
-@_linear_attention_backward.register_fake
+@torch.library.register_fake("sffft::linear_attention_backward")
 def _(q, k, v, log_decay, initial_state, lengths, scale, dy, dfinal_state):
     out = [sf._heads_like(t, *t.shape, q.dtype) for t in (q, k, v)]
     return out if initial_state is None else out + [torch.empty_like(initial_state, memory_format=torch.contiguous_format)]
 
 
-def _la_setup(ctx, inputs, output):
-    q, k, v, log_decay, initial_state, lengths, scale = inputs
-    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
-    ctx.scale = scale
-
-
-def _la_backward(ctx, dy, dfinal_state):
-    q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
-    if dy is None:
-        dy = q.new_zeros((*q.shape[:3], v.shape[3]))
-    out = torch.ops.sffft.linear_attention_backward(q, k, v, log_decay, initial_state, lengths, ctx.scale, dy, dfinal_state)
-    return out[0], out[1], out[2], None, out[3] if initial_state is not None else None, None, None
-
-
-_linear_attention.register_autograd(_la_backward, setup_context=_la_setup)
-
-
-def _eager(*tensors) -> bool:
-    """Whether the tensors are plain CUDA tensors outside of any trace: the call then goes straight to the C ABI, which saves
-    the operator's dispatch (tens of microseconds, and some hundreds with a gradient)."""
-    if torch.compiler.is_compiling():
-        return False
-    return all(t is None or type(t) in (Tensor, torch.nn.Parameter) and t.is_cuda for t in tensors)
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _LinearAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale):
-        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
-        ctx.scale = scale
-        ctx.set_materialize_grads(False)
-        return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dfinal_state):
-        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
-        if dy is None:
-            dy = q.new_zeros((*q.shape[:3], v.shape[3]))
-        dq, dk, dv, ds = sf.linear_attention_backward(q, k, v, log_decay, dy, dfinal_state, ctx.scale, initial_state, lengths)
-        return dq, dk, dv, None, ds, None, None
-
-
-def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: float = 1.0,
-                     initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
-    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n with lambda = exp(log_decay) for each
-    head (see sffft_b200.linear_attention).  Differentiable in q, k, v and initial_state."""
-    if log_decay.requires_grad:
-        raise ValueError("log_decay is a constant: it has no gradient (pass log_decay.detach())")
-    if _eager(q, k, v, log_decay, initial_state, lengths):
-        if _wants_grad(q, k, v, initial_state):
-            return _LinearAttention.apply(q, k, v, log_decay, initial_state, lengths, scale)
-        return sf.linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
-    return _linear_attention(q, k, v, log_decay, initial_state, lengths, scale)
-
-
-@torch.library.custom_op("sffft::linear_attention_step", mutates_args=("state",))
-def _linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor],
-                           scale: float) -> Tensor:
-    return sf.linear_attention_step(q, k, v, log_decay, state, slots, scale)
-
-
-@_linear_attention_step.register_fake
+@torch.library.register_fake("sffft::linear_attention_step")
 def _(q, k, v, log_decay, state, slots, scale):
     return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
 
 
-def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor] = None,
-                          scale: float = 1.0) -> Tensor:
-    """One token for each row, state[slot] updated in place (see sffft_b200.linear_attention_step).  No gradient."""
-    if _wants_grad(q, k, v, log_decay, state):
-        raise ValueError("linear_attention_step updates its state in place and has no gradient: use linear_attention, or no_grad")
-    if _eager(q, k, v, log_decay, state, slots):
-        return sf.linear_attention_step(q, k, v, log_decay, state, slots, scale)
-    return _linear_attention_step(q, k, v, log_decay, state, slots, scale)
-
-
-@torch.library.custom_op("sffft::block_norm", mutates_args=())
-def _block_norm(x: Optional[Tensor], y: Optional[Tensor], gate: Optional[Tensor], post_weight: Optional[Tensor],
-                weight: Optional[Tensor], scale: float, eps: float, groups: int, act: str, dim: int) -> list[Tensor]:
-    """h (with y), n (with weight), then the rstd of y's groups (with post_weight) and of h (with weight)."""
-    h, n, r1, r2 = sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim, stats=True)
-    return [t for t in (None if y is None else h, n, r1, r2) if t is not None]
-
-
-@_block_norm.register_fake
-def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
+@torch.library.register_fake("sffft::block_norm")
+def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim, stats=False):
     C, _, _ = sf.check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     lead = y if y is not None else x
     rows = lead.numel() // C
@@ -285,86 +197,46 @@ def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
         out.append(lead.new_empty(lead.shape, dtype=lead.dtype if x is None else x.dtype))
     if weight is not None:
         out.append(lead.new_empty(lead.shape))
-    if post_weight is not None:
+    if stats and post_weight is not None:
         out.append(lead.new_empty((rows, groups), dtype=torch.float32))
-    if weight is not None:
+    if stats and weight is not None:
         out.append(lead.new_empty((rows,), dtype=torch.float32))
     return out
 
 
-@torch.library.custom_op("sffft::block_norm_backward", mutates_args=())
-def _block_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], x: Optional[Tensor], y: Optional[Tensor],
-                         gate: Optional[Tensor], post_weight: Optional[Tensor], weight: Optional[Tensor],
-                         rstd_post: Optional[Tensor], rstd: Optional[Tensor], scale: float, eps: float, groups: int, act: str,
-                         dim: int) -> list[Tensor]:
-    out = sf.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, scale, eps, groups, act, dim)
-    return [t for t in out if t is not None]
-
-
-@_block_norm_backward.register_fake
+@torch.library.register_fake("sffft::block_norm_backward")
 def _(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, scale, eps, groups, act, dim):
     return [t.new_empty(t.shape) for t in (x, y, gate, post_weight, weight) if t is not None]
 
 
-def _bn_setup(ctx, inputs, output):
-    x, y, gate, post_weight, weight, *rest = inputs
-    ctx.rest = rest
-    kept = list(output)
-    rstd = kept.pop() if weight is not None else None
-    rstd_post = kept.pop() if post_weight is not None else None
-    ctx.save_for_backward(x, y, gate, post_weight, weight, rstd_post, rstd)
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, scale: float = 1.0,
+                     initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """(y, final_state) of S_n = lambda S_{n-1} + k_n v_n^T, y_n = scale S_n^T q_n, lambda = exp(log_decay) for each head.
+
+    q [B][H][L][D], k [B][Hkv][L][D], v [B][Hkv][L][Dv], float32 or bfloat16, any strides; log_decay [H] float32, <= 0;
+    initial_state and final_state [B][H][D][Dv] float32; lengths [B] int32: tokens of each row (default L).  y has
+    q's type and order of axes, and is zero behind a row's last token.  Differentiable (once) in q, k, v and
+    initial_state; log_decay is a constant."""
+    return _attention(q, k, v, log_decay, initial_state, lengths, scale)
 
 
-def _bn_backward(ctx, grads):
-    x, y, gate, post_weight, weight, rstd_post, rstd = ctx.saved_tensors
-    grads = list(grads)
-    lead = y if y is not None else x
-    dh = grads.pop(0) if y is not None else None
-    dn = grads.pop(0) if weight is not None else None
-    if weight is not None and dn is None:
-        dn = lead.new_zeros(lead.shape)
-    if weight is None and dh is None:
-        dh = lead.new_zeros(lead.shape, dtype=lead.dtype if x is None else x.dtype)
-    out = torch.ops.sffft.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, *ctx.rest)
-    out = list(out)
-    return tuple(out.pop(0) if t is not None else None for t in (x, y, gate, post_weight, weight)) + (None,) * 5
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, slots: Optional[Tensor] = None,
+                          scale: float = 1.0) -> Tensor:
+    """One token for each row: state[slot] <- lambda state[slot] + k v^T in place, y = scale state[slot]^T q.  No gradient.
 
-
-_block_norm.register_autograd(_bn_backward, setup_context=_bn_setup)
-
-
-class _BlockNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, gate, post_weight, weight, *rest):
-        h, n, rstd_post, rstd = sf.block_norm(x, y, gate, post_weight, weight, *rest, stats=True)
-        ctx.save_for_backward(x, y, gate, post_weight, weight, rstd_post, rstd)
-        ctx.rest = rest
-        ctx.set_materialize_grads(False)
-        return None if y is None else h, n
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh, dn):
-        x, y, gate, post_weight, weight, rstd_post, rstd = ctx.saved_tensors
-        lead = y if y is not None else x
-        if weight is not None and dn is None:
-            dn = torch.zeros_like(lead)
-        if weight is None and dh is None:
-            dh = torch.zeros_like(lead, dtype=lead.dtype if x is None else x.dtype)
-        return (*sf.block_norm_backward(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, *ctx.rest), *(None,) * 5)
+    q [B][H][D], k [B][Hkv][D], v [B][Hkv][Dv]; state [pool][H][D][Dv] float32, of which only the slots' axis may have a
+    stride of its own; slots [B] int32 (default: row b uses slot b).  A slot outside the pool marks a padded row, whose
+    y is zero; so does a slot that an earlier row of the call has."""
+    return _attention_step(q, k, v, log_decay, state, slots, scale)
 
 
 def block_norm(x: Optional[Tensor] = None, y: Optional[Tensor] = None, gate: Optional[Tensor] = None,
                post_weight: Optional[Tensor] = None, weight: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6,
                groups: int = 1, act: str = "none", dim: int = -1) -> tuple[Tensor, Optional[Tensor]]:
     """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight: the norms before and after a
-    block with its gate and residual scale (see sffft_b200.block_norm).  Differentiable in all its tensors."""
-    if _eager(x, y, gate, post_weight, weight):
-        if not _wants_grad(x, y, gate, post_weight, weight):
-            return sf.block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
-        if y is None:
-            return x, _BlockNorm.apply(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)[1]
-        return _BlockNorm.apply(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
+    block with its gate and residual scale, each part only where its tensor is given (see sffft_b200.block_norm).
+    Differentiable (once) in all its tensors."""
     out = _block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
-    h = x if y is None else out[0]
-    return h, None if weight is None else out[0 if y is None else 1]
+    if y is None:
+        return x, out[0]
+    return out[0], None if weight is None else out[1]
