@@ -175,19 +175,20 @@ void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G
 }
 
 // Segments for the tensor-core kernel, one CTA on an SM.  A CTA's time is that of its chunks one after the other, so cutting
-// pays until the CTAs fill the SMs; it costs a reading of k and v (about kLocalCost of a chunk's time each) and a launch with
-// the sums of earlier states (about kCutCost chunks).
-constexpr double kCutCost = 3.0, kLocalCost = 0.5;
-
-void plan_tc(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
+// pays until the CTAs fill the SMs.  It costs two more launches, and a reading of k and v.  Measured (us a chunk, with one
+// CTA on each SM): 3.1 at head size 128 and 2.0 at 64; of a segment's own state 2.3 and 1.5; 10 for the launches.  At head
+// size 128 a chunk whose state is an output takes 5.0 (its third part of X waits for the product of the others), which
+// with G > 1 is the last segment's lot alone.
+void plan_tc(int B, int H, int L, int D, int Dv, int ntask, bool out, int sms, int* G, int* seg) {
   const long long units = (long long)B * H * ntask * la_tc_slices(D, Dv);
   const int chunks = (L + kLaTcChunk - 1) / kLaTcChunk;
+  const double one = D > 64 ? 3.1 : 2.0, local = D > 64 ? 2.3 : 1.5;
   double best = 0;
   *G = 1;
   for (int g = 1; g <= kMaxSegments && g <= chunks; g++) {
     const long long waves = (units * g + sms - 1) / sms;
     const int per = (chunks + g - 1) / g;
-    const double cost = (double)waves * per * (g > 1 ? 1.0 + kLocalCost : 1.0) + (g > 1 ? kCutCost : 0.0);
+    const double cost = (double)waves * per * (g > 1 ? one + local : D > 64 && out ? 5.0 : one) + (g > 1 ? 10.0 : 0.0);
     if (g == 1 || cost < best) best = cost, *G = g;
   }
   const int per = chunks ? (chunks + *G - 1) / *G : 1;
@@ -228,7 +229,8 @@ Sizes sizes(const sffft_linear_attention_t* p, int backward, int G) {
 
 void plan(const sffft_linear_attention_t* p, int backward, bool tc, int sms, int* G, int* seg) {
   const int D = backward ? (p->D > p->Dv ? p->D : p->Dv) : p->D, Dv = backward ? D : p->Dv;
-  (tc ? plan_tc : plan_general)(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
+  if (tc) plan_tc(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, !backward, sms, G, seg);
+  else plan_general(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
 }
 
 // Chooses the kernel and the segments, hands out the workspace, and launches.

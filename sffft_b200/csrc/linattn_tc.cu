@@ -183,6 +183,11 @@ __device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t t, const uint32_t (&
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
 // {lo, hi} halves of a word
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -200,6 +205,12 @@ __device__ __forceinline__ void wg_sync(int wg) {
     case 2: asm volatile("bar.sync 3, 128;" ::: "memory"); break;
     default: asm volatile("bar.sync 4, 128;" ::: "memory");
   }
+}
+
+// among the 128 threads of an A warpgroup
+__device__ __forceinline__ void a_sync(int a) {
+  if (a == 0) asm volatile("bar.sync 6, 128;" ::: "memory");
+  else asm volatile("bar.sync 7, 128;" ::: "memory");
 }
 
 // two floats in one instruction
@@ -578,7 +589,10 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
         mbar_arrive(bars + B_OS + a);
         if (!wwait(B_O + a, ph)) break;
         tc_fence_after();
-        const uint32_t out = stage_at(c) + (uint32_t)i * 128;   // Q has been read: its products are complete
+        // staged where Q was, whose products are complete: bf16 in the swizzled rows that the TMA store takes, or fp32, 64
+        // (split: 32) columns at a time, from where the warpgroup writes whole rows (a lane's own row would be pieces of 16
+        // bytes in 32 rows at once)
+        const uint32_t out = stage_at(c) + (uint32_t)i * 128;
 #pragma unroll 1
         for (int q = 0; q < DV / 32; q++) {
           uint32_t r[32];
@@ -601,13 +615,23 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
               const uint32_t chunk = (uint32_t)((q & 1) * 4 + e);
               sts128(out + (uint32_t)(q >> 1) * kBlk + ((chunk ^ (uint32_t)(i & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
-          } else if (blk * kTok + i < lp.L) {
-            float* y = (float*)tk.y + b * tk.ys[0] + h * tk.ys[1] + (long long)(blk * kTok + i) * tk.ys[2] + cb + q * 32;
+          } else {
+            // 128-byte rows of 32 columns; Q's tile holds one such block, or two
+            const uint32_t blk_at = stage_at(c) + (SH::q_bytes > kBlk ? (uint32_t)(q & 1) * kBlk : 0u);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)   // Dv is a multiple of 8
-              if (cb + q * 32 + e < tk.Dv)
-                *(float4*)(y + e) = make_float4(tk.scale * __uint_as_float(r[e]), tk.scale * __uint_as_float(r[e + 1]),
-                                                tk.scale * __uint_as_float(r[e + 2]), tk.scale * __uint_as_float(r[e + 3]));
+            for (int e = 0; e < 8; e++)
+              sts128(blk_at + (uint32_t)i * 128 + (((uint32_t)e ^ (uint32_t)(i & 7)) << 4), __float_as_uint(tk.scale * __uint_as_float(r[4 * e])),
+                     __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 1])), __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 2])),
+                     __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 3])));
+            a_sync(a);
+            float* y = (float*)tk.y + b * tk.ys[0] + h * tk.ys[1] + (long long)(blk * kTok) * tk.ys[2] + cb + q * 32;
+#pragma unroll 4
+            for (int x = 0; x < 8; x++) {   // 16 rows of 8 pieces at a time; Dv is a multiple of 8
+              const int row = x * 16 + (i >> 3), e = i & 7;
+              if (blk * kTok + row < lp.L && cb + q * 32 + e * 4 < tk.Dv)
+                *(float4*)(y + (long long)row * tk.ys[2] + e * 4) = lds_f4(blk_at + (uint32_t)row * 128 + ((uint32_t)(e ^ (row & 7)) << 4));
+            }
+            if (SH::q_bytes == kBlk || (q & 1)) a_sync(a);
           }
         }
         fence_async_smem();
@@ -647,9 +671,18 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
           if (col + e < tk.Dv) s[e] = in[(long long)e * tk.D];
       } else if (tk.s0) {
         const float* s0 = tk.s0 + b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + (long long)col * tk.s0s[3];
+        if (tk.s0s[3] == 1 && ((uintptr_t)s0 & 15) == 0) {   // a lane's values lie together
 #pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (col + e < tk.Dv) s[e] = s0[e * tk.s0s[3]] * tk.s0_mul;
+          for (int e = 0; e < 32; e += 4)
+            if (col + e < tk.Dv) {
+              const float4 x = *(const float4*)(s0 + e);
+              s[e] = x.x * tk.s0_mul, s[e + 1] = x.y * tk.s0_mul, s[e + 2] = x.z * tk.s0_mul, s[e + 3] = x.w * tk.s0_mul;
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (col + e < tk.Dv) s[e] = s0[e * tk.s0s[3]] * tk.s0_mul;
+        }
       }
     }
     const uint32_t srow = sm + SH::off_s + (uint32_t)(wg >> 1) * kBlk + (uint32_t)t * 128;
