@@ -54,6 +54,23 @@ __global__ void __launch_bounds__(kStepThreads) la_step_kernel(const __grid_cons
   const T* k = (const T*)prm.k + b * prm.ks[0] + (h / prm.kv_div) * prm.ks[1];
   const T* v = (const T*)prm.v + b * prm.vs[0] + (h / prm.kv_div) * prm.vs[1];
   float* S = prm.state + (ok ? slot : 0) * prm.ss + (long long)h * prm.D * prm.Dv + c;
+  float st[kStepAhead][VEC];
+  auto load = [&](int d0) {
+#pragma unroll
+    for (int a = 0; a < kStepAhead; a++) {
+      const int d = d0 + a * TY;
+      if (d >= prm.D) continue;
+      if constexpr (VEC == 4) {
+        const float4 x = __ldcs((const float4*)(S + (long long)d * prm.Dv));
+        st[a][0] = x.x, st[a][1] = x.y, st[a][2] = x.z, st[a][3] = x.w;
+      } else {
+        st[a][0] = __ldcs(S + (long long)d * prm.Dv);
+      }
+    }
+  };
+  // The first rows of the state are on their way while the slots are looked through.
+  const bool there = ok && in;
+  if (there) load(ty);
   const float lam = LaDecay(prm.ld[h]).pow(1);
   float vv[VEC], acc[VEC];
 #pragma unroll
@@ -62,21 +79,9 @@ __global__ void __launch_bounds__(kStepThreads) la_step_kernel(const __grid_cons
   int again = 0;
   if (prm.slots)
     for (int r = threadIdx.x; r < b; r += kStepThreads) again |= prm.slots[r] == slot;
-  const bool act = !__syncthreads_or(again) && ok;
-  if (act && in) {
+  if (!__syncthreads_or(again) && there) {
     for (int d0 = ty; d0 < prm.D; d0 += TY * kStepAhead) {
-      float s[kStepAhead][VEC];
-#pragma unroll
-      for (int a = 0; a < kStepAhead; a++) {
-        const int d = d0 + a * TY;
-        if (d >= prm.D) continue;
-        if constexpr (VEC == 4) {
-          const float4 x = *(const float4*)(S + (long long)d * prm.Dv);
-          s[a][0] = x.x, s[a][1] = x.y, s[a][2] = x.z, s[a][3] = x.w;
-        } else {
-          s[a][0] = S[(long long)d * prm.Dv];
-        }
-      }
+      if (d0 > ty) load(d0);
 #pragma unroll
       for (int a = 0; a < kStepAhead; a++) {
         const int d = d0 + a * TY;
@@ -84,11 +89,11 @@ __global__ void __launch_bounds__(kStepThreads) la_step_kernel(const __grid_cons
         const float kd = ldf(k + d), qd = ldf(q + d);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
-          s[a][e] = fmaf(lam, s[a][e], kd * vv[e]);
-          acc[e] = fmaf(qd, s[a][e], acc[e]);
+          st[a][e] = fmaf(lam, st[a][e], kd * vv[e]);
+          acc[e] = fmaf(qd, st[a][e], acc[e]);
         }
-        if constexpr (VEC == 4) *(float4*)(S + (long long)d * prm.Dv) = make_float4(s[a][0], s[a][1], s[a][2], s[a][3]);
-        else S[(long long)d * prm.Dv] = s[a][0];
+        if constexpr (VEC == 4) __stcs((float4*)(S + (long long)d * prm.Dv), make_float4(st[a][0], st[a][1], st[a][2], st[a][3]));
+        else __stcs(S + (long long)d * prm.Dv, st[a][0]);
       }
     }
   }
@@ -159,14 +164,14 @@ cudaError_t device_facts(int device, DeviceFacts* f) {
   return ce;
 }
 
-// Segments for the general kernel: enough blocks to give every SM two, each of at least four chunks (the first launch
-// and the sum of earlier states cost about one chunk).
+// Segments for the general kernel: enough blocks to give every SM two, each of at least two chunks (the launches for the
+// segments' own states cost about that).
 void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
   const int chunk = la_general_chunk(D);
   const long long base = (long long)B * H * ((Dv + 63) / 64) * ntask;
   const long long chunks = ((long long)L + chunk - 1) / chunk;
   long long g = (2ll * sms + base - 1) / base;
-  if (g > chunks / 4) g = chunks / 4;
+  if (g > chunks / 2) g = chunks / 2;
   if (g > kMaxSegments) g = kMaxSegments;
   if (g < 1) g = 1;
   const long long per = (chunks + g - 1) / g;

@@ -67,7 +67,7 @@ struct LaDecay {
   }
 };
 
-// fp32 on CUDA cores: any type, strides and head sizes up to 256 (launches: G > 1 two, else one).
+// fp32 on CUDA cores: any type, strides and head sizes up to 256 (G > 1: three launches, else one).
 cudaError_t launch_la_general(const LaParams& prm, bool bf16, cudaStream_t st);
 // positions in a chunk of the general kernel for head sizes up to dmax
 inline int la_general_chunk(int dmax) { return dmax > 128 ? 32 : 64; }

@@ -6,8 +6,8 @@
 // so that a token costs 2 C (D + 64) + 4 * 64 D flop instead of L (D + 64).
 //
 // Few heads and a long row leave most SMs idle, so the positions are then cut into G segments: a first launch leaves
-// the state that each segment builds from zero, and a block of the main launch starts from the sum of the earlier
-// ones (in segment order, so results do not depend on scheduling).  Its price is a second reading of k and v.
+// the state that each segment builds from zero, a second sums them up in segment order, and a block of the main launch
+// starts from the sum before it.  The price is a second reading of k and v.
 //
 // Time reversal (the gradients of k and v) is a matter of addressing: processing position p reads token n-1-p.
 #include <cuda_bf16.h>
@@ -26,6 +26,18 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float
 __device__ __forceinline__ void from_f(float& d, float x) { d = x; }
 __device__ __forceinline__ void from_f(__nv_bfloat16& d, float x) { d = __float2bfloat16_rn(x); }
 
+// N consecutive floats of shared memory, 16 (N = 2: 8) byte aligned
+template <int N>
+__device__ __forceinline__ void lds(const float* p, float (&v)[N]) {
+  if constexpr (N == 4) {
+    const float4 a = *(const float4*)p;
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  } else {
+    const float2 a = *(const float2*)p;
+    v[0] = a.x, v[1] = a.y;
+  }
+}
+
 template <int DM, int C>
 struct GeneralSmem {
   static constexpr int PT = C + 4;   // pitch of the [d][token] images: a multiple of 4, and 4-way conflicts at worst
@@ -33,7 +45,7 @@ struct GeneralSmem {
 };
 
 template <class T, int DM, int C, bool LOCAL>
-__global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_constant__ LaParams prm) {
+__global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) la_general_kernel(const __grid_constant__ LaParams prm) {
   constexpr int PT = GeneralSmem<DM, C>::PT, TI = C / 16;
   extern __shared__ __align__(16) float sm[];
   float* Qt = sm;                  // [DM][PT]
@@ -60,56 +72,62 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
   const T* v = (const T*)tk.v + b * tk.vs[0] + (h / tk.vdiv) * tk.vs[1];
   const long long ybase = b * tk.ys[0] + h * tk.ys[1];
 
-  // state before the segment
-  const float* loc = LOCAL ? nullptr : tk.loc + (long long)bh * prm.G * D * Dv;
+  // state before the segment: the start state, or what the earlier segments leave
+  const float* in = LOCAL || g == 0 ? nullptr : tk.loc + ((long long)bh * prm.G + g - 1) * D * Dv;
   for (int e = tid; e < DM * kCols; e += kThreads) {
     const int d = e / kCols, c = c0 + e % kCols;
     float s = 0.f;
     if (!LOCAL && d < D && c < Dv) {
-      for (int gg = 0; gg < g; gg++) {
-        const int m = min((gg + 1) * prm.seg, n) - min(gg * prm.seg, n);
-        if (m > 0) s = fmaf(dec.pow(m), s, loc[((long long)gg * D + d) * Dv + c]);
-      }
-      if (tk.s0) {
-        const float z = tk.s0[b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + c * tk.s0s[3]] * tk.s0_mul;
-        s = fmaf(dec.pow(ps - (tk.off && ps > 0)), z, s);
-      }
+      if (in) s = in[(long long)d * Dv + c];
+      else if (tk.s0) s = tk.s0[b * tk.s0s[0] + h * tk.s0s[1] + d * tk.s0s[2] + c * tk.s0s[3]] * tk.s0_mul;
     }
     S[e] = s;
   }
   __syncthreads();
 
+  // The next chunk's q, k and v are on their way (in registers) while a chunk is worked on: read element by element, as any
+  // stride and size allow, each would otherwise cost the memory's latency.
+  constexpr int NQ = DM * C / kThreads, NV = C * kCols / kThreads;
+  float rq[LOCAL ? 1 : NQ], rk[NQ], rv[NV];
+  auto fetch = [&](int p0) {
+    const int m = min(C, pe - p0);
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+      const int e = x * kThreads + tid, d = e % DM, i = e / DM;
+      const bool there = i < m && d < D;
+      const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
+      if (!LOCAL) rq[x] = there ? to_f(q[t * tk.qs[2] + d]) : 0.f;
+      rk[x] = there ? to_f(k[t * tk.ks[2] + d]) : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < NV; x++) {
+      const int e = x * kThreads + tid, i = e / kCols, c = c0 + e % kCols;
+      const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
+      rv[x] = i < m && c < Dv ? to_f(v[t * tk.vs[2] + c]) : 0.f;
+    }
+  };
+  if (ps < pe) fetch(ps);
   for (int p0 = ps; p0 < pe; p0 += C) {
     const int m = min(C, pe - p0);
     const int off = (tk.off && p0 == 0) ? 1 : 0;
-    for (int e = tid; e < DM * C; e += kThreads) {
-      const int d = e % DM, i = e / DM;
-      float a = 0.f, c = 0.f;
-      if (i < m && d < D) {
-        const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
-        if (!LOCAL) a = to_f(q[t * tk.qs[2] + d]);
-        c = to_f(k[t * tk.ks[2] + d]);
-      }
-      if (!LOCAL) Qt[d * PT + i] = a;
-      Kt[d * PT + i] = LOCAL ? c * pw[max(m - 1 - i, 0)] : c;
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+      const int e = x * kThreads + tid, d = e % DM, i = e / DM;
+      if (!LOCAL) Qt[d * PT + i] = rq[x];
+      Kt[d * PT + i] = LOCAL ? rk[x] * pw[max(m - 1 - i, 0)] : rk[x];
     }
-    for (int e = tid; e < C * kCols; e += kThreads) {
-      const int i = e / kCols, c = c0 + e % kCols;
-      float a = 0.f;
-      if (i < m && c < Dv) {
-        const long long t = tk.rev ? n - 1 - (p0 + i) : p0 + i;
-        a = to_f(v[t * tk.vs[2] + c]);
-      }
-      V[e] = a;
-    }
+#pragma unroll
+    for (int x = 0; x < NV; x++) V[x * kThreads + tid] = rv[x];
     __syncthreads();
+    if (p0 + C < pe) fetch(p0 + C);
     if (!LOCAL) {
       {
         float acc[TI][TI] = {};
+#pragma unroll 4
         for (int d = 0; d < D; d++) {
           float a[TI], c[TI];
-#pragma unroll
-          for (int x = 0; x < TI; x++) a[x] = Qt[d * PT + ty * TI + x], c[x] = Kt[d * PT + tx * TI + x];
+          lds<TI>(Qt + d * PT + ty * TI, a);
+          lds<TI>(Kt + d * PT + tx * TI, c);
 #pragma unroll
           for (int x = 0; x < TI; x++)
 #pragma unroll
@@ -125,23 +143,21 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
       }
       __syncthreads();
       float o[TI][4] = {}, r[TI][4] = {};
+#pragma unroll 4
       for (int j = 0; j < m; j++) {
         float a[TI], c[4];
-#pragma unroll
-        for (int x = 0; x < TI; x++) a[x] = Pt[j * PT + ty * TI + x];
-#pragma unroll
-        for (int y = 0; y < 4; y++) c[y] = V[j * kCols + tx * 4 + y];
+        lds<TI>(Pt + j * PT + ty * TI, a);
+        lds<4>(V + j * kCols + tx * 4, c);
 #pragma unroll
         for (int x = 0; x < TI; x++)
 #pragma unroll
           for (int y = 0; y < 4; y++) o[x][y] = fmaf(a[x], c[y], o[x][y]);
       }
+#pragma unroll 4
       for (int d = 0; d < D; d++) {
         float a[TI], c[4];
-#pragma unroll
-        for (int x = 0; x < TI; x++) a[x] = Qt[d * PT + ty * TI + x];
-#pragma unroll
-        for (int y = 0; y < 4; y++) c[y] = S[d * kCols + tx * 4 + y];
+        lds<TI>(Qt + d * PT + ty * TI, a);
+        lds<4>(S + d * kCols + tx * 4, c);
 #pragma unroll
         for (int x = 0; x < TI; x++)
 #pragma unroll
@@ -175,16 +191,16 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
       for (int x = 0; x < 4; x++)
 #pragma unroll
         for (int y = 0; y < 4; y++) acc[x][y] = 0.f;
-      for (int j = 0; j < m; j++) {
-        float a[4], c[4];
+      for (int j = 0; j < m; j += 4) {   // behind the last position there are zeros
+        float a[4][4], c[4][4];   // [d][j], [j][column]
 #pragma unroll
-        for (int x = 0; x < 4; x++) a[x] = Kt[(d0 + x) * PT + j];
+        for (int x = 0; x < 4; x++) lds<4>(Kt + (d0 + x) * PT + j, a[x]), lds<4>(V + (j + x) * kCols + tx * 4, c[x]);
 #pragma unroll
-        for (int y = 0; y < 4; y++) c[y] = V[j * kCols + tx * 4 + y];
+        for (int z = 0; z < 4; z++)
 #pragma unroll
-        for (int x = 0; x < 4; x++)
+          for (int x = 0; x < 4; x++)
 #pragma unroll
-          for (int y = 0; y < 4; y++) acc[x][y] = fmaf(a[x], c[y], acc[x][y]);
+            for (int y = 0; y < 4; y++) acc[x][y] = fmaf(a[x][z], c[z][y], acc[x][y]);
       }
 #pragma unroll
       for (int x = 0; x < 4; x++)
@@ -224,12 +240,45 @@ __global__ void __launch_bounds__(kThreads) la_general_kernel(const __grid_const
   }
 }
 
+// What the segments up to each one leave, the start state's part included, from what each leaves alone; in place.  A
+// thread takes one element of a state.
+__global__ void __launch_bounds__(256) la_general_prefix_kernel(const __grid_constant__ LaParams prm) {
+  const LaTask& tk = prm.task[blockIdx.z];
+  const int size = tk.D * tk.Dv, e = blockIdx.y * 256 + threadIdx.x;
+  const int bh = blockIdx.x, b = bh / prm.H, h = bh % prm.H;
+  if (e >= size) return;
+  int n = prm.L;
+  if (prm.len) n = min(max(prm.len[b], 0), prm.L);
+  const LaDecay dec(prm.ld[h]);
+  float s = 0.f;
+  if (tk.s0) s = tk.s0[b * tk.s0s[0] + h * tk.s0s[1] + (e / tk.Dv) * tk.s0s[2] + (e % tk.Dv) * tk.s0s[3]] * tk.s0_mul;
+  float* loc = tk.loc + (long long)bh * prm.G * size + e;
+  for (int g0 = 0; g0 < prm.G - 1; g0 += 8) {
+    float x[8];   // the loads do not wait for the sums
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (g0 + i < prm.G - 1) x[i] = loc[(long long)(g0 + i) * size];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int g = g0 + i;
+      if (g >= prm.G - 1) break;
+      const int a = min(g * prm.seg, n), m = min((g + 1) * prm.seg, n) - a;
+      if (m > 0) s = fmaf(dec.pow(m - (tk.off && a == 0)), s, x[i]);
+      loc[(long long)g * size] = s;
+    }
+  }
+}
+
 template <class T, int DM, int C>
 cudaError_t launch_t(const LaParams& prm, int dv_max, cudaStream_t st) {
   const dim3 grid((unsigned)(prm.B * prm.H * prm.G), (unsigned)((dv_max + kCols - 1) / kCols), (unsigned)prm.ntask);
   constexpr int bytes = GeneralSmem<DM, C>::bytes;
   if (prm.G > 1) {
-    const cudaError_t ce = launch(la_general_kernel<T, DM, C, true>, grid, kThreads, bytes, st, prm);
+    cudaError_t ce = launch(la_general_kernel<T, DM, C, true>, grid, kThreads, bytes, st, prm);
+    if (ce != cudaSuccess) return ce;
+    int size = 0;
+    for (int i = 0; i < prm.ntask; i++) size = max(size, prm.task[i].D * prm.task[i].Dv);
+    ce = launch(la_general_prefix_kernel, dim3((unsigned)(prm.B * prm.H), (unsigned)((size + 255) / 256), (unsigned)prm.ntask), 256, 0, st, prm);
     if (ce != cudaSuccess) return ce;
   }
   return launch(la_general_kernel<T, DM, C, false>, grid, kThreads, bytes, st, prm);
