@@ -91,8 +91,8 @@ enum {
   B_S = 24, B_P = 26,         // products ready; P ready [A]
   B_O1 = 28, B_OS = 30,       // Q S taken; scaled [A]
   B_O = 32, B_OFREE = 34,     // O complete; its TMEM read [A]
-  B_X = 36, B_INC,            // X ready, its product taken
-  B_X2, B_INC2,               // third part ready, its product taken
+  B_X = 36, B_INC,            // X ready (split: of even chunks), its product taken
+  B_X2, B_INC2,               // third part ready (split: X of odd chunks), its product taken
   B_ST,                       // S taken over and published; once more before the first chunk (not LOCAL)
   B_FIN, B_COUNT
 };
@@ -366,6 +366,12 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   auto sph = [](int c) { return (uint32_t)(c / NS) & 1; };         // phase of a stage's barrier
   auto aph = [](int c) { return (uint32_t)(c / (NA ? NA : 1)) & 1; };   // of an A warpgroup's
   auto grp = [](int c) { return NA ? c % NA : 0; };
+  // Split: two parts of X leave room for the next chunk's, which is then made before this one's product is taken; so X has a
+  // barrier for every other chunk.
+  const bool two_x = SH::split && !LOCAL && !three;
+  auto x_bar = [](int c) { return SH::split && !LOCAL && (c & 1) ? (int)B_X2 : (int)B_X; };
+  auto x_ph = [](int c) { return (uint32_t)(SH::split && !LOCAL ? c >> 1 : c) & 1; };
+  auto x_col = [&](int c) { return SH::c_x + (two_x ? (uint32_t)(c & 1) * 64 : 0u); };
 
   if (*stop) {
     // nothing has been started
@@ -378,14 +384,14 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       auto load_kv = [&]() {
         const int c = kv++;
         uint64_t* bar = bars + B_KV + c % NS;
-        mbar_expect(bar, SH::q_bytes + SH::v_bytes);
+        mbar_expect(bar, (SH::split && !LOCAL ? 2 : 1) * SH::q_bytes + SH::v_bytes);   // split: with Q
         for (int i = 0; i < DQ / 64; i++) tma_load(stage_at(c) + SH::off_k + i * kBlk, mp + 1, i * 64, block(c) * kTok, hk, b, bar);
         for (int i = 0; i < NB; i++) tma_load(stage_at(c) + SH::off_v + i * kBlk, mp + 2, cb + i * 64, block(c) * kTok, hv, b, bar);
       };
       auto load_q = [&]() {
         const int c = qs++;
-        uint64_t* bar = bars + B_Q + c % NS;
-        mbar_expect(bar, SH::q_bytes);
+        uint64_t* bar = bars + (SH::split ? B_KV : B_Q) + c % NS;
+        if (!SH::split) mbar_expect(bar, SH::q_bytes);
         for (int i = 0; i < DQ / 64; i++) tma_load(stage_at(c) + i * kBlk, mp + 0, i * 64, block(c) * kTok, hq, b, bar);
       };
       while (kv < min(nc, NS)) {
@@ -418,7 +424,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (*stop) {   // copies in flight end before the block does
         for (int c = max(0, kv - NS); c < kv; c++) mbar_wait_bounded(bars + B_KV + c % NS, sph(c), kWaitLimit);
-        for (int c = max(0, qs - NS); c < qs; c++) mbar_wait_bounded(bars + B_Q + c % NS, sph(c), kWaitLimit);
+        for (int c = max(0, qs - NS); !SH::split && c < qs; c++) mbar_wait_bounded(bars + B_Q + c % NS, sph(c), kWaitLimit);
       }
     }
   } else if (warp == SH::threads / 32 - 1) {
@@ -429,9 +435,10 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
     auto kstep = [](int k) { return (uint32_t)(k >> 2) * kBlk + (uint32_t)(k & 3) * 32; };   // K-major: 16 values on
     const bool later = three && !SH::whole_x;
     auto any = [](bool x) { return __any_sync(~0u, x) != 0; };   // a condition that the compiler too sees to be uniform
-    // Each waits for its operands and issues its product; false: the CTA gives up.
+    // Each waits for its operands and issues its product; false: the CTA gives up.  A wait costs a hundred cycles, so what an
+    // earlier one implies is not asked again.
     auto q_k = [&](int c) {
-      if (!wwait(B_KV + c % NS, sph(c)) || !wwait(B_Q + c % NS, sph(c))) return false;
+      if (!wwait(B_KV + c % NS, sph(c)) || (!SH::split && !wwait(B_Q + c % NS, sph(c)))) return false;
       if (SH::split && c >= NA && !wwait(B_OFREE + grp(c), aph(c - NA))) return false;   // else P V has read P
       const uint64_t qd = make_sdesc(stage_at(c), 16, 1024, LT_SW128), kd = make_sdesc(stage_at(c) + SH::off_k, 16, 1024, LT_SW128);
       tc_fence_after();
@@ -443,8 +450,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       __syncwarp();
       return true;
     };
-    auto q_s = [&](int c) {
-      if (!wwait(B_ST, c & 1)) return false;
+    auto q_s = [&](int c) {   // after x_v, which has seen S
       if (SH::split ? !wwait(B_P + grp(c), aph(c)) : c > 0 && !wwait(B_OFREE, (c - 1) & 1)) return false;
       const uint64_t qd = make_sdesc(stage_at(c), 16, 1024, LT_SW128), sd = make_sdesc(sm + SH::off_s, kBlk, 1024, LT_SW128);
       tc_fence_after();
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       return true;
     };
     auto p_v = [&](int c) {
-      if (!wwait(B_OS + grp(c), aph(c)) || !wwait(B_P + grp(c), aph(c))) return false;
+      if (!wwait(B_OS + grp(c), aph(c))) return false;   // and P, from the same threads before
       const uint64_t vd = make_sdesc(stage_at(c) + SH::off_v, kBlk, 1024, LT_SW128);
       tc_fence_after();
       const bool state = any(!fresh || c > 0);
@@ -475,24 +481,24 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       return true;
     };
     // X^T V: parts first .. last - 1 of X.  Split: 64 positions against both halves of V, 64 rows of 128 bytes apart.
-    auto increment = [&](int c, int first, int last, bool keep) {
+    auto increment = [&](int c, uint32_t x_at, int first, int last, bool keep) {
       const uint64_t vd = make_sdesc(stage_at(c) + SH::off_v, SH::split ? kBlk / 2 : kBlk, 1024, LT_SW128);
 #pragma unroll
       for (int part = first; part < last; part++)
 #pragma unroll
         for (int k = 0; k < (SH::split ? 4 : 8); k++)
-          mma_ts(tm + SH::c_inc(c), tm + SH::c_x + part * SH::part_cols + k * 8, at(vd, k * 2048), id_inc,
-                 keep || part > first || k > 0);
+          mma_ts(tm + SH::c_inc(c), tm + x_at + part * SH::part_cols + k * 8, at(vd, k * 2048), id_inc, keep || part > first || k > 0);
     };
     auto x_v = [&](int c) {
       // The increment's columns have been taken over: from the last chunk, once its state is published; LOCAL, from the last
       // but one, before X of this one came.
-      if (!wwait(B_KV + c % NS, sph(c)) || !wwait(B_X, c & 1) || (!LOCAL && !wwait(B_ST, c & 1))) return false;
-      const bool all = any(SH::whole_x && three);
+      if ((LOCAL && !wwait(B_KV + c % NS, sph(c))) || !wwait(x_bar(c), x_ph(c)) || (!LOCAL && !wwait(B_ST, c & 1))) return false;
+      const bool all = any(SH::whole_x && three), odd = any(x_col(c) != SH::c_x);
       tc_fence_after();
       if (elect_one()) {
-        if (all) increment(c, 0, 3, false);
-        else increment(c, 0, 2, false);
+        if (all) increment(c, SH::c_x, 0, 3, false);
+        else if (odd) increment(c, SH::c_x + 64, 0, 2, false);
+        else increment(c, SH::c_x, 0, 2, false);
         mma_commit(bars + B_INC);
         if (LOCAL) mma_commit(bars + B_PV + c % NS);
       }
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       if (!wwait(B_X2, c & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
-        increment(c, 0, 1, true);
+        increment(c, SH::c_x, 0, 1, true);
         mma_commit(bars + B_INC2);
       }
       __syncwarp();
@@ -740,7 +746,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
               r[2 * i + 1] &= mask;
             }
           }
-          const uint32_t to = tl + ((uint32_t)(16 * half) << 16) + SH::c_x + xcol + jj / 2;
+          const uint32_t to = tl + ((uint32_t)(16 * half) << 16) + x_col(c) + xcol + jj / 2;
           if (SH::whole_x && three) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -806,12 +812,14 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
         fence_async_smem();
       }
       make_x(c, m, false);
-      mbar_arrive(bars + B_X);
+      mbar_arrive(bars + x_bar(c));
       return true;
     };
-    // X of the next chunk goes before this one's state: it needs only the columns that this one's product has read.
+    // X of the next chunk goes before this one's state: it needs only the columns that this one's product has read, or, with
+    // columns of its own (two_x), the last one's.
     if (nc > 0 && give_x(0))
       for (int c = 0; c < nc; c++) {
+        if (two_x && c + 1 < nc && !give_x(c + 1)) break;
         if (!wwait(B_INC, c & 1)) break;
         tc_fence_after();
         if (three && !SH::whole_x) {
@@ -820,7 +828,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
           if (!wwait(B_INC2, c & 1)) break;
           tc_fence_after();
         }
-        if (c + 1 < nc && !give_x(c + 1)) break;
+        if (!two_x && c + 1 < nc && !give_x(c + 1)) break;
         if (!LOCAL && !wwait(B_O1 + grp(c), aph(c))) break;   // the product with the old S has been taken
         take(c);
         if (LOCAL) continue;
