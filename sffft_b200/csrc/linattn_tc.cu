@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
               F2 x = mul2({lo_f(r[i]), hi_f(r[i])}, {w[i & ~1], w[i | 1]});
               r[i] = upper2(x);
               x = sub2(x, cut2(x));
-              y[i] = pack_bf16(x.a, x.b);
+              y[i] = three ? upper2(x) : pack_bf16(x.a, x.b);   // cut off where a third follows
             }
             tmem_st_16x128b_x4(to, r);
             tmem_st_16x128b_x4(to + SH::part_cols, y);

@@ -96,6 +96,29 @@ def test_lengths_of_rows(state, dtype):
             assert (got[name][b, :, min(int(n[b]), L):] == 0).all()
 
 
+@pytest.mark.parametrize("D,Dv", [(64, 64), (64, 128), (128, 64), (128, 128), (96, 72)])
+@pytest.mark.parametrize("L", [2, 3, 130])
+def test_states_of_bf16_rows_are_exact_to_32_bits(L, D, Dv):
+    """Fast decay, so that a state is a sum of few terms lambda^m k v.  Each term is a product of 24 + 8 + 8 bits: lambda^m
+    and its product with k are off by 2 and 1 half steps of fp32, the three bf16 parts of that leave less than one, and of
+    the up to 3 * 16 additions (16 positions an instruction) of a row's last positions each truncates: 2^-23 of the
+    magnitude.  Terms further back than 16 positions weigh less than e^-64.  64 * 2^-23 holds them all."""
+    t = make(2, 3, 3, L, D, Dv, BF, L + D, state=False)
+    ld = torch.tensor([-4.0, -4.7, -5.3], device="cuda")
+    value, mag = ref.attention(t["q"], t["k"], t["v"], ld, 0.125)["state"]
+    _, s = sf.linear_attention(t["q"], t["k"], t["v"], ld, 0.125)
+    off = (s.double() - value).abs()
+    # a tenth of that where it is the usual: two roundings to bf16 would leave 2^-17 = 64 * 2^-23 at the most, 2^-19 usually
+    assert (off <= 64 * 2.0 ** -23 * mag).all()
+    assert torch.linalg.norm(off) <= 4 * 2.0 ** -23 * torch.linalg.norm(value)
+    ds = torch.zeros_like(s)
+    value, mag = ref.attention(t["q"], t["k"], t["v"], ld, 0.125, ds, None, t["dy"], ds)["ds0"]
+    d0 = sf.linear_attention_backward(t["q"], t["k"], t["v"], ld, t["dy"], ds, 0.125, ds)[3]
+    off = (d0.double() - value).abs()
+    assert (off <= 64 * 2.0 ** -23 * mag).all()
+    assert torch.linalg.norm(off) <= 4 * 2.0 ** -23 * torch.linalg.norm(value)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_decays_at_the_ends_of_their_range(dtype):
     check(make(1, 4, 4, 400, 64, 64, dtype, 9), decays(4, "cuda", "edges"), 0.125)
