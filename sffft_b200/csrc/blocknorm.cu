@@ -533,10 +533,10 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bw
 // read once.  Backward would have to keep five tiles; instead all three sums that a position needs are taken in one
 // reading,
 //   m = mean(t z),  A_g = sum_g s u (dh + rstd t),  B_g = sum_g s u z   (s = scale f post_weight):  sum_g s u dx = A - m B
-// and the second reading, which writes the results, finds the tile in L2: one block on each SM keeps 148 tiles at work,
-// 71 MB for 768 channels in fp32.
+// and the second reading, which writes the results, finds the tile in L2: two blocks on each SM keep 296 tiles at work,
+// 145 MB for 768 channels in fp32 and 73 in bf16, of 126 (two blocks: 72 us for [8][768][1024] in fp32; one: 91).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kPos = 32, kFirstThreads = 512, kFirstWarps = kFirstThreads / 32, kManyGroups = 32;
+constexpr int kPos = 32, kFirstThreads = 512, kFirstWarps = kFirstThreads / 32, kManyGroups = 8;
 
 template <int VEC>
 struct FirstShape {
@@ -554,7 +554,7 @@ __device__ __forceinline__ void first_sums(int groups, int gc, float* part, floa
   for (int g = many ? warp : 0; g < groups; g += many ? kFirstWarps : 1) {
     float s[N][VEC] = {};
     if (in)
-#pragma unroll 2
+#pragma unroll 4
       for (int c = first; c < gc; c += step) add(g * gc + c, s);
 #pragma unroll
     for (int k = 0; k < N; k++) {
@@ -615,10 +615,20 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
   const long long L = p.inner;
   if (p.pw) {
     float* const out[1] = {r1};
+    if constexpr (KEEP) {   // y's tile first, many loads at a time: the sums over groups would wait for each
+      if (ft.in)
+#pragma unroll 8
+        for (int c = ty; c < p.C; c += SH::TY) {
+          float v[VEC];
+          ldv<VEC>(y + c * L, v);
+          stv<VEC>(tile + c * kPos + tx * VEC, v);
+        }
+      __syncthreads();
+    }
     first_sums<VEC, 1>(p.groups, p.gc, part, out, ft.in, [&](int c, float (&s)[1][VEC]) {
       float v[VEC];
-      ldv<VEC>(y + c * L, v);
-      if (KEEP) stv<VEC>(tile + c * kPos + tx * VEC, v);
+      if constexpr (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, v);
+      else ldv<VEC>(y + c * L, v);
 #pragma unroll
       for (int e = 0; e < VEC; e++) s[0][e] = fmaf(v[e], v[e], s[0][e]);
     });
@@ -699,7 +709,7 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
 }
 
 template <class TX, class TY, int VEC>
-__global__ void __launch_bounds__(kFirstThreads) norm_first_bwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const __grid_constant__ NormParams p) {
   using SH = FirstShape<VEC>;
   extern __shared__ __align__(16) float dyn[];
   float* sA = dyn;                           // [groups][kPos]
@@ -956,9 +966,9 @@ int check(const sffft_block_norm_t* d, const void* x, const void* y, const void*
 
 int backward_blocks(const sffft_block_norm_t* d, int sms) {
   const long long units = d->inner ? (d->rows / d->inner) * ((d->inner + kPos - 1) / kPos) : d->rows;
-  // rows: as many blocks of a row's threads as an SM's registers hold at 128 each; channels first: one
+  // rows: as many blocks of a row's threads as an SM's registers hold at 128 each; channels first: two
   const int threads = (d->channels / (d->io == SFFFT_IO_BF16 ? 8 : 4) + 31) / 32 * 32;
-  const int per_sm = d->inner || threads > 256 ? 1 : threads <= 32 ? 4 : 512 / threads;
+  const int per_sm = d->inner ? 2 : threads > 256 ? 1 : threads <= 32 ? 4 : 512 / threads;
   const long long most = (long long)per_sm * sms;
   return (int)(units < most ? units : most);
 }
