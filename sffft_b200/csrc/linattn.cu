@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 #include <cmath>
 
 #include "../../include/sffft.h"
@@ -122,13 +123,15 @@ struct LaReduceParams {
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) la_reduce_kernel(const __grid_constant__ LaReduceParams p) {
   const long long plane = (long long)p.L * p.D;
-  const int pieces = p.D / VEC;
-  const unsigned total = (unsigned)p.L * (unsigned)pieces;   // below 2^31: D is at most 256 and L 2^30 / 128 or memory ends
+  const unsigned pieces = p.D / VEC;
+  // pieces of a row and head: within 32 bits where they are 8 values (2^32 of them for two heads alone would be 256 GB)
+  typedef typename std::conditional<VEC == 8, unsigned, unsigned long long>::type Index;
+  const Index total = (Index)p.L * pieces;
   for (int bg = blockIdx.y; bg < p.B * p.G; bg += gridDim.y) {
     const float* w = p.w + (long long)bg * p.R * plane;
     T* out = (T*)p.out + (bg / p.G) * p.os[0] + (bg % p.G) * p.os[1];
-    for (unsigned e = blockIdx.x * 256u + threadIdx.x; e < total; e += gridDim.x * 256u) {
-      const unsigned t = e / (unsigned)pieces, d = (e - t * (unsigned)pieces) * VEC;
+    for (Index e = blockIdx.x * 256u + threadIdx.x; e < total; e += gridDim.x * 256u) {
+      const unsigned t = (unsigned)(e / pieces), d = (unsigned)(e - (Index)t * pieces) * VEC;
       float s[VEC] = {};
       for (int r = 0; r < p.R; r++) {
         const float* x = w + r * plane + (long long)e * VEC;
@@ -429,7 +432,7 @@ int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const vo
   if (!slots && p->pool < p->B) return SFFFT_ERR_INVALID_ARGUMENT;
   if ((long long)p->B * p->H > INT_MAX || (long long)p->D * p->Dv > INT_MAX || p->Dv > 32 * 65535) return SFFFT_ERR_UNSUPPORTED;
   if (p->B == 0) return SFFFT_OK;
-  if (!q || !k || !v || !log_decay || !state || !y) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!q || !k || !v || !log_decay || (!state && p->pool > 0) || !y) return SFFFT_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)state & 3) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
   DeviceFacts f;
   const cudaError_t fe = device_facts(p->device, &f);

@@ -245,6 +245,26 @@ def test_streams_graphs_and_compile():
     assert all(torch.equal(a, b) for a, b in zip(f(t["x"], t["y"]), want))
 
 
+def test_training_step_under_compile():
+    t, dh, dn = make((2, 40, 96), -1, BF, F32, "channel")
+    names = ("x", "y", "gate", "post_weight", "weight")
+
+    def loss(*a):
+        h, n = ops.block_norm(*a, scale=0.5, groups=4, act="silu")
+        return (h * dh).sum() + (n * dn).sum(dtype=torch.float32)
+
+    grads = []
+    for f in (loss, torch.compile(loss, fullgraph=True)):
+        leaves = [t[n].clone().requires_grad_() for n in names]
+        f(*leaves).backward()
+        grads.append([x.grad for x in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    x, w = (t[n].clone().requires_grad_() for n in ("x", "weight"))
+    g, = torch.autograd.grad(ops.block_norm(x, weight=w)[1].sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):     # no second derivative
+        g.sum().backward()
+
+
 def test_layouts_agree():
     """[B][C][L] and [B][L][C] give the same numbers, up to the order of the sums over channels."""
     t, dh, dn = make((2, 64, 48), 1, F32, F32)

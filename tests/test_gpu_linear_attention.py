@@ -292,6 +292,47 @@ def test_streams_graphs_and_compile():
     del back
 
 
+def test_training_step_under_compile():
+    t = make(2, 4, 2, 300, 64, 64, BF, 15, True)
+    ld = decays(4, "cuda")
+    names = ("q", "k", "v", "s0")
+
+    def loss(q, k, v, s0):
+        y, s = ops.linear_attention(q, k, v, ld, 0.125, s0)
+        return (y * t["dy"]).sum(dtype=torch.float32) + (s * t["ds"]).sum()
+
+    grads = []
+    for f in (loss, torch.compile(loss, fullgraph=True)):
+        leaves = [t[n].clone().requires_grad_() for n in names]
+        f(*leaves).backward()
+        grads.append([x.grad for x in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_training_step_in_a_graph():
+    """Forward and backward captured, with gradients in buffers of their own, and replayed on new values."""
+    t = make(2, 4, 2, 300, 64, 64, BF, 16, True)
+    ld = decays(4, "cuda")
+    leaves = [t[n].clone().requires_grad_() for n in ("q", "k", "v")]
+
+    def step():
+        y, _ = ops.linear_attention(*leaves, ld, 0.125)
+        return torch.autograd.grad(y, leaves, t["dy"])
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    g.replay()
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_threads_of_their_own():
     """Calls from threads that have made no CUDA call yet (autograd's are such), while others call too."""
     import threading
@@ -387,6 +428,24 @@ def test_step_with_padded_rows_and_a_slot_named_twice():
     want = ops.linear_attention_step(q[[0, 2]], k[[0, 2]], v[[0, 2]], ld, alone, slots[[0, 2]])
     assert torch.equal(y[[0, 2]], want) and torch.equal(state, alone)
     assert torch.equal(state[[1, 3]], before[[1, 3]])
+
+
+def test_step_without_a_pool():
+    q = torch.ones((2, 3, 16), device="cuda")
+    y = ops.linear_attention_step(q, q, q, decays(3, "cuda"), torch.empty((0, 3, 16, 16), device="cuda"),
+                                  torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert (y == 0).all()
+
+
+def test_step_marks_its_state_as_changed():
+    q = torch.ones((1, 1, 16), device="cuda")
+    s = torch.zeros((1, 1, 16, 16), device="cuda")
+    x = torch.ones((1, 1, 16, 16), device="cuda", requires_grad=True)
+    z = (x * s).sum()
+    with torch.no_grad():
+        ops.linear_attention_step(q, q, q, decays(1, "cuda"), s)
+    with pytest.raises(RuntimeError):     # s was needed as it was
+        z.backward()
 
 
 def test_step_continues_a_prompt():
