@@ -230,7 +230,8 @@ int sffft_multi_pipe_destroy(sffft_multi_t multi);
  *   initial_state, final_state [B][H][D][Dv] fp32 contiguous; NULL: zero, not wanted.
  *
  * D up to 256 and Dv up to 4096 (backward: 256), any L; other sizes return SFFFT_ERR_UNSUPPORTED.  A value of q, k or v
- * that is not finite may reach all outputs of its row and head.  Outputs must not overlap inputs.  `work`: caller-owned
+ * that is not finite may reach all outputs of its row and head.  Outputs must not overlap inputs (final_state ==
+ * initial_state is refused).  `work`: caller-owned
  * device memory of sffft_linear_attention_workspace_bytes (256-byte aligned), not shared by calls that can overlap.
  * Calls run on `device` in stream order and can be captured in graphs; the caller's current device is left as it was.
  * Results do not depend on scheduling: no atomics. */
@@ -238,7 +239,7 @@ typedef struct {
   int B, H, Hkv, L, D, Dv;
   int io;                 /* SFFFT_IO_* of q, k, v, y and their gradients */
   int device;
-  float scale;            /* finite, not 0 */
+  float scale;            /* finite, not 0 (backward: 1 / scale finite) */
   long long q_stride[3], k_stride[3], v_stride[3], y_stride[3];
 } sffft_linear_attention_t;
 int sffft_linear_attention_workspace_bytes(const sffft_linear_attention_t* p, int backward, size_t* bytes);

@@ -946,6 +946,8 @@ cudaError_t norm_any(const NormParams& p, int res_io, int io, bool bwd, cudaStre
   return norm_t<__nv_bfloat16, __nv_bfloat16>(p, bwd, st);
 }
 
+size_t io_size(int io) { return io == SFFFT_IO_BF16 ? 2 : 4; }
+
 int check(const sffft_block_norm_t* d, const void* x, const void* y, const void* gate, const void* pw, const void* w) {
   auto io_ok = [](int v) { return v == SFFFT_IO_FP32 || v == SFFFT_IO_BF16; };
   if (!d || d->rows < 0 || d->channels < 1 || d->inner < 0 || d->groups < 1 || d->channels % d->groups != 0 ||
@@ -961,6 +963,8 @@ int check(const sffft_block_norm_t* d, const void* x, const void* y, const void*
   if (!x && d->res_io != d->io) return SFFFT_ERR_UNSUPPORTED;
   if (d->channels > kMaxChannels || d->rows > INT_MAX) return SFFFT_ERR_UNSUPPORTED;
   if (d->inner && d->groups > 256) return SFFFT_ERR_UNSUPPORTED;
+  if (!on_elements(io_size(d->io), {y, gate}) || !on_elements(io_size(d->res_io), {x}) || !on_elements(io_size(d->weight_io), {pw, w}))
+    return SFFFT_ERR_INVALID_ARGUMENT;
   return SFFFT_OK;
 }
 
@@ -1007,6 +1011,8 @@ int sffft_block_norm(const sffft_block_norm_t* d, const void* x, const void* y, 
   int rc = check(d, x, y, gate, post_weight, weight);
   if (rc) return rc;
   if ((y && !h) || (weight && !n)) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!on_elements(io_size(d->res_io), {h}) || !on_elements(io_size(d->io), {n}) || !on_elements(4, {rstd_post, rstd}))
+    return SFFFT_ERR_INVALID_ARGUMENT;
   if (d->rows == 0) return SFFFT_OK;
   int sms;
   if ((rc = facts(d->device, &sms))) return rc;
@@ -1041,6 +1047,9 @@ int sffft_block_norm_backward(const sffft_block_norm_t* d, const void* x, const 
       (weight && (!dweight || !rstd || !dn)) || (!weight && !dh))
     return SFFFT_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!on_elements(io_size(d->res_io), {dh, dx}) || !on_elements(io_size(d->io), {dn, dy, dgate}) ||
+      !on_elements(io_size(d->weight_io), {dpost_weight, dweight}) || !on_elements(4, {rstd_post, rstd}))
+    return SFFFT_ERR_INVALID_ARGUMENT;
   int sms;
   if ((rc = facts(d->device, &sms))) return rc;
   NormParams p = params(d, x, y, gate, post_weight, weight);

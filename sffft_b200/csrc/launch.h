@@ -2,8 +2,18 @@
 // that a call runs on.
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <initializer_list>
 
 namespace sffft {
+
+// Whether tensors of `size`-byte elements lie on whole elements: a kernel's access to any other address is a fault.
+inline bool on_elements(size_t size, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % size != 0) return false;
+  return true;
+}
 
 template <class K, class P>
 cudaError_t launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& prm) {

@@ -204,6 +204,8 @@ void plan_tc(int B, int H, int L, int D, int Dv, int ntask, bool out, int sms, i
   *G = chunks ? (chunks + per - 1) / per : 1;
 }
 
+size_t io_size(int io) { return io == SFFFT_IO_BF16 ? 2 : 4; }
+
 struct Sizes {
   size_t loc[kLaMaxTasks], grad_k, grad_v, total;
 };
@@ -246,6 +248,11 @@ int run(const sffft_linear_attention_t* p, int backward, LaParams* prm, const De
         cudaStream_t st) {
   const bool bf = p->io == SFFFT_IO_BF16, tc = bf && la_tc_takes(*prm);
   plan(p, backward, tc, f.sms, &prm->G, &prm->seg);
+  if (tc) {
+    long long slices = 0;
+    for (int i = 0; i < prm->ntask; i++) slices += la_tc_slices(prm->task[i].D, prm->task[i].Dv);
+    if ((long long)p->B * p->H * prm->G * slices * prm->ntask > INT_MAX) return SFFFT_ERR_UNSUPPORTED;   // CTAs of a launch
+  }
   const Sizes sz = sizes(p, backward, prm->G);
   const size_t need = sz.total - sz.grad_k - sz.grad_v;
   if (need && (!work || work_bytes < need)) return SFFFT_ERR_WORKSPACE;
@@ -325,6 +332,9 @@ int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, con
   if (p->B == 0) return SFFFT_OK;
   if (p->L > 0 && (!q || !k || !v || !y)) return SFFFT_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!on_elements(io_size(p->io), {q, k, v, y}) || !on_elements(4, {log_decay, lengths, initial_state, final_state}))
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  if (initial_state && initial_state == final_state) return SFFFT_ERR_INVALID_ARGUMENT;   // segments start from it all along
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
@@ -349,11 +359,15 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
                                     void* work, size_t work_bytes, void* stream) {
   int rc = common_checks(p, log_decay);
   if (rc) return rc;
-  if (!g) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!g || !std::isfinite(1.f / p->scale)) return SFFFT_ERR_INVALID_ARGUMENT;
   if (p->Dv > 256) return SFFFT_ERR_UNSUPPORTED;   // v takes the place of q in two of the three passes
   if (p->B == 0) return SFFFT_OK;
   if (p->L > 0 && (!q || !k || !v || !dy || !dq || !dk || !dv)) return SFFFT_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)work & 255) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!on_elements(io_size(p->io), {q, k, v, dy, dq, dk, dv}) ||
+      !on_elements(4, {log_decay, lengths, initial_state, dfinal_state, dinitial_state}))
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  if (dinitial_state && dinitial_state == dfinal_state) return SFFFT_ERR_INVALID_ARGUMENT;   // as forward
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
@@ -433,7 +447,7 @@ int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const vo
   if ((long long)p->B * p->H > INT_MAX || (long long)p->D * p->Dv > INT_MAX || p->Dv > 32 * 65535) return SFFFT_ERR_UNSUPPORTED;
   if (p->B == 0) return SFFFT_OK;
   if (!q || !k || !v || !log_decay || (!state && p->pool > 0) || !y) return SFFFT_ERR_INVALID_ARGUMENT;
-  if (((uintptr_t)state & 3) != 0) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (!on_elements(io_size(p->io), {q, k, v, y}) || !on_elements(4, {log_decay, state, slots})) return SFFFT_ERR_INVALID_ARGUMENT;
   DeviceFacts f;
   const cudaError_t fe = device_facts(p->device, &f);
   if (fe != cudaSuccess) return sffft_note_cuda_error(fe);

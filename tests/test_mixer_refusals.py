@@ -183,6 +183,41 @@ def test_c_abi_statuses():
     assert lib.sffft_block_norm_workspace_bytes(bn(), None) == sf.ERR_INVALID_ARGUMENT
 
 
+def test_c_abi_refuses_addresses_between_elements():
+    lib = sf.lib()
+    la = ctypes.byref(sf.LinearAttentionDesc(1, 2, 2, 4, 8, 8, sf.IO["bf16"], 0, 1.0))
+    g = ctypes.byref(sf.LinearAttentionGrads())
+    step = ctypes.byref(sf.LinearAttentionStepDesc(2, 2, 2, 8, 8, 2, sf.IO["bf16"], 0, 1.0))
+    bn = ctypes.byref(sf.BlockNormDesc(4, 8, 0, 1, sf.IO["bf16"], sf.IO["fp32"], sf.IO["fp32"], 0, 0, 1.0, 1e-6, 0))
+
+    def refused(f, *args, odd):   # each of the addresses in turn
+        for i in odd:
+            a = list(args)
+            a[i] += 1 if a[i] else 257
+            assert f(*a) == sf.ERR_INVALID_ARGUMENT, (f.__name__, i)
+
+    refused(lib.sffft_linear_attention, la, 16, 16, 16, 16, 16, 16, 16, 32, 0, 0, None, odd=[*range(1, 9), 9])
+    refused(lib.sffft_linear_attention_backward, la, g, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 32, 0, 0, None, odd=range(2, 14))
+    refused(lib.sffft_linear_attention_step, step, 16, 16, 16, 16, 16, 16, 16, None, odd=range(1, 8))
+    refused(lib.sffft_block_norm, bn, 16, 16, None, 16, 16, 16, 16, 16, 16, None, odd=[1, 2, 4, 5, 6, 7, 8, 9])
+    refused(lib.sffft_block_norm_backward, bn, 16, 16, None, 16, 16, 16, 16, 16, 16, 16, 16, None, 16, 16, 256, 0, None,
+            odd=[1, 2, 4, 5, 6, 7, 8, 9, 10, 11, 13, 14, 15])
+
+
+def test_c_abi_refuses_a_state_in_its_own_place():
+    lib = sf.lib()
+    la = ctypes.byref(sf.LinearAttentionDesc(1, 2, 2, 4, 8, 8, 0, 0, 1.0))
+    g = ctypes.byref(sf.LinearAttentionGrads())
+    assert lib.sffft_linear_attention(la, 16, 16, 16, 16, None, 32, 16, 32, None, 0, None) == sf.ERR_INVALID_ARGUMENT
+    assert lib.sffft_linear_attention_backward(la, g, 16, 16, 16, 16, None, 16, 16, 32, 16, 16, 16, 32, None, 0, None) == sf.ERR_INVALID_ARGUMENT
+
+
+def test_backward_refuses_a_scale_without_a_reciprocal():
+    la = ctypes.byref(sf.LinearAttentionDesc(1, 2, 2, 4, 8, 8, 0, 0, 1e-40))
+    assert sf.lib().sffft_linear_attention_backward(la, ctypes.byref(sf.LinearAttentionGrads()), 16, 16, 16, 16, None, 16, 16, None, 16,
+                                                    16, 16, None, None, 0, None) == sf.ERR_INVALID_ARGUMENT
+
+
 def test_shapes_without_a_gpu():
     m = lambda *s, dtype=torch.bfloat16: torch.empty(s, device="meta", dtype=dtype)  # noqa: E731
     y, s = ops.linear_attention(m(B, H, L, D), m(B, HKV, L, D), m(B, HKV, L, DV), m(H, dtype=torch.float32))
