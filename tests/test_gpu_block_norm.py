@@ -1,5 +1,6 @@
 """The joint between two blocks (norm, gate, residual scale, residual stream, norm) on the device: values and gradients
 against the formulas in 64 bits for each of its parts, both layouts, odd sizes, strides, streams and graphs."""
+import ctypes
 import itertools
 
 import pytest
@@ -263,6 +264,26 @@ def test_training_step_under_compile():
     g, = torch.autograd.grad(ops.block_norm(x, weight=w)[1].sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):     # no second derivative
         g.sum().backward()
+
+
+@pytest.mark.parametrize("C,groups,dtype", [(96, 4, F32), (768, 12, BF), (1030, 1, BF), (8192, 2, F32)])
+def test_results_in_the_place_of_x_and_y(C, groups, dtype):
+    t, _, _ = make((9, C), -1, dtype, F32)
+    kw = dict(scale=0.5, eps=1e-5, groups=groups, act="silu")
+    h, n = sf.block_norm(**t, **kw)
+    p = lambda x: x.data_ptr()  # noqa: E731
+    x, y, gate, pw, w = t.values()
+    desc = sf.BlockNormDesc(9, C, 0, groups, sf.IO["bf16" if dtype == BF else "fp32"], 0, 0, sf.GATE["full"], sf.ACT["silu"], 0.5, 1e-5,
+                            x.device.index, C, C, C)
+    assert sf.lib().sffft_block_norm(ctypes.byref(desc), p(x), p(y), p(gate), p(pw), p(w), p(x), p(y), None, None,
+                                     torch.cuda.current_stream().cuda_stream) == sf.OK
+    assert torch.equal(x, h) and torch.equal(y, n)
+
+
+@pytest.mark.parametrize("C,groups", [(96, 96), (800, 200), (8191, 8191)])
+def test_groups_of_a_few_channels(C, groups):
+    t, dh, dn = make((5, C), -1, F32, F32, seed=groups)
+    check(t, dh, dn, groups)
 
 
 def test_layouts_agree():
