@@ -44,7 +44,9 @@ struct NormParams {
   long long rows, xs, ys, gs; // rows layout: row strides
   int C, groups, gc, inner;   // gc channels in a group; inner: L of [B][C][L]
   int gate_kind, act, w_bf16;
+  unsigned gmul;              // 2^31 / gc, rounded up: group_of
   int blocks;                 // backward: blocks of the grid
+  int sums_shared;            // channels first, backward: sums over rows in shared memory
   float scale, eps;
 };
 
@@ -162,6 +164,9 @@ struct RawV {
         const uint4 a = ((const uint4*)p)[i];
         w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
       }
+    } else if constexpr (bytes == 8) {
+      const uint2 a = *(const uint2*)p;
+      w[0] = a.x, w[1] = a.y;
     } else if constexpr (bytes == 4) {
       w[0] = *(const uint32_t*)p;
     } else {
@@ -534,7 +539,13 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bw
 // reading,
 //   m = mean(t z),  A_g = sum_g s u (dh + rstd t),  B_g = sum_g s u z   (s = scale f post_weight):  sum_g s u dx = A - m B
 // and the second reading, which writes the results, finds the tile in L2: two blocks on each SM keep 296 tiles at work,
-// 145 MB for 768 channels in fp32 and 73 in bf16, of 126 (two blocks: 72 us for [8][768][1024] in fp32; one: 91).
+// 145 MB for 768 channels in fp32 and 73 in bf16, of 126 (two blocks: 76 us for [8][768][1024] in fp32; one: 85).
+//
+// What bounds both is the latency of a thread's loads: 1024 threads on an SM with 64 registers (forward: 40 to 64, and 98 KB
+// of tile for 768 channels) hold no more of them in flight.  Measured, of the bytes that must move: [8][768][1024] fp32, one
+// group: 33 us forward (3.8 TB/s), 76 backward (2.6); [8][768][4096] bf16, 12 groups: 87 and 211 us (2.9, 1.9 TB/s).
+// Forward's loads are taken two (fp32) or four channels at a time, which was 125 -> 87 us of the latter; backward has no
+// registers for a second channel (212 -> 259 us where it was made to).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kPos = 32, kFirstThreads = 512, kFirstWarps = kFirstThreads / 32, kManyGroups = 8;
 
@@ -543,19 +554,40 @@ struct FirstShape {
   static constexpr int TX = kPos / VEC, TR = 32 / TX, TY = kFirstWarps * TR;   // lanes across, channels in a warp, in the block
 };
 
-// Sums of N quantities over each group: `add(c, s)` adds channel c's to the thread's s[N][VEC].  out[k]: [groups][kPos].
-// part: [min(groups, kManyGroups - 1)][kFirstWarps][kPos] floats for each quantity.  Ends with the block in step.
-template <int VEC, int N, class F>
-__device__ __forceinline__ void first_sums(int groups, int gc, float* part, float* const (&out)[N], bool in, F add) {
+// c / gc: c gmul / 2^31 is above it by less than c / 2^31, which is less than 1 / gc (both are at most kMaxChannels).
+__device__ __forceinline__ int group_of(const NormParams& p, int c) { return (int)__umulhi(2u * (unsigned)c, p.gmul); }
+
+// Channels c, c + step, .. below `end`, the loads of U of them before the first one's use: results that are stored in between
+// may be anyone's memory to the compiler, which therefore does not move a load ahead of them itself.
+template <int U, class R, class L, class F>
+__device__ __forceinline__ void channels(int c, int end, int step, L load, F use) {
+  for (; c + (U - 1) * step < end; c += U * step) {
+    R r[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) load(c + i * step, r[i]);
+#pragma unroll
+    for (int i = 0; i < U; i++) use(c + i * step, r[i]);
+  }
+  if constexpr (U > 1)
+    for (; c < end; c += step) {
+      R r;
+      load(c, r);
+      use(c, r);
+    }
+}
+
+// Sums of N quantities over each group: `add(c, r, s)` adds channel c's, loaded by load(c, r), to the thread's s[N][VEC].
+// out[k]: [groups][kPos].  part: [min(groups, kManyGroups - 1)][kFirstWarps][kPos] floats for each quantity.  Ends with the
+// block in step.
+template <int VEC, int N, int U, class R, class L, class F>
+__device__ __forceinline__ void first_sums(int groups, int gc, float* part, float* const (&out)[N], bool in, L load, F add) {
   using SH = FirstShape<VEC>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = lane % SH::TX, tr = lane / SH::TX;
   const bool many = groups >= kManyGroups;
   const int first = many ? tr : warp * SH::TR + tr, step = many ? SH::TR : SH::TY;
   for (int g = many ? warp : 0; g < groups; g += many ? kFirstWarps : 1) {
     float s[N][VEC] = {};
-    if (in)
-#pragma unroll 4
-      for (int c = first; c < gc; c += step) add(g * gc + c, s);
+    if (in) channels<U, R>(g * gc + first, (g + 1) * gc, step, load, [&](int c, const R& r) { add(c, r, s); });
 #pragma unroll
     for (int k = 0; k < N; k++) {
 #pragma unroll
@@ -613,6 +645,7 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
   const TY *y = (const TY*)p.y + ft.base, *gate = (const TY*)p.gate;
   const TX* x = (const TX*)p.x + ft.base;
   const long long L = p.inner;
+  constexpr int kAhead = sizeof(TX) + sizeof(TY) <= 6 ? 4 : 2;   // with fp32 alone, [8][768][1024]: 33 us; 4: 37
   if (p.pw) {
     float* const out[1] = {r1};
     if constexpr (KEEP) {   // y's tile first, many loads at a time: the sums over groups would wait for each
@@ -625,13 +658,18 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
         }
       __syncthreads();
     }
-    first_sums<VEC, 1>(p.groups, p.gc, part, out, ft.in, [&](int c, float (&s)[1][VEC]) {
-      float v[VEC];
-      if constexpr (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, v);
-      else ldv<VEC>(y + c * L, v);
+    first_sums<VEC, 1, 4, RawV<TY, VEC>>(
+        p.groups, p.gc, part, out, ft.in,
+        [&](int c, RawV<TY, VEC>& r) {
+          if constexpr (!KEEP) r.load(y + c * L);
+        },
+        [&](int c, const RawV<TY, VEC>& r, float (&s)[1][VEC]) {
+          float v[VEC];
+          if constexpr (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, v);
+          else r.get(v);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) s[0][e] = fmaf(v[e], v[e], s[0][e]);
-    });
+          for (int e = 0; e < VEC; e++) s[0][e] = fmaf(v[e], v[e], s[0][e]);
+        });
     for (int i = threadIdx.x; i < p.groups * kPos; i += kFirstThreads) r1[i] = rsqrtf(r1[i] / (float)p.gc + p.eps);
     __syncthreads();
     if (p.r1 && ft.in)
@@ -639,52 +677,59 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
 #pragma unroll
         for (int e = 0; e < VEC; e++) p.r1[(ft.row + e) * p.groups + g] = r1[g * kPos + tx * VEC + e];
   }
-  auto value = [&](int c, float (&h)[VEC]) {
-#pragma unroll
-    for (int e = 0; e < VEC; e++) h[e] = 0.f;
+  struct Raw {
+    RawV<TY, VEC> y, g;
+    RawV<TX, VEC> x;
+    float pw, gc;
+  };
+  auto load = [&](int c, Raw& r) {
+    r.y.zero(), r.g.zero(), r.x.zero();
+    float t[1] = {1.f};
+    if (p.y && !(KEEP && p.pw)) r.y.load(y + c * L);
+    if (p.gate_kind == GATE_FULL) r.g.load(gate + ft.base + c * L);
+    if (p.x) r.x.load(x + c * L);
+    if (p.pw) ldw<1>(p.pw, p.w_bf16, c, t);
+    r.pw = t[0];
+    r.gc = p.gate_kind == GATE_CHANNEL ? ldf(gate + c) : 0.f;
+  };
+  auto value = [&](int c, const Raw& r, float (&h)[VEC]) {
+    float xv[VEC];
+    r.x.get(xv);
+    r.y.get(h);
     if (p.y) {
       if (KEEP && p.pw) ldv<VEC>(tile + c * kPos + tx * VEC, h);
-      else ldv<VEC>(y + c * L, h);
       if (p.pw) {
-        float w[1];
-        ldw<1>(p.pw, p.w_bf16, c, w);
-        const float* r = r1 + (p.groups > 1 ? c / p.gc : 0) * kPos + tx * VEC;
+        const float* rs = r1 + group_of(p, c) * kPos + tx * VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) h[e] *= r[e] * w[0];
+        for (int e = 0; e < VEC; e++) h[e] *= rs[e] * r.pw;
       }
       if (p.gate_kind) {
         float gv[VEC], f[VEC];
-        if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
+        if (p.gate_kind == GATE_FULL) r.g.get(gv);
         else
 #pragma unroll
-          for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
+          for (int e = 0; e < VEC; e++) gv[e] = r.gc;
         act_fwd<VEC>(p.act, gv, f);
 #pragma unroll
         for (int e = 0; e < VEC; e++) h[e] *= f[e];
       }
-#pragma unroll
-      for (int e = 0; e < VEC; e++) h[e] *= p.scale;
     }
-    if (p.x) {
-      float xv[VEC];
-      ldv<VEC>(x + c * L, xv);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) h[e] += xv[e];
-    }
+    for (int e = 0; e < VEC; e++) h[e] = p.x ? fmaf(p.scale, h[e], xv[e]) : p.scale * h[e];
   };
   if (!p.w) {
     if (ft.in)
-      for (int c = ty; c < p.C; c += SH::TY) {
+      channels<kAhead, Raw>(ty, p.C, SH::TY, load, [&](int c, const Raw& r) {
         float h[VEC];
-        value(c, h);
+        value(c, r, h);
         stv<VEC>((TX*)p.h + ft.base + c * L, h);
-      }
+      });
     return;
   }
   float* const out[1] = {r2};
-  first_sums<VEC, 1>(1, p.C, part, out, ft.in, [&](int c, float (&s)[1][VEC]) {
+  first_sums<VEC, 1, kAhead, Raw>(1, p.C, part, out, ft.in, load, [&](int c, const Raw& r, float (&s)[1][VEC]) {
     float h[VEC];
-    value(c, h);
+    value(c, r, h);
     if (p.h) stv<VEC>((TX*)p.h + ft.base + c * L, h);
     if (KEEP) stv<VEC>(tile + c * kPos + tx * VEC, h);
 #pragma unroll
@@ -697,15 +742,26 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
     rs[e] = rsqrtf(r2[tx * VEC + e] / (float)p.C + p.eps);
     if (p.r2 && ty == 0) p.r2[ft.row + e] = rs[e];
   }
-  for (int c = ty; c < p.C; c += SH::TY) {
-    float h[VEC], w[1];
-    if (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, h);
-    else value(c, h);
-    ldw<1>(p.w, p.w_bf16, c, w);
+  struct Last {
+    Raw r;
+    float w;
+  };
+  channels<kAhead, Last>(
+      ty, p.C, SH::TY,
+      [&](int c, Last& l) {
+        if constexpr (!KEEP) load(c, l.r);
+        float w[1];
+        ldw<1>(p.w, p.w_bf16, c, w);
+        l.w = w[0];
+      },
+      [&](int c, const Last& l) {
+        float h[VEC];
+        if constexpr (KEEP) ldv<VEC>(tile + c * kPos + tx * VEC, h);
+        else value(c, l.r, h);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) h[e] *= rs[e] * w[0];
-    stv<VEC>((TY*)p.n + ft.base + c * L, h);
-  }
+        for (int e = 0; e < VEC; e++) h[e] *= rs[e] * l.w;
+        stv<VEC>((TY*)p.n + ft.base + c * L, h);
+      });
 }
 
 template <class TX, class TY, int VEC>
@@ -715,72 +771,91 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
   float* sA = dyn;                           // [groups][kPos]
   float* sB = sA + p.groups * kPos;
   float* sM = sB + p.groups * kPos;          // [groups][kPos], then [kPos]
-  float* part = sM + p.groups * kPos;
+  float* sQ = sM + p.groups * kPos;          // [groups][kPos]: rstd of y's groups
+  float* part = sQ + p.groups * kPos;
   const int tx = threadIdx.x % SH::TX, ty = threadIdx.x / SH::TX;
-  float* out = p.part + (long long)blockIdx.x * 3 * p.C;   // this block's sums; a channel always belongs to one ty
+  // this block's sums; a channel always belongs to one ty
+  float* out = p.part + (long long)blockIdx.x * 3 * p.C;
+  float* acc = p.sums_shared ? part + first_part_floats(p.groups, 3) : out;
   const long long L = p.inner;
-  const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
+  const int per = (p.inner + kPos - 1) / kPos;
+  const long long tiles = (p.rows / p.inner) * per;
   const TY* gate = (const TY*)p.gate;
   bool first = true;
   for (long long tile = blockIdx.x; tile < tiles; tile += p.blocks, first = false) {
     const FirstTile ft = first_tile<VEC>(p, tile);
+    if (p.pw) {
+      const long long row0 = tile / per * p.inner + tile % per * kPos;
+      const int there = min(kPos, p.inner - (int)(tile % per) * kPos) * p.groups;
+      for (int i = threadIdx.x; i < kPos * p.groups; i += kFirstThreads)
+        sQ[i % p.groups * kPos + i / p.groups] = i < there ? p.r1[row0 * p.groups + i] : 0.f;
+      __syncthreads();
+    }
     float r2[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) r2[e] = p.w && ft.in ? p.r2[ft.row + e] : 0.f;
-    struct Values {
-      float u[VEC], f[VEC], df[VEC], z[VEC], d[VEC], tn[VEC], q[VEC];   // d: dh + rstd t;  q: rstd of y's group
-      float pw, w;
+    struct Raw {
+      RawV<TY, VEC> y, g, dn;
+      RawV<TX, VEC> x, dh;
+      float pw, w, gc;
     };
-    auto load = [&](int c, Values& v, bool with_df) {
-      float gv[VEC], xv[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; e++) v.u[e] = v.d[e] = v.tn[e] = xv[e] = 0.f, v.f[e] = v.q[e] = 1.f, v.df[e] = 0.f;
-      v.pw = 1.f;
-      v.w = 0.f;
-      float t[1];
-      if (p.y) ldv<VEC>((const TY*)p.y + ft.base + c * L, v.u);
-      if (p.gate_kind == GATE_FULL) ldv<VEC>(gate + ft.base + c * L, gv);
-      else if (p.gate_kind == GATE_CHANNEL)
-#pragma unroll
-        for (int e = 0; e < VEC; e++) gv[e] = ldf(gate + c);
-      if (p.dh) ldv<VEC>((const TX*)p.dh + ft.base + c * L, v.d);
+    auto load = [&](int c, Raw& r) {
+      const long long at = ft.base + c * L;
+      r.y.zero(), r.g.zero(), r.dn.zero(), r.x.zero(), r.dh.zero();
+      float t[1] = {1.f}, w[1] = {0.f};
+      if (p.y) r.y.load((const TY*)p.y + at);
+      if (p.gate_kind == GATE_FULL) r.g.load(gate + at);
+      if (p.dh) r.dh.load((const TX*)p.dh + at);
       if (p.w) {
-        if (p.x) ldv<VEC>((const TX*)p.x + ft.base + c * L, xv);
-        ldv<VEC>((const TY*)p.dn + ft.base + c * L, v.tn);
-        ldw<1>(p.w, p.w_bf16, c, t);
-        v.w = t[0];
+        if (p.x) r.x.load((const TX*)p.x + at);
+        r.dn.load((const TY*)p.dn + at);
+        ldw<1>(p.w, p.w_bf16, c, w);
       }
-      if (p.pw) {
-        ldw<1>(p.pw, p.w_bf16, c, t);
-        v.pw = t[0];
-        const float* r = p.r1 + ft.row * p.groups + (p.groups > 1 ? c / p.gc : 0);
+      if (p.pw) ldw<1>(p.pw, p.w_bf16, c, t);
+      r.pw = t[0];
+      r.w = w[0];
+      r.gc = p.gate_kind == GATE_CHANNEL ? ldf(gate + c) : 0.f;
+    };
+    struct Values {
+      float u[VEC], f[VEC], df[VEC], z[VEC], d[VEC], tn[VEC];   // d: dh + rstd t
+    };
+    auto values = [&](const float* q, const Raw& r, Values& v, bool with_df) {   // q: rstd of y's group
+      float xv[VEC];
+      r.y.get(v.u);
+      r.dh.get(v.d);
+      r.dn.get(v.tn);
+      r.x.get(xv);
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          v.q[e] = r[e * p.groups];
-          v.u[e] *= v.q[e];
-        }
-      }
+      for (int e = 0; e < VEC; e++) v.f[e] = 1.f, v.df[e] = 0.f;
+      if (p.pw)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v.u[e] *= q[e];
       if (p.gate_kind) {
+        float gv[VEC];
+        if (p.gate_kind == GATE_FULL) r.g.get(gv);
+        else
+#pragma unroll
+          for (int e = 0; e < VEC; e++) gv[e] = r.gc;
         if (with_df) act_both<VEC>(p.act, gv, v.f, v.df);
         else act_fwd<VEC>(p.act, gv, v.f);
       }
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
-        v.z[e] = (p.y ? fmaf(p.scale * v.f[e], v.u[e] * v.pw, xv[e]) : xv[e]) * r2[e];
-        v.d[e] = fmaf(r2[e], v.tn[e] * v.w, v.d[e]);
+        v.z[e] = (p.y ? fmaf(p.scale * v.f[e], v.u[e] * r.pw, xv[e]) : xv[e]) * r2[e];
+        v.d[e] = fmaf(r2[e], v.tn[e] * r.w, v.d[e]);
       }
     };
     if (p.w || p.pw) {
       float* const sums[3] = {sA, sB, sM};
-      first_sums<VEC, 3>(p.groups, p.gc, part, sums, ft.in, [&](int c, float (&s)[3][VEC]) {
+      first_sums<VEC, 3, 1, Raw>(p.groups, p.gc, part, sums, ft.in, load, [&](int c, const Raw& r, float (&s)[3][VEC]) {
         Values v;
-        load(c, v, false);
+        values(sQ + group_of(p, c) * kPos + tx * VEC, r, v, false);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
-          const float su = p.scale * v.f[e] * v.pw * v.u[e];
+          const float su = p.scale * v.f[e] * r.pw * v.u[e];
           s[0][e] = fmaf(su, v.d[e], s[0][e]);
           s[1][e] = fmaf(su, v.z[e], s[1][e]);
-          s[2][e] = fmaf(v.tn[e] * v.w, v.z[e], s[2][e]);
+          s[2][e] = fmaf(v.tn[e] * r.w, v.z[e], s[2][e]);
         }
       });
       if (p.groups > 1) {
@@ -795,48 +870,60 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
     float m2[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) m2[e] = p.w ? sM[tx * VEC + e] * r2[e] / (float)p.C : 0.f;
-    for (int c = ty; c < p.C; c += SH::TY) {
-      float sw = 0.f, sp = 0.f, sg = 0.f;
-      if (ft.in) {
-        Values v;
-        load(c, v, true);
-        float dg[VEC];
+    const float inv_g = 1.f / (float)p.gc;
+    // Positions beyond L take part with zeros: the TX lanes of a channel are neighbours and add up.
+    channels<1, Raw>(
+        ty, p.C, SH::TY,
+        [&](int c, Raw& r) {
+          if (ft.in) load(c, r);
+        },
+        [&](int c, const Raw& r) {
+          float sw = 0.f, sp = 0.f, sg = 0.f;
+          if (ft.in) {
+            const int g = group_of(p, c) * kPos + tx * VEC;
+            Values v;
+            values(sQ + g, r, v, true);
+            float dg[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          sw = fmaf(v.tn[e], v.z[e], sw);
-          v.d[e] = fmaf(-m2[e], v.z[e], v.d[e]);
-        }
-        if (p.dx) stv<VEC>((TX*)p.dx + ft.base + c * L, v.d);
-        if (p.y) {
-          const int g = (p.groups > 1 ? c / p.gc : 0) * kPos + tx * VEC;
+            for (int e = 0; e < VEC; e++) {
+              sw = fmaf(v.tn[e], v.z[e], sw);
+              v.d[e] = fmaf(-m2[e], v.z[e], v.d[e]);
+            }
+            if (p.dx) stv<VEC>((TX*)p.dx + ft.base + c * L, v.d);
+            if (p.y) {
 #pragma unroll
-          for (int e = 0; e < VEC; e++) {
-            dg[e] = p.scale * v.d[e] * v.u[e] * v.pw * v.df[e];
-            sg += dg[e];
-            const float da = p.scale * v.f[e] * v.d[e];
-            sp = fmaf(da, v.u[e], sp);
-            v.d[e] = p.pw ? v.q[e] * fmaf(-fmaf(-m2[e], sB[g + e], sA[g + e]) / (float)p.gc, v.u[e], da * v.pw) : da;
+              for (int e = 0; e < VEC; e++) {
+                dg[e] = p.scale * v.d[e] * v.u[e] * r.pw * v.df[e];
+                sg += dg[e];
+                const float da = p.scale * v.f[e] * v.d[e];
+                sp = fmaf(da, v.u[e], sp);
+                v.d[e] = p.pw ? sQ[g + e] * fmaf(-fmaf(-m2[e], sB[g + e], sA[g + e]) * inv_g, v.u[e], da * r.pw) : da;
+              }
+              if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + ft.base + c * L, dg);
+              stv<VEC>((TY*)p.dy + ft.base + c * L, v.d);
+            }
           }
-          if (p.gate_kind == GATE_FULL) stv<VEC>((TY*)p.dgate + ft.base + c * L, dg);
-          stv<VEC>((TY*)p.dy + ft.base + c * L, v.d);
-        }
-      }
-      // the TX lanes of a channel are neighbours; lanes of a warp whose channel is beyond C have left together
-      const unsigned mask = SH::TX == 32 ? ~0u : ((1u << SH::TX) - 1) << ((threadIdx.x & 31) / SH::TX * SH::TX);
+          // lanes of a warp whose channel is beyond C have left together
+          const unsigned mask = SH::TX == 32 ? ~0u : ((1u << SH::TX) - 1) << ((threadIdx.x & 31) / SH::TX * SH::TX);
 #pragma unroll
-      for (int o = SH::TX / 2; o; o >>= 1) {
-        sw += __shfl_xor_sync(mask, sw, o);
-        sp += __shfl_xor_sync(mask, sp, o);
-        sg += __shfl_xor_sync(mask, sg, o);
-      }
-      if (tx == 0) {
-        if (p.w) out[c] = (first ? 0.f : out[c]) + sw;
-        if (p.pw) out[p.C + c] = (first ? 0.f : out[p.C + c]) + sp;
-        if (p.gate_kind == GATE_CHANNEL) out[2 * p.C + c] = (first ? 0.f : out[2 * p.C + c]) + sg;
-      }
-    }
+          for (int o = SH::TX / 2; o; o >>= 1) {
+            sw += __shfl_xor_sync(mask, sw, o);
+            sp += __shfl_xor_sync(mask, sp, o);
+            sg += __shfl_xor_sync(mask, sg, o);
+          }
+          if (tx == 0) {
+            if (p.w) acc[c] = (first ? 0.f : acc[c]) + sw;
+            if (p.pw) acc[p.C + c] = (first ? 0.f : acc[p.C + c]) + sp;
+            if (p.gate_kind == GATE_CHANNEL) acc[2 * p.C + c] = (first ? 0.f : acc[2 * p.C + c]) + sg;
+          }
+        });
     __syncthreads();
   }
+  if (p.sums_shared)
+    for (int i = threadIdx.x; i < 3 * p.C; i += kFirstThreads) {
+      const int k = i / p.C;
+      if (k == 0 ? p.w != nullptr : k == 1 ? p.pw != nullptr : p.gate_kind == GATE_CHANNEL) out[i] = acc[i];
+    }
 }
 
 // Sums the blocks' parts: a block takes 32 channels, 32 threads down the parts, added in a fixed order.
@@ -912,8 +999,10 @@ template <class TX, class TY, int VEC>
 cudaError_t first_v(const NormParams& p, bool bwd, cudaStream_t st) {
   const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
   if (bwd) {
-    const int smem = 4 * (3 * p.groups * kPos + first_part_floats(p.groups, 3));
-    return launch(norm_first_bwd_kernel<TX, TY, VEC>, dim3((unsigned)p.blocks), kFirstThreads, smem, st, p);
+    const int smem = 4 * (4 * p.groups * kPos + first_part_floats(p.groups, 3)), with = smem + 4 * 3 * p.C;
+    NormParams q = p;
+    q.sums_shared = with <= kMaxShared / 2;   // two blocks on an SM
+    return launch(norm_first_bwd_kernel<TX, TY, VEC>, dim3((unsigned)p.blocks), kFirstThreads, q.sums_shared ? with : smem, st, q);
   }
   const int smem = 4 * ((p.groups + 1) * kPos + first_part_floats(p.groups, 1)), kept = smem + 4 * p.C * kPos;
   if (kept <= kMaxShared)
@@ -994,6 +1083,7 @@ NormParams params(const sffft_block_norm_t* d, const void* x, const void* y, con
   if (!x) p.xs = 0;
   if (!y) p.ys = 0;
   p.C = d->channels; p.groups = d->groups; p.gc = d->channels / d->groups; p.inner = d->inner;
+  p.gmul = ((1u << 31) + p.gc - 1) / p.gc;
   p.gate_kind = d->gate; p.act = d->act; p.w_bf16 = d->weight_io == SFFFT_IO_BF16;
   p.scale = d->scale; p.eps = d->eps;
   return p;
