@@ -280,7 +280,7 @@ int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const vo
  * The joint between two blocks (no reference counterpart): the norm behind a block, its gate and residual scale, the
  * residual stream, and the norm before the next block, in one pass.  On each row of `channels` values
  *
- *   a = y * rstd_g(y) * post_weight     (a = y where post_weight is NULL; rstd over each of `groups` runs of channels)
+ *   a = y * rstd_g(y) * post_weight     (a = y where post_weight is NULL, whatever groups; rstd over each of `groups` runs of channels)
  *   h = x + scale * act(gate) * a       (without x where it is NULL; without the gate where gate is NULL)
  *   n = h * rstd(h) * weight            (not computed where weight is NULL)
  *

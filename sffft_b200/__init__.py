@@ -768,8 +768,6 @@ def check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, d
         raise ValueError("the weights must have one type")
     if groups < 1 or C % groups:
         raise ValueError(f"{C} channels do not fall into {groups} groups")
-    if groups > 1 and post_weight is None:
-        raise ValueError("groups are those of the norm with post_weight")
     if act not in ACT:
         raise ValueError(f"act must be one of {sorted(ACT)}")
     if not math.isfinite(scale):
@@ -834,7 +832,8 @@ def _norm_desc(x, y, gate, post_weight, weight, scale, eps, groups, act, dim):
 def block_norm(x=None, y=None, gate=None, post_weight=None, weight=None, scale=1.0, eps=1e-6, groups=1, act="none", dim=-1,
                stats=False):
     """(h, n) with a = y rstd_g(y) post_weight, h = x + scale act(gate) a, n = h rstd(h) weight, each part only where its
-    tensor is given; rstd(z) = (mean z^2 + eps)^-1/2 over the channels (over each of `groups` runs of them for y).
+    tensor is given; rstd(z) = (mean z^2 + eps)^-1/2 over the channels (over each of `groups` runs of them for y,
+    which says nothing without post_weight).
 
     The channels are the last axis, or axis 1 of [B][C][L] tensors (`dim=1`, the layout of the convolution).  gate: shaped
     like y, or [C]; act: "none", "silu" or "sigmoid".  y, gate and n have one type (float32 or bfloat16); x and h have it

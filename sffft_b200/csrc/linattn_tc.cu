@@ -25,6 +25,13 @@
 //
 // A segment's own contribution to the state (LOCAL) needs X^T V alone.
 //
+// Measured (bytes: q, k, v and y once).  8 x 12 heads x 4096 x 64: 74 us, 2.7 TB/s on 96 of 148
+// SMs, 3800 cycles a chunk: bound by the chain from one chunk's state to the next's, X (1100), its product (1170), taking it
+// over (470) and the wake-up between them (490), with the issuing warp's own 500 a step.  2 x 8 heads x 16384 x 128 in
+// segments: 110 us in three launches, 2.4 TB/s (3.7 with the second reading of k and v), 5800 cycles a chunk.  The tensor
+// pipe is busy for 31 to 35 %.  Tried and slower: four state warpgroups at head size 64 (85 us), the third part of X kept in
+// registers at 128 (spills, 167 -> 194 us), the next launch's prologue overlapped with the last one's end (no gain).
+//
 // Every wait is bounded: after kWaitLimit ns the waiting role raises the CTA's flag, all roles leave, and the device's
 // status word says so.
 #include <cuda.h>

@@ -262,7 +262,6 @@ NormCall norm_call(const optional<Tensor>& x, const optional<Tensor>& y, const o
     }
   need(!pw || !w || pw->scalar_type() == w->scalar_type(), "the weights must have one type");
   need(groups >= 1 && C % groups == 0, C, " channels do not fall into ", groups, " groups");
-  need(groups == 1 || pw, "groups are those of the norm with post_weight");
   const int a = act == "none" ? SFFFT_ACT_NONE : act == "silu" ? SFFFT_ACT_SILU : act == "sigmoid" ? SFFFT_ACT_SIGMOID : -1;
   need(a >= 0, "act must be none, silu or sigmoid");
   need(std::isfinite(scale), "scale must be finite");

@@ -286,6 +286,17 @@ def test_groups_of_a_few_channels(C, groups):
     check(t, dh, dn, groups)
 
 
+def test_groups_without_the_norm_of_y():
+    for shape, dim in (((3, 5, 96), -1), ((2, 96, 36), 1)):
+        t, dh, dn = make(shape, dim, BF, F32, post=False)
+        kw = dict(scale=0.5, act="silu", dim=dim)
+        for f in (sf.block_norm, ops.block_norm):
+            assert all(torch.equal(a, b) for a, b in zip(f(**t, **kw, groups=8), f(**t, **kw)))
+        r2 = sf.block_norm(**t, **kw, stats=True)[3]
+        a, b = (sf.block_norm_backward(dh, dn, **t, rstd=r2, **kw, groups=g) for g in (8, 1))
+        assert all(x is y or torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_layouts_agree():
     """[B][C][L] and [B][L][C] give the same numbers, up to the order of the sums over channels."""
     t, dh, dn = make((2, 64, 48), 1, F32, F32)

@@ -100,7 +100,6 @@ BAD_BN = {
     "weights of two types": dict(weight=torch.zeros(32, dtype=torch.bfloat16)),
     "groups that do not divide": dict(groups=5),
     "no groups": dict(groups=0),
-    "groups without a norm": dict(groups=4, post_weight=None),
     "another activation": dict(act="gelu"),
     "a gate without y": dict(y=None, post_weight=None),
     "only x": dict(y=None, gate=None, post_weight=None, weight=None),
@@ -173,7 +172,6 @@ def test_c_abi_statuses():
     assert call(bn(), y=None) == sf.ERR_INVALID_ARGUMENT           # a weight for y without y
     assert call(bn(), y=None, pw=None, w=None) == sf.ERR_INVALID_ARGUMENT
     assert call(bn(), h=None) == sf.ERR_INVALID_ARGUMENT and call(bn(), n=None) == sf.ERR_INVALID_ARGUMENT
-    assert call(bn(groups=2), pw=None) == sf.ERR_INVALID_ARGUMENT
     assert call(bn(res_io=1)) == sf.ERR_UNSUPPORTED and call(bn(channels=8193)) == sf.ERR_UNSUPPORTED
     assert call(bn(rows=0)) == sf.OK
     back = lambda d, r1=16, r2=16, dh=16, dn=16, dx=16, work=256: lib.sffft_block_norm_backward(  # noqa: E731
