@@ -60,7 +60,25 @@ struct __align__(64) LaTcParams {
   LaParams p;
   int blocks;   // chunks in a segment
   int slices;   // CTAs over the columns of v
+  int by_length;   // CTAs take the rows from the longest to the shortest
 };
+
+// The row that the CTAs numbered b take.  Where they come to between one and two for each SM, a long row that starts last
+// leaves the other SMs idle behind it: 8 rows of 600 to 1999 tokens x 12 heads of 64 x 128 took 58 to 70 us in their own
+// order and 57 to 65 longest first.  With more CTAs, or a row cut into segments, the order of lengths won nothing (16 x 6 x
+// 1999 x 128: 233 and 245 us).  Called by whole warps, each for itself: a lane ranks one row, ties by number.
+constexpr int kMaxSorted = 32;
+__device__ __forceinline__ int row_of(const LaTcParams& prm, int b) {
+  if (!prm.by_length) return b;
+  const int i = threadIdx.x & 31, mine = i < prm.p.B ? min(max(prm.p.len[i], 0), prm.p.L) : -1;
+  int rank = 0;
+#pragma unroll
+  for (int j = 0; j < kMaxSorted; j++) {
+    const int other = __shfl_sync(~0u, mine, j);
+    rank += other > mine || (other == mine && j < i);
+  }
+  return __ffs(__ballot_sync(~0u, rank == b)) - 1;   // ranks are a permutation of the lanes, the rows' first
+}
 
 template <int DQ, int DV, bool LOCAL>
 struct Shape {
@@ -322,7 +340,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   u /= lp.ntask;
   const LaTask& tk = lp.task[ti];
   const int cb = vi * DV;
-  const int g = u % lp.G, bh = u / lp.G, b = bh / lp.H, h = bh % lp.H;
+  const int g = u % lp.G, h = u / lp.G % lp.H, b = row_of(prm, u / lp.G / lp.H), bh = b * lp.H + h;
   if (cb >= tk.Dv || (LOCAL && g == lp.G - 1)) return;   // nothing follows the last segment
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n = lp.L;
@@ -961,8 +979,10 @@ bool make_map(CUtensorMap* m, const void* p, const long long (&s)[3], int B, int
 int tile_v(int D, int Dv) { return D > 64 && Dv > 64 ? 128 : 64; }
 
 template <int DQ, int DV>
-cudaError_t launch_shape(const LaTcParams& prm, cudaStream_t st) {
+cudaError_t launch_shape(LaTcParams& prm, cudaStream_t st) {
   const dim3 grid((unsigned)(prm.p.B * prm.p.H * prm.p.G * prm.p.ntask * prm.slices));
+  prm.by_length = prm.p.len && prm.p.B <= kMaxSorted && prm.p.G == 1 && grid.x > (unsigned)prm.p.sms &&
+                  grid.x <= 2u * (unsigned)prm.p.sms;
   if (prm.p.G > 1) {
     using SH = Shape<DQ, DV, true>;
     cudaError_t ce = launch(la_tc_kernel<DQ, DV, true>, grid, SH::threads, (int)SH::smem, st, prm);

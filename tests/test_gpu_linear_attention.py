@@ -96,6 +96,17 @@ def test_lengths_of_rows(state, dtype):
             assert (got[name][b, :, min(int(n[b]), L):] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,H", [(2, 90), (9, 20), (31, 6), (32, 8), (33, 6), (32, 20)])
+def test_many_rows_of_many_lengths(B, H, dtype):
+    """More blocks than run at once, which may take the longest rows first; some of one length."""
+    L = 140
+    t = make(B, H, 2, L, 64, 64, dtype, B, True)
+    n = torch.randint(0, L + 1, (B,), device="cuda", dtype=torch.int32, generator=torch.Generator("cuda").manual_seed(B))
+    n[1::4] = 77
+    check(t, decays(H, "cuda"), 0.3, n)
+
+
 @pytest.mark.parametrize("D,Dv", [(64, 64), (64, 128), (128, 64), (128, 128), (96, 72)])
 @pytest.mark.parametrize("L", [2, 3, 130])
 def test_states_of_bf16_rows_are_exact_to_32_bits(L, D, Dv):
