@@ -548,7 +548,9 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bw
 // of tile for 768 channels) hold no more of them in flight.  Measured, of the bytes that must move: [8][768][1024] fp32, one
 // group: 33 us forward (3.8 TB/s), 76 backward (2.6); [8][768][4096] bf16, 12 groups: 87 and 211 us (2.9, 1.9 TB/s).
 // Forward's loads are taken two (fp32) or four channels at a time, which was 125 -> 87 us of the latter; backward has no
-// registers for a second channel (212 -> 259 us where it was made to).
+// registers for a second channel (212 -> 259 us where it was made to) but where threads hold single values.  They do where L
+// is no multiple of 4, and their instructions then bound both: [3][768][2187] fp32: 32 and 101 us (3.1, 1.6 TB/s);
+// [8][768][4095] bf16, 12 groups: 151 and 536 (1.7, 0.75 TB/s; 691 one channel at a time).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kPos = 32, kFirstThreads = 512, kFirstWarps = kFirstThreads / 32, kManyGroups = 8;
 
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
   const TY *y = (const TY*)p.y + ft.base, *gate = (const TY*)p.gate;
   const TX* x = (const TX*)p.x + ft.base;
   const long long L = p.inner;
-  constexpr int kAhead = sizeof(TX) + sizeof(TY) <= 6 ? 4 : 2;   // with fp32 alone, [8][768][1024]: 33 us; 4: 37
+  constexpr int kAhead = VEC == 1 || sizeof(TX) + sizeof(TY) <= 6 ? 4 : 2;   // with fp32 alone, [8][768][1024]: 33 us; 4: 37
   if (p.pw) {
     float* const out[1] = {r1};
     if constexpr (KEEP) {   // y's tile first, many loads at a time: the sums over groups would wait for each
@@ -771,6 +773,7 @@ template <class TX, class TY, int VEC>
 __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const __grid_constant__ NormParams p) {
   using SH = FirstShape<VEC>;
   extern __shared__ __align__(16) float dyn[];
+  constexpr int kAhead = VEC == 1 ? 2 : 1;   // what 64 registers hold
   float* sA = dyn;                           // [groups][kPos]
   float* sB = sA + p.groups * kPos;
   float* sM = sB + p.groups * kPos;          // [groups][kPos], then [kPos]
@@ -850,7 +853,7 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
     };
     if (p.w || p.pw) {
       float* const sums[3] = {sA, sB, sM};
-      first_sums<VEC, 3, 1, Raw>(p.groups, p.gc, part, sums, ft.in, load, [&](int c, const Raw& r, float (&s)[3][VEC]) {
+      first_sums<VEC, 3, kAhead, Raw>(p.groups, p.gc, part, sums, ft.in, load, [&](int c, const Raw& r, float (&s)[3][VEC]) {
         Values v;
         values(sQ + group_of(p, c) * kPos + tx * VEC, r, v, false);
 #pragma unroll
@@ -875,7 +878,7 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
     for (int e = 0; e < VEC; e++) m2[e] = p.w ? sM[tx * VEC + e] * r2[e] / (float)p.C : 0.f;
     const float inv_g = 1.f / (float)p.gc;
     // Positions beyond L take part with zeros: the TX lanes of a channel are neighbours and add up.
-    channels<1, Raw>(
+    channels<kAhead, Raw>(
         ty, p.C, SH::TY,
         [&](int c, Raw& r) {
           if (ft.in) load(c, r);
