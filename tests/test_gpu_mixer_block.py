@@ -1,8 +1,11 @@
 """The operators together, as the layers of a model use them: norm, linear attention or the convolution, norm by heads with
 gate, residual stream, norm; prompts, single tokens and training."""
+import ctypes
+
 import pytest
 import torch
 
+import sffft_b200 as sf
 import sffft_b200.torch_ops as ops
 from tests import mixer_ref as ref
 
@@ -105,3 +108,62 @@ def test_the_convolution_between_its_norms():
     a = want["h"] - x.double()
     assert torch.linalg.norm(h.double() - want["h"]) <= 2 * 5.1e-4 * torch.linalg.norm(a) + 1e-6 * torch.linalg.norm(want["h"])
     assert torch.linalg.norm(n2.double() - want["n"]) <= 4 * 5.1e-4 * torch.linalg.norm(want["n"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_calls_without_their_workspace_are_refused(dtype):
+    """In C, where the workspace is the caller's: the call does nothing, and with what was asked for it gives Python's results."""
+    lib, io = sf.lib(), sf.IO["bf16" if dtype == BF else "fp32"]
+    st = torch.cuda.current_stream().cuda_stream
+    Hq, Hk, Lq = 2, 1, 2048
+    q, k, v = (torch.randn((1, n, Lq, D), device="cuda").to(dtype) for n in (Hq, Hk, Hk))
+    ld = torch.tensor([-0.01, -0.1], device="cuda")
+    y, s = torch.full_like(q, 7), torch.full((1, Hq, D, D), 7.0, device="cuda")
+    three = ctypes.c_longlong * 3
+    sq, sk = three(Hq * Lq * D, Lq * D, D), three(Hk * Lq * D, Lq * D, D)
+    desc = sf.LinearAttentionDesc(1, Hq, Hk, Lq, D, D, io, q.device.index, 0.125, sq, sk, sk, sq)
+    need = ctypes.c_size_t()
+    p = lambda t: t.data_ptr()  # noqa: E731
+
+    def forward(work, n):
+        return lib.sffft_linear_attention(ctypes.byref(desc), p(q), p(k), p(v), p(ld), None, None, p(y), p(s), work, n, st)
+
+    assert forward(None, 0) == sf.ERR_WORKSPACE
+    assert (y == 7).all() and (s == 7).all()
+    assert lib.sffft_linear_attention_workspace_bytes(ctypes.byref(desc), 0, ctypes.byref(need)) == sf.OK and need.value > 0
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    assert forward(p(work), 256) == sf.ERR_WORKSPACE and (y == 7).all()
+    assert forward(p(work), need.value) == sf.OK
+    assert all(torch.equal(a, b) for a, b in zip((y, s), sf.linear_attention(q, k, v, ld, 0.125)))
+
+    dy = torch.randn_like(q)
+    dq, dk, dv = (torch.full_like(t, 7) for t in (q, k, v))
+    grads = sf.LinearAttentionGrads(sq, sq, sk, sk)
+
+    def backward(work, n):
+        return lib.sffft_linear_attention_backward(ctypes.byref(desc), ctypes.byref(grads), p(q), p(k), p(v), p(ld), None, None, p(dy),
+                                                   None, p(dq), p(dk), p(dv), None, work, n, st)
+
+    assert backward(None, 0) == sf.ERR_WORKSPACE
+    assert lib.sffft_linear_attention_workspace_bytes(ctypes.byref(desc), 1, ctypes.byref(need)) == sf.OK
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    assert backward(p(work), 1 << 20) == sf.ERR_WORKSPACE
+    assert all((t == 7).all() for t in (dq, dk, dv))
+    assert backward(p(work), need.value) == sf.OK
+    assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), sf.linear_attention_backward(q, k, v, ld, dy, None, 0.125)))
+
+    x, w = torch.randn((50, 64), device="cuda").to(dtype), torch.ones(64, device="cuda")
+    _, _, _, r = sf.block_norm(x, weight=w, stats=True)
+    dn, dx, dw = torch.randn_like(x), torch.full_like(x, 7), torch.full_like(w, 7)
+    bn = sf.BlockNormDesc(50, 64, 0, 1, io, io, 0, 0, 0, 1.0, 1e-6, x.device.index, 64, 0, 0)
+
+    def norm_backward(work, n):
+        return lib.sffft_block_norm_backward(ctypes.byref(bn), p(x), None, None, None, p(w), None, p(r), None, p(dn), p(dx), None, None,
+                                             None, p(dw), work, n, st)
+
+    assert norm_backward(None, 0) == sf.ERR_WORKSPACE and (dx == 7).all() and (dw == 7).all()
+    assert lib.sffft_block_norm_workspace_bytes(ctypes.byref(bn), ctypes.byref(need)) == sf.OK
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    assert norm_backward(p(work), need.value) == sf.OK
+    got = sf.block_norm_backward(None, dn, x, weight=w, rstd=r)
+    assert torch.equal(dx, got[0]) and torch.equal(dw, got[4])
