@@ -297,6 +297,18 @@ def test_groups_without_the_norm_of_y():
         assert all(x is y or torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^31 values apart."""
+    C, far = 96, (1 << 31) + 32
+    buf = torch.empty(far + 3 * C, dtype=BF, device="cuda")
+    t, dh, dn = make((2, C), -1, BF, BF)
+    for i, name in enumerate(("x", "y", "gate")):
+        view = torch.as_strided(buf, (2, C), (far, 1), i * C)
+        view.copy_(t[name])
+        t[name] = view
+    check(t, dh, dn, 4)
+
+
 def test_layouts_agree():
     """[B][C][L] and [B][L][C] give the same numbers, up to the order of the sums over channels."""
     t, dh, dn = make((2, 64, 48), 1, F32, F32)
