@@ -108,6 +108,8 @@ struct Shape {
 // next phase needs something that the waiting role does after it has seen this one.  The thread that loads is ahead of
 // nothing, so what it waits for has a barrier for each stage, whose next phase needs that thread's own next load.
 // Those of the stages complete once for each NS chunks, those of an A warpgroup once for each NA, the others once a chunk.
+// tests/test_mixer_protocol.py restates the roles and checks these rules, and that accesses to TMEM and to the tiles are
+// ordered, for every shape: who changes a role changes it there too.
 enum {
   B_KV = 0, B_Q = 6,          // K and V, Q loaded [stage]
   B_REL = 10,                 // K and V read by the state warpgroups and X^T V [stage]
@@ -464,7 +466,8 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
     // earlier one implies is not asked again.
     auto q_k = [&](int c) {
       if (!wwait(B_KV + c % NS, sph(c)) || (!SH::split && !wwait(B_Q + c % NS, sph(c)))) return false;
-      if (SH::split && c >= NA && !wwait(B_OFREE + grp(c), aph(c - NA))) return false;   // else P V has read P
+      // P of an earlier chunk lies where the product goes, and products with different accumulators are not kept in order.
+      if (SH::split ? c >= NA && !wwait(B_OFREE + grp(c), aph(c - NA)) : c > 0 && !wwait(B_O, (c - 1) & 1)) return false;
       const uint64_t qd = make_sdesc(stage_at(c), 16, 1024, LT_SW128), kd = make_sdesc(stage_at(c) + SH::off_k, 16, 1024, LT_SW128);
       tc_fence_after();
       if (elect_one()) {
