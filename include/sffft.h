@@ -333,6 +333,14 @@ int sffft_debug_wait_timeout(int limit_us);
 int sffft_debug_conv_timeout(sffft_plan_t plan, const void* u, const void* Kf, void* y, int B, int H, int limit_us,
                              void* stream);
 
+/* Debug: from here on, linear attention on the tensor cores that this host thread launches limits each barrier wait to
+ * limit_us microseconds (1..1e6; 0: the default, 2 s), and with `withhold` one thread leaves out an arrival: 1: that the last
+ * chunk's keys are ready for the state's product, 2: that the outputs are scaled, 3: that they are staged.  The
+ * waits that need it run out, every role sees the flag, lets its copies and products in flight end, frees TMEM and
+ * returns; sffft_linear_attention_check then reports SFFFT_ERR_TIMEOUT and the context stays usable.  (0, 0) puts the
+ * defaults back. */
+int sffft_debug_linear_attention(int limit_us, int withhold);
+
 #ifdef __cplusplus
 }
 #endif

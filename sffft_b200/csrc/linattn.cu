@@ -156,6 +156,10 @@ __global__ void __launch_bounds__(256) la_reduce_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSegments = 32;
 
+// sffft_debug_linear_attention's, for the calls of its thread
+thread_local unsigned long long t_wait_ns = kLaWaitNs;
+thread_local int t_withhold = LA_WITHHOLD_NONE;
+
 struct DeviceFacts {
   int sms = 0, ok = 0;
 };
@@ -249,6 +253,8 @@ void plan(const sffft_linear_attention_t* p, int backward, bool tc, int sms, int
 int run(const sffft_linear_attention_t* p, int backward, LaParams* prm, const DeviceFacts& f, char* work, size_t work_bytes,
         cudaStream_t st) {
   const bool bf = p->io == SFFFT_IO_BF16, tc = bf && la_tc_takes(*prm);
+  prm->wait_ns = t_wait_ns;
+  prm->withhold = t_withhold;
   plan(p, backward, tc, f.sms, &prm->G, &prm->seg);
   if (tc) {
     long long slices = 0;
@@ -438,6 +444,14 @@ int sffft_linear_attention_check(int device) {
   int status = 0;
   const cudaError_t ce = la_tc_status(&status);
   return ce == cudaSuccess ? status : sffft_note_cuda_error(ce);
+}
+
+int sffft_debug_linear_attention(int limit_us, int withhold) {
+  if (limit_us < 0 || limit_us > 1000000 || withhold < LA_WITHHOLD_NONE || withhold > LA_WITHHOLD_OOUT || (withhold && !limit_us))
+    return SFFFT_ERR_INVALID_ARGUMENT;
+  t_wait_ns = limit_us ? 1000ull * (unsigned long long)limit_us : kLaWaitNs;
+  t_withhold = withhold;
+  return SFFFT_OK;
 }
 
 int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const void* q, const void* k, const void* v,

@@ -42,7 +42,13 @@ struct LaParams {
   int ntask, B, H, L;
   int G, seg;        // segments that the positions are cut into, and positions in each
   int sms;
+  unsigned long long wait_ns;   // tensor cores: the limit of a wait
+  int withhold;                 // test hook of sffft_debug_linear_attention: an arrival that one thread leaves out
 };
+
+// X of a segment's last chunk; the scaling of O; O's staging.
+enum { LA_WITHHOLD_NONE = 0, LA_WITHHOLD_X = 1, LA_WITHHOLD_OS = 2, LA_WITHHOLD_OOUT = 3 };
+constexpr unsigned long long kLaWaitNs = 2000000000ull;
 
 // lambda^n from log2(lambda) held as the sum hi + lo of two floats: hi * n is split exactly, so that the error is
 // that of one exp2f, not of |hi * n| roundings.

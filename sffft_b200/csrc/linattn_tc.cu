@@ -32,8 +32,9 @@
 // pipe is busy for 31 to 35 %.  Tried and slower: four state warpgroups at head size 64 (85 us), the third part of X kept in
 // registers at 128 (spills, 167 -> 194 us), the next launch's prologue overlapped with the last one's end (no gain).
 //
-// Every wait is bounded: after kWaitLimit ns the waiting role raises the CTA's flag, all roles leave, and the device's
-// status word says so.
+// Every wait on an mbarrier is bounded: after LaParams::wait_ns the waiting role raises the CTA's flag, all roles leave, and
+// the device's status word says so.  The named barriers (bar.sync) stand where every thread of theirs comes by, given up or
+// not: behind the state warpgroups' loop, and at the block's ends.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -52,7 +53,7 @@ static __device__ int g_la_status;
 namespace {
 
 constexpr int kTok = 128;   // positions in a chunk
-constexpr uint64_t kWaitLimit = 2000000000ull;
+constexpr uint64_t kCopyLimit = 2000000000ull;   // of what is in flight when a CTA gives up
 constexpr uint32_t kBlk = kTok * 128;   // bytes of a 64-column tile of 128 positions: 128-byte rows, 128-byte swizzle
 
 struct __align__(64) LaTcParams {
@@ -91,7 +92,7 @@ struct Shape {
   static constexpr uint32_t q_bytes = DQ / 64 * kBlk, v_bytes = NB * kBlk;
   static constexpr uint32_t off_k = LOCAL ? 0 : q_bytes, off_v = off_k + q_bytes, stage = off_v + v_bytes;
   static constexpr uint32_t off_s = NS * stage, off_tab = off_s + NB * kBlk, off_bar = off_tab + 4 * 160;
-  static constexpr uint32_t smem = off_bar + 42 * 8 + 8;
+  static constexpr uint32_t smem = off_bar + 42 * 8 + 16;
   static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one CTA on an SM: each takes all of TMEM");
   // TMEM columns.  Products Q K^T (P over their first half) and O of A warpgroup a; the increment of S; X.
   __host__ __device__ static constexpr uint32_t c_p(int a) { return (uint32_t)a * 128; }
@@ -234,12 +235,6 @@ __device__ __forceinline__ void wg_sync(int wg) {
   }
 }
 
-// among the 128 threads of an A warpgroup
-__device__ __forceinline__ void a_sync(int a) {
-  if (a == 0) asm volatile("bar.sync 6, 128;" ::: "memory");
-  else asm volatile("bar.sync 7, 128;" ::: "memory");
-}
-
 // two floats in one instruction
 struct F2 {
   float a, b;
@@ -288,7 +283,7 @@ __device__ __forceinline__ bool try_wait_for(uint64_t* bar, uint32_t parity) {
 
 struct Waiter {
   uint64_t* bars;
-  volatile int* stop;
+  volatile int* stop;   // the limit of a wait lies two words behind
   // false: the CTA gives up
   __device__ __forceinline__ bool operator()(int b, uint32_t parity) const {
     if (try_wait_for(bars + b, parity)) return true;
@@ -298,7 +293,7 @@ struct Waiter {
     const uint64_t t0 = global_ns();
     while (!try_wait_for(bars + b, parity)) {
       if (*stop) return false;
-      if (global_ns() - t0 > kWaitLimit) {
+      if (global_ns() - t0 > *(volatile uint64_t*)(stop + 2)) {
         *stop = 1;
         atomicExch(&g_la_status, SFFFT_ERR_TIMEOUT);
         return false;
@@ -361,8 +356,8 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       const bool x = (i >= B_REL && i < B_PV) || i == B_X || i == B_X2 || i == B_ST;
       mbar_init(bars + i, a ? 128u : x ? 128u * NW : 1u);
     }
-    *stop = (sm & 1023u) != 0;   // swizzled tiles need the alignment that the launch gives
-    if (*stop) atomicExch(&g_la_status, SFFFT_ERR_DEVICE);
+    *stop = 0;
+    *(volatile uint64_t*)(stop + 2) = lp.wait_ns;
     fence_mbar_init();
   }
   for (int i = threadIdx.x; i < 160; i += blockDim.x) {
@@ -378,11 +373,10 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   tc_fence_after();
   // The CTA holds all 512 columns, which begin at address 0: a constant, so that the products' operands need no registers.
   constexpr uint32_t tm = 0;
-  if (*slot != tm && threadIdx.x == 0) {
-    *stop = 1;
-    atomicExch(&g_la_status, SFFFT_ERR_DEVICE);
-  }
-  if (*slot != tm) __syncthreads();   // (all see the same slot)
+  // Swizzled tiles need the alignment that the launch gives.  Not by `stop`, which an early role may raise before a late one
+  // has looked: all threads have to decide alike.
+  const bool dead = *slot != tm || (sm & 1023u) != 0;
+  if (dead && threadIdx.x == 0) atomicExch(&g_la_status, SFFFT_ERR_DEVICE);
   const Waiter wait{bars, stop};
   const WarpWaiter wwait{wait};
   auto power = [&](int e) { return tab[rev ? 32 + e : 127 - e]; };   // 0 <= e < 128
@@ -400,7 +394,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   auto x_ph = [](int c) { return (uint32_t)(SH::split && !LOCAL ? c >> 1 : c) & 1; };
   auto x_col = [&](int c) { return SH::c_x + (two_x ? (uint32_t)(c & 1) * 64 : 0u); };
 
-  if (*stop) {
+  if (dead) {
     // nothing has been started
   } else if (warp == SH::threads / 32 - 2) {
     // ---- loads, stores ----
@@ -450,8 +444,8 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (*stop) {   // copies in flight end before the block does
-        for (int c = max(0, kv - NS); c < kv; c++) mbar_wait_bounded(bars + B_KV + c % NS, sph(c), kWaitLimit);
-        for (int c = max(0, qs - NS); !SH::split && c < qs; c++) mbar_wait_bounded(bars + B_Q + c % NS, sph(c), kWaitLimit);
+        for (int c = max(0, kv - NS); c < kv; c++) mbar_wait_bounded(bars + B_KV + c % NS, sph(c), kCopyLimit);
+        for (int c = max(0, qs - NS); !SH::split && c < qs; c++) mbar_wait_bounded(bars + B_Q + c % NS, sph(c), kCopyLimit);
       }
     }
   } else if (warp == SH::threads / 32 - 1) {
@@ -559,7 +553,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
     if (*stop) {   // products in flight end before TMEM is given back
       if (elect_one()) {
         mma_commit(bars + B_FIN);
-        mbar_wait_bounded(bars + B_FIN, 0, kWaitLimit);
+        mbar_wait_bounded(bars + B_FIN, 0, kCopyLimit);
       }
       __syncwarp();
     }
@@ -620,12 +614,13 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
           tmem_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(bars + B_OS + a);
+        if (!(lp.withhold == LA_WITHHOLD_OS && i == 0)) mbar_arrive(bars + B_OS + a);
         if (!wwait(B_O + a, ph)) break;
         tc_fence_after();
         // staged where Q was, whose products are complete: bf16 in the swizzled rows that the TMA store takes, or fp32, 64
-        // (split: 32) columns at a time, from where the warpgroup writes whole rows (a lane's own row would be pieces of 16
-        // bytes in 32 rows at once)
+        // (split: 32) columns at a time, from where the warp writes its 32 rows as whole ones (a lane's own row would be
+        // pieces of 16 bytes in 32 rows at once).  A warp's rows are its own business: a barrier among the warps would not
+        // be bounded, and one of them may have given up.
         const uint32_t out = stage_at(c) + (uint32_t)i * 128;
 #pragma unroll 1
         for (int q = 0; q < DV / 32; q++) {
@@ -657,21 +652,21 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
               sts128(blk_at + (uint32_t)i * 128 + (((uint32_t)e ^ (uint32_t)(i & 7)) << 4), __float_as_uint(tk.scale * __uint_as_float(r[4 * e])),
                      __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 1])), __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 2])),
                      __float_as_uint(tk.scale * __uint_as_float(r[4 * e + 3])));
-            a_sync(a);
+            __syncwarp();
             float* y = (float*)tk.y + b * tk.ys[0] + h * tk.ys[1] + (long long)(blk * kTok) * tk.ys[2] + cb + q * 32;
 #pragma unroll 4
-            for (int x = 0; x < 8; x++) {   // 16 rows of 8 pieces at a time; Dv is a multiple of 8
-              const int row = x * 16 + (i >> 3), e = i & 7;
+            for (int x = 0; x < 8; x++) {   // 4 rows of 8 pieces at a time; Dv is a multiple of 8
+              const int row = quad * 32 + x * 4 + (lane >> 3), e = lane & 7;
               if (blk * kTok + row < lp.L && cb + q * 32 + e * 4 < tk.Dv)
                 *(float4*)(y + (long long)row * tk.ys[2] + e * 4) = lds_f4(blk_at + (uint32_t)row * 128 + ((uint32_t)(e ^ (row & 7)) << 4));
             }
-            if (SH::q_bytes == kBlk || (q & 1)) a_sync(a);
+            if (SH::q_bytes == kBlk || (q & 1)) __syncwarp();
           }
         }
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(bars + B_OFREE + a);
-        mbar_arrive(bars + B_OOUT + c % NS);
+        if (!(lp.withhold == LA_WITHHOLD_OOUT && i == 0)) mbar_arrive(bars + B_OOUT + c % NS);
       }
       // chunks of the segment behind the row's last token
       const int z0 = max(g * prm.blocks, nblk) * kTok, z1 = min((long long)(g + 1) * prm.blocks * kTok, (long long)lp.L);
@@ -840,7 +835,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
         fence_async_smem();
       }
       make_x(c, m, false);
-      mbar_arrive(bars + x_bar(c));
+      if (!(lp.withhold == LA_WITHHOLD_X && c == nc - 1 && wg == 0 && t == 0)) mbar_arrive(bars + x_bar(c));
       return true;
     };
     // X of the next chunk goes before this one's state: it needs only the columns that this one's product has read, or, with
