@@ -253,18 +253,19 @@ __device__ __forceinline__ void group_sums(float (&v)[NV], int nvec, int per, in
   for (int j = 0; j < NV; j++) v[j] = j * tpr + t < nvec ? grp[(j * tpr + t) / per] : 0.f;
 }
 
-// Shared memory of a row: vector sums and group sums (only where group_sums needs them).
+// Shared memory of a row: vector sums and group sums (only where group_sums needs them).  All of it is dynamic, row_sums' too:
+// a launch's limit counts both kinds.
 __host__ __device__ inline int rows_smem_floats(int nvec, int groups) { return groups > 1 ? nvec + groups : 0; }
+constexpr int kRedForward = 2 * 32, kRedBackward = 2 * 3 * 32;   // floats of row_sums, where a row is a block's
 
 constexpr int kRowsPerBlock = 4;   // where a row is a warp's
 
 template <class TX, class TY, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 32 * kRowsPerBlock) norm_rows_kernel(const __grid_constant__ NormParams p) {
-  extern __shared__ __align__(16) float dyn[];
-  __shared__ float red[2 * 32];
+  extern __shared__ __align__(16) float red[];
   const int tpr = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nvec = p.C / VEC;
   const int sub = BLOCK ? 0 : threadIdx.x >> 5, nw = tpr >> 5, per = p.gc / VEC;
-  float* vec = dyn + sub * rows_smem_floats(nvec, p.groups);
+  float* vec = red + (BLOCK ? kRedForward : 0) + sub * rows_smem_floats(nvec, p.groups);
   const long long r = BLOCK ? (long long)blockIdx.x : blockIdx.x * (long long)kRowsPerBlock + sub;
   if (r >= p.rows) return;   // whole warps
   int turn = 0;
@@ -387,11 +388,10 @@ struct RawRow {
 template <class TX, class TY, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bwd_kernel(const __grid_constant__ NormParams p) {
   constexpr bool AHEAD = NV == 1;   // registers for the next row
-  extern __shared__ __align__(16) float dyn[];
-  __shared__ float red[2 * 3 * 32];
+  extern __shared__ __align__(16) float red[];
   const int tpr = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nvec = p.C / VEC;
   const int sub = BLOCK ? 0 : threadIdx.x >> 5, nw = tpr >> 5, per = p.gc / VEC;
-  float* vec = dyn + sub * rows_smem_floats(nvec, p.groups);
+  float* vec = red + (BLOCK ? kRedBackward : 0) + sub * rows_smem_floats(nvec, p.groups);
   int turn = 0, grp[NV];
   float sw[NV][VEC], sp[NV][VEC], sg[NV][VEC];
 #pragma unroll
@@ -968,13 +968,13 @@ template <class TX, class TY, int VEC, int NV, bool BLOCK>
 cudaError_t rows_fwd(const NormParams& p, cudaStream_t st) {
   const int nvec = p.C / VEC, tpr = BLOCK ? ((nvec + NV - 1) / NV + 31) / 32 * 32 : 32, rpb = BLOCK ? 1 : kRowsPerBlock;
   return launch(norm_rows_kernel<TX, TY, VEC, NV, BLOCK>, dim3((unsigned)((p.rows + rpb - 1) / rpb)), tpr * rpb,
-                4 * rpb * rows_smem_floats(nvec, p.groups), st, p);
+                4 * ((BLOCK ? kRedForward : 0) + rpb * rows_smem_floats(nvec, p.groups)), st, p);
 }
 template <class TX, class TY, int VEC, int NV, bool BLOCK>
 cudaError_t rows_bwd(const NormParams& p, cudaStream_t st) {
   const int nvec = p.C / VEC, tpr = BLOCK ? ((nvec + NV - 1) / NV + 31) / 32 * 32 : 32, rpb = BLOCK ? 1 : kRowsPerBlock;
   return launch(norm_rows_bwd_kernel<TX, TY, VEC, NV, BLOCK>, dim3((unsigned)p.blocks), tpr * rpb,
-                4 * rpb * rows_smem_floats(nvec, p.groups), st, p);
+                4 * ((BLOCK ? kRedBackward : 0) + rpb * rows_smem_floats(nvec, p.groups)), st, p);
 }
 
 // Vectors of a thread: one, as long as a block's threads do.

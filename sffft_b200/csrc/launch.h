@@ -15,6 +15,8 @@ inline bool on_elements(size_t size, std::initializer_list<const void*> ps) {
   return true;
 }
 
+// `smem` bytes of dynamic shared memory.  Kernels that take more than 48 KB of it have no static shared memory, which the limit
+// would count too.
 template <class K, class P>
 cudaError_t launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& prm) {
   if (smem > 48 * 1024) {   // a property of the kernel on the current device; setting it again costs under 1 us
