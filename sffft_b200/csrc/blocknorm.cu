@@ -962,8 +962,6 @@ __global__ void __launch_bounds__(1024) norm_part_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kMaxShared = 227 * 1024;
-
 template <class TX, class TY, int VEC, int NV, bool BLOCK>
 cudaError_t rows_fwd(const NormParams& p, cudaStream_t st) {
   const int nvec = p.C / VEC, tpr = BLOCK ? ((nvec + NV - 1) / NV + 31) / 32 * 32 : 32, rpb = BLOCK ? 1 : kRowsPerBlock;

@@ -15,13 +15,17 @@ inline bool on_elements(size_t size, std::initializer_list<const void*> ps) {
   return true;
 }
 
+constexpr int kMaxShared = 227 * 1024;   // of a block on sm_100
+
 // `smem` bytes of dynamic shared memory.  Kernels that take more than 48 KB of it have no static shared memory, which the limit
 // would count too.
 template <class K, class P>
 cudaError_t launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& prm) {
-  if (smem > 48 * 1024) {   // a property of the kernel on the current device; setting it again costs under 1 us
+  if (smem > 48 * 1024) {
+    // A property of the kernel on the current device, which other threads' calls set too: always to the most that there
+    // is, so that none takes away what another is about to launch with.  Setting it again costs under 1 us.
     const cudaError_t ce =
-        cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
     if (ce != cudaSuccess) return ce;
   }
   cudaLaunchConfig_t cfg = {};
