@@ -260,7 +260,9 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
                                     void* work, size_t work_bytes, void* stream);
 
 /* Waits for the device and returns (and clears) what its linear attention kernels reported: SFFFT_OK, or
- * SFFFT_ERR_TIMEOUT when a barrier wait of one gave up, and its outputs are not valid. */
+ * SFFFT_ERR_TIMEOUT when a barrier wait of one gave up, and its outputs are not valid.  Until then every later call on the
+ * device (the single-token one too, whose states may come from there) returns the same status and does nothing,
+ * without waiting: as soon as the kernel that reported it has ended. */
 int sffft_linear_attention_check(int device);
 
 /* One token for each of B rows: S <- lambda S + k v^T in place, y = scale * S^T q.  The states lie in a pool of slots

@@ -666,7 +666,8 @@ def linear_attention_backward(q, k, v, log_decay, dy, dfinal_state=None, scale=1
 
 
 def linear_attention_check(device: int = 0):
-    """Waits for the device and raises if one of its linear attention kernels reported a device-side error."""
+    """Waits for the device and raises if one of its linear attention kernels reported a device-side error, and clears it.
+    Until then later calls raise the same, without waiting for a device."""
     _check(lib().sffft_linear_attention_check(device), "device status")
 
 

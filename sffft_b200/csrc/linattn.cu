@@ -268,7 +268,8 @@ int run(const sffft_linear_attention_t* p, int backward, LaParams* prm, const De
     prm->task[i].loc = (float*)work;
     work += sz.loc[i];
   }
-  const cudaError_t ce = tc ? launch_la_tc(*prm, st) : launch_la_general(*prm, bf, st);
+  cudaError_t ce = tc ? la_tc_word(p->device, &prm->status) : cudaSuccess;
+  if (ce == cudaSuccess) ce = tc ? launch_la_tc(*prm, st) : launch_la_general(*prm, bf, st);
   return ce == cudaSuccess ? SFFFT_OK : sffft_note_cuda_error(ce);
 }
 
@@ -343,6 +344,7 @@ int sffft_linear_attention(const sffft_linear_attention_t* p, const void* q, con
   if (!on_elements(io_size(p->io), {q, k, v, y}) || !on_elements(4, {log_decay, lengths, initial_state, final_state}))
     return SFFFT_ERR_INVALID_ARGUMENT;
   if (initial_state && initial_state == final_state) return SFFFT_ERR_INVALID_ARGUMENT;   // segments start from it all along
+  if ((rc = la_tc_reported(p->device))) return rc;
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
@@ -376,6 +378,7 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
       !on_elements(4, {log_decay, lengths, initial_state, dfinal_state, dinitial_state}))
     return SFFFT_ERR_INVALID_ARGUMENT;
   if (dinitial_state && dinitial_state == dfinal_state) return SFFFT_ERR_INVALID_ARGUMENT;   // as forward
+  if ((rc = la_tc_reported(p->device))) return rc;
   DeviceFacts f;
   if ((rc = start(p, &f))) return rc;
   LaParams prm = {};
@@ -442,7 +445,7 @@ int sffft_linear_attention_check(int device) {
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return sffft_note_cuda_error(scope.err);
   int status = 0;
-  const cudaError_t ce = la_tc_status(&status);
+  const cudaError_t ce = la_tc_status(device, &status);
   return ce == cudaSuccess ? status : sffft_note_cuda_error(ce);
 }
 
@@ -464,6 +467,7 @@ int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const vo
   if (p->B == 0) return SFFFT_OK;
   if (!q || !k || !v || !log_decay || (!state && p->pool > 0) || !y) return SFFFT_ERR_INVALID_ARGUMENT;
   if (!on_elements(io_size(p->io), {q, k, v, y}) || !on_elements(4, {log_decay, state, slots})) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (const int rc = la_tc_reported(p->device)) return rc;   // the states may come from the call that reported it
   DeviceFacts f;
   const cudaError_t fe = device_facts(p->device, &f);
   if (fe != cudaSuccess) return sffft_note_cuda_error(fe);

@@ -43,6 +43,7 @@ struct LaParams {
   int G, seg;        // segments that the positions are cut into, and positions in each
   int sms;
   unsigned long long wait_ns;   // tensor cores: the limit of a wait
+  int* status;                  // and where one that runs out is reported
   int withhold;                 // test hook of sffft_debug_linear_attention: an arrival that one thread leaves out
 };
 
@@ -81,7 +82,12 @@ inline int la_general_chunk(int dmax) { return dmax > 128 ? 32 : 64; }
 // bf16 on the tensor cores: D up to 128, D and Dv multiples of 8, 16-byte aligned rows (la_tc_takes), any length.
 bool la_tc_takes(const LaParams& prm);
 cudaError_t launch_la_tc(const LaParams& prm, cudaStream_t st);
-cudaError_t la_tc_status(int* status);   // waits for the current device; reads and clears its status word
+// The status word of a device (where kernels write it), what has been reported there so far, and, having waited for the current
+// device, the same with the word cleared.
+constexpr int kLaMaxDevices = 64;
+cudaError_t la_tc_word(int device, int** word);
+int la_tc_reported(int device);
+cudaError_t la_tc_status(int device, int* status);
 constexpr int kLaTcChunk = 128;
 int la_tc_slices(int D, int Dv);   // CTAs over the columns of v
 

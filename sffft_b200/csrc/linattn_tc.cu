@@ -33,12 +33,14 @@
 // registers at 128 (spills, 167 -> 194 us), the next launch's prologue overlapped with the last one's end (no gain).
 //
 // Every wait on an mbarrier is bounded: after LaParams::wait_ns the waiting role raises the CTA's flag, all roles leave, and
-// the device's status word says so.  The named barriers (bar.sync) stand where every thread of theirs comes by, given up or
+// the device's status word says so, which lies in host memory so that a later call can look at it without waiting.  The named barriers (bar.sync) stand where every thread of theirs comes by, given up or
 // not: behind the state warpgroups' loop, and at the block's ends.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 
 #include "../../include/sffft.h"
 #include "launch.h"
@@ -47,8 +49,6 @@
 #include "tc.cuh"
 
 namespace sffft {
-
-static __device__ int g_la_status;
 
 namespace {
 
@@ -284,6 +284,7 @@ __device__ __forceinline__ bool try_wait_for(uint64_t* bar, uint32_t parity) {
 struct Waiter {
   uint64_t* bars;
   volatile int* stop;   // the limit of a wait lies two words behind
+  volatile int* status;
   // false: the CTA gives up
   __device__ __forceinline__ bool operator()(int b, uint32_t parity) const {
     if (try_wait_for(bars + b, parity)) return true;
@@ -295,7 +296,7 @@ struct Waiter {
       if (*stop) return false;
       if (global_ns() - t0 > *(volatile uint64_t*)(stop + 2)) {
         *stop = 1;
-        atomicExch(&g_la_status, SFFFT_ERR_TIMEOUT);
+        *status = SFFFT_ERR_TIMEOUT;
         return false;
       }
     }
@@ -376,8 +377,8 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
   // Swizzled tiles need the alignment that the launch gives.  Not by `stop`, which an early role may raise before a late one
   // has looked: all threads have to decide alike.
   const bool dead = *slot != tm || (sm & 1023u) != 0;
-  if (dead && threadIdx.x == 0) atomicExch(&g_la_status, SFFFT_ERR_DEVICE);
-  const Waiter wait{bars, stop};
+  if (dead && threadIdx.x == 0) *(volatile int*)lp.status = SFFFT_ERR_DEVICE;
+  const Waiter wait{bars, stop, lp.status};
   const WarpWaiter wwait{wait};
   auto power = [&](int e) { return tab[rev ? 32 + e : 127 - e]; };   // 0 <= e < 128
 
@@ -1042,13 +1043,47 @@ cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
   return cudaSuccess;
 }
 
-cudaError_t la_tc_status(int* status) {
-  void* p = nullptr;
-  cudaError_t ce = cudaGetSymbolAddress(&p, g_la_status);
-  const int zero = 0;
-  if (ce == cudaSuccess) ce = cudaDeviceSynchronize();
-  if (ce == cudaSuccess) ce = cudaMemcpy(status, p, sizeof(int), cudaMemcpyDeviceToHost);
-  if (ce == cudaSuccess && *status) ce = cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice);
+// Status words of the devices, in page-locked host memory that every device can write.
+namespace {
+std::atomic<int*> g_words{nullptr};
+}
+
+cudaError_t la_tc_word(int device, int** word) {
+  static std::mutex mutex;
+  if (device < 0 || device >= kLaMaxDevices) return cudaErrorInvalidDevice;
+  int* p = g_words.load(std::memory_order_acquire);
+  if (!p) {
+    std::lock_guard<std::mutex> lock(mutex);
+    p = g_words.load(std::memory_order_relaxed);
+    if (!p) {
+      // The first call may be one that a graph captures, where allocations are refused unless the thread says otherwise.
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaError_t ce = cudaThreadExchangeStreamCaptureMode(&mode);
+      if (ce != cudaSuccess) return ce;
+      void* m = nullptr;
+      ce = cudaHostAlloc(&m, kLaMaxDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (ce != cudaSuccess) return ce;
+      p = (int*)m;
+      std::fill(p, p + kLaMaxDevices, 0);
+      g_words.store(p, std::memory_order_release);
+    }
+  }
+  void* on_device = nullptr;
+  const cudaError_t ce = cudaHostGetDevicePointer(&on_device, p + device, 0);
+  *word = (int*)on_device;
+  return ce;
+}
+
+int la_tc_reported(int device) {
+  const int* p = g_words.load(std::memory_order_acquire);
+  return p && device >= 0 && device < kLaMaxDevices ? *(const volatile int*)(p + device) : SFFFT_OK;
+}
+
+cudaError_t la_tc_status(int device, int* status) {
+  const cudaError_t ce = cudaDeviceSynchronize();
+  *status = ce == cudaSuccess ? la_tc_reported(device) : SFFFT_OK;
+  if (*status) ((volatile int*)g_words.load())[device] = 0;
   return ce;
 }
 

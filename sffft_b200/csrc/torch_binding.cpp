@@ -42,6 +42,8 @@ void status(int rc, const char* what) {
   if (rc == SFFFT_OK) return;
   std::string s = what;
   add(s, ": "), add(s, sffft_status_string(rc)), add(s, " (status "), add(s, (int64_t)rc), add(s, ")");
+  if (rc == SFFFT_ERR_TIMEOUT)
+    add(s, ": results of an earlier call are not valid; sffft_b200.linear_attention_check(device) reports and clears this");
   TORCH_CHECK(false, s);
 }
 

@@ -2,6 +2,9 @@
 2 ms; all roles leave, the status says so, and the next call on the same context gives what it gave before (a block that kept
 its TMEM would block every later one on its SM)."""
 import contextlib
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -11,6 +14,7 @@ import sffft_b200 as sf
 pytestmark = pytest.mark.gpu
 
 BF = torch.bfloat16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 X, SCALED, STAGED = 1, 2, 3
 
 
@@ -50,3 +54,50 @@ def test_all_roles_leave_when_a_wait_runs_out(shape, what):
         sf.linear_attention_check()          # the check cleared the status
         assert all(torch.equal(a, b) for a, b in zip(call(), want))
         sf.linear_attention_check()
+
+
+def test_later_calls_raise_until_the_status_is_cleared():
+    import sffft_b200.torch_ops as ops
+    r = lambda *s: torch.randn(s, device="cuda")  # noqa: E731
+    q, ld, s0 = r(1, 2, 100, 64).to(BF), torch.full((2,), -0.1, device="cuda"), r(1, 2, 64, 64)
+    want, _ = sf.linear_attention(q, q, q, ld)
+    leaf = q.clone().requires_grad_()
+    y, _ = ops.linear_attention(leaf, q, q, ld)
+    with withheld(SCALED):
+        sf.linear_attention(q, q, q, ld)
+    torch.cuda.synchronize()     # the kernel has reported; nothing has read it
+    before = s0.clone()
+    for call in (lambda: ops.linear_attention(q, q, q, ld), lambda: y.sum().backward(),
+                 lambda: ops.linear_attention(q.float(), q.float(), q.float(), ld),
+                 lambda: ops.linear_attention_step(q[:, :, 0], q[:, :, 0], q[:, :, 0], ld, s0)):
+        with pytest.raises(RuntimeError, match="timed out.*linear_attention_check"):
+            call()
+    for call in (lambda: sf.linear_attention(q, q, q, ld), lambda: sf.linear_attention_backward(q, q, q, ld, q),
+                 lambda: sf.linear_attention_step(q[:, :, 0], q[:, :, 0], q[:, :, 0], ld, s0)):
+        with pytest.raises(sf.SffftError) as e:
+            call()
+        assert e.value.status == sf.ERR_TIMEOUT
+    assert torch.equal(s0, before)
+    with pytest.raises(sf.SffftError):
+        sf.linear_attention_check()
+    assert torch.equal(ops.linear_attention(q, q, q, ld)[0], want)
+    sf.linear_attention_check()
+
+
+def test_a_process_whose_first_call_is_captured():
+    """The status word is allocated by the first call, which a graph may capture."""
+    code = """if 1:
+        import torch
+        import sffft_b200 as sf
+        q = torch.randn((1, 2, 300, 64), device="cuda").to(torch.bfloat16)
+        ld = torch.full((2,), -0.1, device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y, s = sf.linear_attention(q, q, q, ld)
+        g.replay()
+        a, b = sf.linear_attention(q, q, q, ld)
+        assert torch.equal(a, y) and torch.equal(b, s) and s.abs().max() > 0
+        """
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
