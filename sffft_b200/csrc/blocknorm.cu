@@ -623,6 +623,9 @@ __host__ __device__ inline int first_part_floats(int groups, int n) {
   return groups >= kManyGroups ? kFirstWarps * kPos : n * groups * kFirstWarps * kPos;
 }
 
+// Tiles of a row of the batch (inner + kPos - 1 may pass 31 bits).
+__host__ __device__ inline int first_tiles(int inner) { return inner / kPos + (inner % kPos != 0); }
+
 struct FirstTile {
   long long base;   // element (channel 0, first position of the thread)
   long long row;    // row index of that position
@@ -631,9 +634,8 @@ struct FirstTile {
 
 template <int VEC>
 __device__ __forceinline__ FirstTile first_tile(const NormParams& p, long long tile) {
-  const int per = (p.inner + kPos - 1) / kPos;
-  const long long b = tile / per;
-  const int l = (int)(tile % per) * kPos + (int)(threadIdx.x % FirstShape<VEC>::TX) * VEC;
+  const int per = first_tiles(p.inner);
+  const long long b = tile / per, l = tile % per * kPos + (threadIdx.x % FirstShape<VEC>::TX) * VEC;
   return {b * p.C * p.inner + l, b * p.inner + l, l < p.inner};
 }
 
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
   float* out = p.part + (long long)blockIdx.x * 3 * p.C;
   float* acc = p.sums_shared ? part + first_part_floats(p.groups, 3) : out;
   const long long L = p.inner;
-  const int per = (p.inner + kPos - 1) / kPos;
+  const int per = first_tiles(p.inner);
   const long long tiles = (p.rows / p.inner) * per;
   const TY* gate = (const TY*)p.gate;
   bool first = true;
@@ -1001,7 +1003,7 @@ cudaError_t rows_v(const NormParams& p, bool bwd, cudaStream_t st) {
 
 template <class TX, class TY, int VEC>
 cudaError_t first_v(const NormParams& p, bool bwd, cudaStream_t st) {
-  const long long tiles = (p.rows / p.inner) * ((p.inner + kPos - 1) / kPos);
+  const long long tiles = (p.rows / p.inner) * first_tiles(p.inner);
   if (bwd) {
     const int smem = 4 * (4 * p.groups * kPos + first_part_floats(p.groups, 3)), with = smem + 4 * 3 * p.C;
     NormParams q = p;
@@ -1061,7 +1063,7 @@ int check(const sffft_block_norm_t* d, const void* x, const void* y, const void*
 }
 
 int backward_blocks(const sffft_block_norm_t* d, int sms) {
-  const long long units = d->inner ? (d->rows / d->inner) * ((d->inner + kPos - 1) / kPos) : d->rows;
+  const long long units = d->inner ? (d->rows / d->inner) * first_tiles(d->inner) : d->rows;
   // rows: as many blocks of a row's threads as an SM's registers hold at 128 each; channels first: two
   const int threads = (d->channels / (d->io == SFFFT_IO_BF16 ? 8 : 4) + 31) / 32 * 32;
   const int per_sm = d->inner ? 2 : threads > 256 ? 1 : threads <= 32 ? 4 : 512 / threads;
