@@ -370,6 +370,17 @@ bool wants(std::initializer_list<const optional<Tensor>*> ts) {
   return false;
 }
 
+// A tensor of forward-mode differentiation need not require a gradient, and would pass the autograd functions by: the result
+// would have no tangent, which counts as a zero one.
+template <class... T>
+void need_no_tangent(const char* what, const T&... ts) {
+  auto has = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) return t._fw_grad(0).defined();
+    else return t && t->_fw_grad(0).defined();
+  };
+  need(!(has(ts) || ...), what, " has no forward-mode derivative");
+}
+
 Tensor or_none(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 optional<Tensor> opt(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 
@@ -417,6 +428,7 @@ struct Attention : torch::autograd::Function<Attention> {
 std::tuple<Tensor, Tensor> attention_grad(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                           const optional<Tensor>& s0, const optional<Tensor>& lengths, double scale) {
   need(!log_decay.requires_grad(), "log_decay is a constant: it has no gradient (pass log_decay.detach())");
+  need_no_tangent("linear_attention", q, k, v, log_decay, s0);
   if (wants({&s0}) || (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))) {
     auto out = Attention::apply(q, k, v, log_decay, s0, lengths, scale);
     return {out[0], out[1]};
@@ -430,6 +442,7 @@ Tensor step_grad(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   need(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                      log_decay.requires_grad() || state.requires_grad()),
                     "linear_attention_step updates its state in place and has no gradient: use linear_attention, or no_grad");
+  need_no_tangent("linear_attention_step", q, k, v, log_decay, state);
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     Tensor y = step_op().call(q, k, v, log_decay, state, slots, scale);
@@ -477,6 +490,7 @@ struct Norm : torch::autograd::Function<Norm> {
 std::vector<Tensor> norm_grad(const optional<Tensor>& x, const optional<Tensor>& y, const optional<Tensor>& gate,
                               const optional<Tensor>& pw, const optional<Tensor>& w, double scale, double eps, int64_t groups,
                               c10::string_view act, int64_t dim, bool stats) {
+  need_no_tangent("block_norm", x, y, gate, pw, w);
   if (wants({&x, &y, &gate, &pw, &w})) {
     need(!stats, "stats are for calls without a gradient");
     return Norm::apply(x, y, gate, pw, w, scale, eps, groups, std::string(act), dim);

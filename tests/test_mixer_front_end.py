@@ -1,6 +1,15 @@
 """Linear attention and block_norm on the CPU: what the PyTorch operators, the Python functions and the C ABI do with a call
 before anything runs on a device."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
 import sffft_b200 as sf
+import sffft_b200.torch_ops as ops
+
+
+def meta(*s, dtype=torch.float32):
+    return torch.empty(s, device="meta", dtype=dtype)
 
 
 def test_the_wait_limit_refuses_what_it_does_not_know():
@@ -8,3 +17,24 @@ def test_the_wait_limit_refuses_what_it_does_not_know():
     for bad in ((-1, 0), (1000001, 0), (2000, -1), (2000, 4), (0, 1)):
         assert f(*bad) == sf.ERR_INVALID_ARGUMENT
     assert f(2000, 3) == sf.OK and f(0, 0) == sf.OK
+
+
+ATTENTION = dict(q=meta(2, 4, 10, 16), k=meta(2, 2, 10, 16), v=meta(2, 2, 10, 24), log_decay=meta(4), initial_state=meta(2, 4, 16, 24))
+STEP = dict(q=meta(2, 4, 16), k=meta(2, 2, 16), v=meta(2, 2, 24), log_decay=meta(4), state=meta(5, 4, 16, 24))
+NORM = dict(x=meta(3, 32), y=meta(3, 32), gate=meta(3, 32), post_weight=meta(32), weight=meta(32))
+
+
+@pytest.mark.parametrize("op,args", [(ops.linear_attention, ATTENTION), (ops.linear_attention_step, STEP), (ops.block_norm, NORM)],
+                         ids=["linear_attention", "linear_attention_step", "block_norm"])
+def test_forward_mode_derivatives_are_refused(op, args):
+    """They would come out as zero: a tensor with a tangent need not require a gradient."""
+    for name, x in args.items():
+        with forward_ad.dual_level():
+            dual = dict(args, **{name: forward_ad.make_dual(x, torch.ones_like(x))})
+            with pytest.raises(ValueError, match="forward-mode"):
+                op(**dual)
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                op(**dual)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.func.jvp(lambda t: op(**dict(args, **{name: t})), (x,), (x,))
+        op(**args)
