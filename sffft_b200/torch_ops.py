@@ -173,12 +173,12 @@ _block_norm = torch.ops.sffft.block_norm.default
 def _(q, k, v, log_decay, initial_state, lengths, scale):
     sf.check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
     B, H, L, D = q.shape
-    return sf._heads_like(q, B, H, L, v.shape[3], q.dtype), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
+    return sf._heads_like(sf._unit(q), B, H, L, v.shape[3], q.dtype), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
 
 
 @torch.library.register_fake("sffft::linear_attention_backward")
 def _(q, k, v, log_decay, initial_state, lengths, scale, dy, dfinal_state):
-    out = [sf._heads_like(t, *t.shape, q.dtype) for t in (q, k, v)]
+    out = [sf._heads_like(sf._unit(t), *t.shape, q.dtype) for t in (q, k, v)]   # as the operator orders them: behind its copies
     return out if initial_state is None else out + [torch.empty_like(initial_state, memory_format=torch.contiguous_format)]
 
 

@@ -38,3 +38,23 @@ def test_forward_mode_derivatives_are_refused(op, args):
         with pytest.raises(ValueError, match="forward-mode"):
             torch.func.jvp(lambda t: op(**dict(args, **{name: t})), (x,), (x,))
         op(**args)
+
+
+def strided(heads, d, L=10, B=2):
+    """[B][heads][L][d] whose values are two apart and whose positions are outermost."""
+    return torch.empty((B, L, heads, 2 * d), device="meta")[..., ::2].transpose(1, 2)
+
+
+def test_traced_strides_where_the_last_axis_is_not_contiguous():
+    """The operators copy such a tensor first, and order their outputs like the copy."""
+    B, H, Hkv, L, D, Dv = 2, 4, 2, 10, 16, 24
+    q, k, v, ld = strided(H, D), strided(Hkv, D), strided(Hkv, Dv), meta(H)
+    y, s = ops.linear_attention(q, k, v, ld)
+    assert y.stride() == (H * L * Dv, L * Dv, Dv, 1) and s.is_contiguous()
+    grads = torch.ops.sffft.linear_attention_backward(q, k, v, ld, None, None, 1.0, meta(B, H, L, Dv), None)
+    assert [g.stride() for g in grads] == [(H * L * D, L * D, D, 1), (Hkv * L * D, L * D, D, 1), (Hkv * L * Dv, L * Dv, Dv, 1)]
+    # and where it is contiguous, like the tensor itself
+    q = meta(B, L, H, D).transpose(1, 2)
+    assert ops.linear_attention(q, k, v, ld)[0].stride() == (H * L * Dv, Dv, H * Dv, 1)
+    grads = torch.ops.sffft.linear_attention_backward(q, k, v, ld, None, None, 1.0, meta(B, H, L, Dv), None)
+    assert grads[0].stride() == (H * L * D, D, H * D, 1)
