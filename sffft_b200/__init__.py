@@ -596,7 +596,7 @@ def check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths, fi
         raise ValueError("q, k and v must have one type")
     if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
         raise ValueError(f"log_decay must be a float32 [{H}] tensor")
-    if log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay is a constant: it has no gradient (pass log_decay.detach())")
     if not math.isfinite(scale) or scale == 0:
         raise ValueError("scale must be finite and not 0")

@@ -427,7 +427,8 @@ struct Attention : torch::autograd::Function<Attention> {
 
 std::tuple<Tensor, Tensor> attention_grad(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                           const optional<Tensor>& s0, const optional<Tensor>& lengths, double scale) {
-  need(!log_decay.requires_grad(), "log_decay is a constant: it has no gradient (pass log_decay.detach())");
+  need(!at::GradMode::is_enabled() || !log_decay.requires_grad(),
+       "log_decay is a constant: it has no gradient (pass log_decay.detach())");
   need_no_tangent("linear_attention", q, k, v, log_decay, s0);
   if (wants({&s0}) || (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))) {
     auto out = Attention::apply(q, k, v, log_decay, s0, lengths, scale);

@@ -58,3 +58,20 @@ def test_traced_strides_where_the_last_axis_is_not_contiguous():
     assert ops.linear_attention(q, k, v, ld)[0].stride() == (H * L * Dv, Dv, H * Dv, 1)
     grads = torch.ops.sffft.linear_attention_backward(q, k, v, ld, None, None, 1.0, meta(B, H, L, Dv), None)
     assert grads[0].stride() == (H * L * D, D, H * D, 1)
+
+
+def test_a_decay_that_is_a_parameter_serves_without_gradients():
+    """Where no gradient is asked for nothing is lost by it: prompts take it as single tokens do."""
+    ld = meta(4).requires_grad_()
+    with torch.no_grad():
+        y, _ = ops.linear_attention(**dict(ATTENTION, log_decay=ld))
+        assert y.shape == (2, 4, 10, 24)
+        ops.linear_attention_step(**dict(STEP, log_decay=ld))
+        sf.check_linear_attention(**dict(ATTENTION, log_decay=ld), scale=1.0, lengths=None)
+    with torch.inference_mode():
+        ops.linear_attention(**dict(ATTENTION, log_decay=ld))
+    for op, args in ((ops.linear_attention, ATTENTION), (ops.linear_attention_step, STEP)):
+        with pytest.raises(ValueError):
+            op(**dict(args, log_decay=ld))
+    with pytest.raises(ValueError):
+        sf.check_linear_attention(**dict(ATTENTION, log_decay=ld), scale=1.0, lengths=None)
