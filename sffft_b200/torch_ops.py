@@ -160,34 +160,54 @@ def _(X: Tensor, config: str = "") -> Tensor:
 # Linear attention and the norms around a block: operators of csrc/torch_binding.cpp (kernels and gradients); here the
 # functions that users call, and shapes for tracing
 # ---------------------------------------------------------------------------------------------------------------
+_missing = None   # why the operators are not there: said when one is called, since the ones above do without
 if not os.path.exists(sf.TORCH_LIB_PATH):
-    raise RuntimeError(f"native library missing: {sf.TORCH_LIB_PATH} (run `make -C sffft_b200`)")
-sf.lib()   # which it is linked with
-torch.ops.load_library(sf.TORCH_LIB_PATH)
-_attention = torch.ops.sffft.linear_attention.default
-_attention_step = torch.ops.sffft.linear_attention_step.default
-_block_norm = torch.ops.sffft.block_norm.default
+    _missing = f"native library missing: {sf.TORCH_LIB_PATH} (run `make -C sffft_b200`)"
+else:
+    try:
+        sf.lib()   # which it is linked with
+        torch.ops.load_library(sf.TORCH_LIB_PATH)
+    except (OSError, RuntimeError) as e:
+        _missing = f"native library not loadable: {sf.TORCH_LIB_PATH} ({e}; run `make -C sffft_b200` with this PyTorch)"
 
 
-@torch.library.register_fake("sffft::linear_attention")
+def _operator(name):
+    if _missing is None:
+        return getattr(torch.ops.sffft, name).default
+
+    def call(*_):
+        raise RuntimeError(_missing)
+    return call
+
+
+def _fake(name):
+    return torch.library.register_fake(f"sffft::{name}") if _missing is None else lambda f: f
+
+
+_attention = _operator("linear_attention")
+_attention_step = _operator("linear_attention_step")
+_block_norm = _operator("block_norm")
+
+
+@_fake("linear_attention")
 def _(q, k, v, log_decay, initial_state, lengths, scale):
     sf.check_linear_attention(q, k, v, log_decay, scale, initial_state, lengths)
     B, H, L, D = q.shape
     return sf._heads_like(sf._unit(q), B, H, L, v.shape[3], q.dtype), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
 
 
-@torch.library.register_fake("sffft::linear_attention_backward")
+@_fake("linear_attention_backward")
 def _(q, k, v, log_decay, initial_state, lengths, scale, dy, dfinal_state):
     out = [sf._heads_like(sf._unit(t), *t.shape, q.dtype) for t in (q, k, v)]   # as the operator orders them: behind its copies
     return out if initial_state is None else out + [torch.empty_like(initial_state, memory_format=torch.contiguous_format)]
 
 
-@torch.library.register_fake("sffft::linear_attention_step")
+@_fake("linear_attention_step")
 def _(q, k, v, log_decay, state, slots, scale):
     return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
 
 
-@torch.library.register_fake("sffft::block_norm")
+@_fake("block_norm")
 def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim, stats=False):
     C, _, _ = sf.check_block_norm(x, y, gate, post_weight, weight, scale, eps, groups, act, dim)
     lead = y if y is not None else x
@@ -204,7 +224,7 @@ def _(x, y, gate, post_weight, weight, scale, eps, groups, act, dim, stats=False
     return out
 
 
-@torch.library.register_fake("sffft::block_norm_backward")
+@_fake("block_norm_backward")
 def _(dh, dn, x, y, gate, post_weight, weight, rstd_post, rstd, scale, eps, groups, act, dim):
     return [t.new_empty(t.shape) for t in (x, y, gate, post_weight, weight) if t is not None]
 

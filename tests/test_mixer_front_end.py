@@ -1,11 +1,17 @@
 """Linear attention and block_norm on the CPU: what the PyTorch operators, the Python functions and the C ABI do with a call
 before anything runs on a device."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import sffft_b200 as sf
 import sffft_b200.torch_ops as ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def meta(*s, dtype=torch.float32):
@@ -75,3 +81,30 @@ def test_a_decay_that_is_a_parameter_serves_without_gradients():
             op(**dict(args, log_decay=ld))
     with pytest.raises(ValueError):
         sf.check_linear_attention(**dict(ATTENTION, log_decay=ld), scale=1.0, lengths=None)
+
+
+@pytest.mark.parametrize("what", ["missing", "not loadable"])
+def test_the_convolution_does_not_need_the_mixers_library(what, tmp_path):
+    """A build of lib/libsffft.so alone serves the convolution and the transforms; linear attention and block_norm say what is
+    missing when they are called."""
+    path = tmp_path / "libsffft_torch.so"
+    if what == "not loadable":
+        path.write_bytes(b"no library")
+    code = f"""if 1:
+        import torch, sffft_b200 as sf
+        sf.TORCH_LIB_PATH = {str(path)!r}
+        import sffft_b200.torch_ops as ops
+        u, k = torch.empty((2, 3, 256), device="meta"), torch.empty((3, 256), device="meta")
+        assert ops.causal_conv(u, k).shape == u.shape and ops.rfft(u).shape == (2, 3, 129)
+        q = torch.empty((1, 2, 5, 16), device="meta")
+        for call in (lambda: ops.linear_attention(q, q, q, torch.empty(2, device="meta")), lambda: ops.block_norm(q, weight=q[0, 0, 0]),
+                     lambda: ops.linear_attention_step(q[:, :, 0], q[:, :, 0], q[:, :, 0], torch.empty(2, device="meta"), q)):
+            try:
+                call()
+            except RuntimeError as e:
+                assert "libsffft_torch.so" in str(e), e
+            else:
+                raise AssertionError("no error")
+        """
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
