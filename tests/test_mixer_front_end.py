@@ -108,3 +108,21 @@ def test_the_convolution_does_not_need_the_mixers_library(what, tmp_path):
         """
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_the_build_does_without_pytorch(tmp_path):
+    """A dry run with a Python that has none builds all but the PyTorch operators, and says so; with this one it builds them."""
+    bare = tmp_path / "python"
+    bare.write_text(f'#!/bin/sh\nexec {sys.executable} -I -S "$@"\n')
+    bare.chmod(0o755)
+
+    def dry(python):   # (whether the note was printed, what would be built)
+        r = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "sffft_b200"), f"PYTHON={python}", "all"],
+                           capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stderr
+        return any(line.startswith("libsffft_torch.so") for line in r.stdout.splitlines()), r.stdout
+
+    said, out = dry(bare)
+    assert said and "torch_binding.cpp" not in out and "csrc/api.cu" in out and "csrc/cli.cpp" in out
+    said, out = dry(sys.executable)
+    assert not said and "torch_binding.cpp" in out
