@@ -266,9 +266,10 @@ int sffft_linear_attention_backward(const sffft_linear_attention_t* p, const sff
 int sffft_linear_attention_check(int device);
 
 /* One token for each of B rows: S <- lambda S + k v^T in place, y = scale * S^T q.  The states lie in a pool of slots
- * of [H][D][Dv] fp32, state_stride elements apart; row b uses slot slots[b] (int32, device), or slot b where slots is
- * NULL.  A row whose slot is not in [0, pool) is padding: it gets y = 0 and no state changes.  The same holds for a row
- * that names a slot which an earlier row of the call names.  Strides are {row, head}. */
+ * of [H][D][Dv] fp32, state_stride elements apart (at least H D Dv where there is more than one); row b uses slot
+ * slots[b] (int32, device), or slot b where slots is NULL.  A row whose slot is not in [0, pool) is padding: it gets y = 0
+ * and no state changes.  The same holds for a row that names a slot which an earlier row of the call names.  Strides are
+ * {row, head}. */
 typedef struct {
   int B, H, Hkv, D, Dv, pool;
   int io, device;

@@ -463,6 +463,7 @@ int sffft_linear_attention_step(const sffft_linear_attention_step_t* p, const vo
       (p->io != SFFFT_IO_FP32 && p->io != SFFFT_IO_BF16) || p->device < 0 || !std::isfinite(p->scale))
     return SFFFT_ERR_INVALID_ARGUMENT;
   if (!slots && p->pool < p->B) return SFFFT_ERR_INVALID_ARGUMENT;
+  if (p->pool > 1 && p->state_stride < (long long)p->H * p->D * p->Dv) return SFFFT_ERR_INVALID_ARGUMENT;   // slots that overlap
   if ((long long)p->B * p->H > INT_MAX || (long long)p->D * p->Dv > INT_MAX || p->Dv > 32 * 65535) return SFFFT_ERR_UNSUPPORTED;
   if (p->B == 0) return SFFFT_OK;
   if (!q || !k || !v || !log_decay || (!state && p->pool > 0) || !y) return SFFFT_ERR_INVALID_ARGUMENT;

@@ -1,5 +1,6 @@
 """Linear attention and block_norm on the CPU: what the PyTorch operators, the Python functions and the C ABI do with a call
 before anything runs on a device."""
+import ctypes
 import os
 import subprocess
 import sys
@@ -126,3 +127,20 @@ def test_the_build_does_without_pytorch(tmp_path):
     assert said and "torch_binding.cpp" not in out and "csrc/api.cu" in out and "csrc/cli.cpp" in out
     said, out = dry(sys.executable)
     assert not said and "torch_binding.cpp" in out
+
+
+def test_c_abi_refuses_slots_that_overlap():
+    """Rows of one call would update the same memory."""
+    call = lambda d: sf.lib().sffft_linear_attention_step(ctypes.byref(d), 16, 16, 16, 16, 16, None, 16, None)  # noqa: E731
+    for stride in (0, 2 * 8 * 8 - 1, -2 * 8 * 8):
+        d = sf.LinearAttentionStepDesc(2, 2, 2, 8, 8, 2, 0, 0, 1.0)
+        d.state_stride = stride
+        assert call(d) == sf.ERR_INVALID_ARGUMENT, stride
+    one = sf.LinearAttentionStepDesc(0, 2, 2, 8, 8, 1, 0, 0, 1.0)     # a pool of one slot has no stride
+    assert call(one) == sf.OK
+    apart = sf.LinearAttentionStepDesc(2, 2, 2, 8, 8, 2, 1, 0, 1.0)
+    apart.state_stride = 2 * 8 * 8
+    for i in range(7):     # and, with slots apart, an address between elements
+        a = [16] * 5 + [None, 16]
+        a[i] = 17
+        assert sf.lib().sffft_linear_attention_step(ctypes.byref(apart), *a, None) == sf.ERR_INVALID_ARGUMENT, i
