@@ -106,26 +106,31 @@ __device__ __forceinline__ void ldw(const void* w, int bf16, int c, float (&v)[V
   else ldv<VEC>((const float*)w + c, v);
 }
 
-// By the approximate exp and division, a few units in the last place (more for |x| in the tens, where the result is next to
-// 0 or 1): the exact ones were a third of the instructions of a kernel that their issue held back, 65 -> 55 us for
-// 32768 rows of 768.
-__device__ __forceinline__ float sigmoidf(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// The approximate division is off by at most 2 units in the last place; the exact one, with the exact exp, was a third of the
+// instructions of a kernel that their issue held back, 65 -> 55 us for 32768 rows of 768.  A gate in fp32 has the
+// exact exp (2 units).  A gate in bf16 has the approximate one, whose error grows with |x| to 32 units at 87, 2^-18: the
+// gate, rounded to 2^-8 of itself, moves the result by |x| times that (61 us for the same rows; 65 with the exact one).
+template <class T>
+__device__ __forceinline__ float sigmoidf(float x) {
+  if constexpr (sizeof(T) == 4) return __fdividef(1.f, 1.f + expf(-x));
+  else return __fdividef(1.f, 1.f + __expf(-x));
+}
 
-// act(gate) of a thread's values, and its derivative (one branch for all of them)
-template <int VEC>
+// act(gate) of a thread's values, gate of type T, and its derivative (one branch for all of them)
+template <class T, int VEC>
 __device__ __forceinline__ void act_fwd(int act, const float (&g)[VEC], float (&f)[VEC]) {
   if (act == SFFFT_ACT_NONE) {
 #pragma unroll
     for (int e = 0; e < VEC; e++) f[e] = g[e];
   } else if (act == SFFFT_ACT_SILU) {
 #pragma unroll
-    for (int e = 0; e < VEC; e++) f[e] = g[e] * sigmoidf(g[e]);
+    for (int e = 0; e < VEC; e++) f[e] = g[e] * sigmoidf<T>(g[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < VEC; e++) f[e] = sigmoidf(g[e]);
+    for (int e = 0; e < VEC; e++) f[e] = sigmoidf<T>(g[e]);
   }
 }
-template <int VEC>
+template <class T, int VEC>
 __device__ __forceinline__ void act_both(int act, const float (&g)[VEC], float (&f)[VEC], float (&df)[VEC]) {
   if (act == SFFFT_ACT_NONE) {
 #pragma unroll
@@ -133,14 +138,14 @@ __device__ __forceinline__ void act_both(int act, const float (&g)[VEC], float (
   } else if (act == SFFFT_ACT_SILU) {
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
-      const float s = sigmoidf(g[e]);
+      const float s = sigmoidf<T>(g[e]);
       f[e] = g[e] * s;
       df[e] = fmaf(f[e], 1.f - s, s);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
-      f[e] = sigmoidf(g[e]);
+      f[e] = sigmoidf<T>(g[e]);
       df[e] = fmaf(-f[e], f[e], f[e]);
     }
   }
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 32 * kRowsPerBlock) norm_rows_k
       if (p.gate_kind) {
         float g[VEC], f[VEC];
         rg[j].get(g);
-        act_fwd<VEC>(p.act, g, f);
+        act_fwd<TY, VEC>(p.act, g, f);
 #pragma unroll
         for (int e = 0; e < VEC; e++) v[j][e] *= f[e];
       }
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bw
       float f[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; e++) f[e] = 1.f;
-      if (p.gate_kind) act_fwd<VEC>(p.act, g, f);
+      if (p.gate_kind) act_fwd<TY, VEC>(p.act, g, f);
       if (!p.pw) {   // without y u is zero
 #pragma unroll
         for (int e = 0; e < VEC; e++) s[j][e] = p.scale * f[e];
@@ -484,7 +489,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kRowsPerBlock) norm_rows_bw
         float g[VEC], f[VEC], df[VEC];
         if (p.gate_kind == GATE_FULL) now.g[j].get(g);
         else ldv<VEC>((const TY*)p.gate + i * VEC, g);
-        act_both<VEC>(p.act, g, f, df);
+        act_both<TY, VEC>(p.act, g, f, df);
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
           const float du = p.scale * d[j][e] * u[j][e];
@@ -716,7 +721,7 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
         else
 #pragma unroll
           for (int e = 0; e < VEC; e++) gv[e] = r.gc;
-        act_fwd<VEC>(p.act, gv, f);
+        act_fwd<TY, VEC>(p.act, gv, f);
 #pragma unroll
         for (int e = 0; e < VEC; e++) h[e] *= f[e];
       }
@@ -844,8 +849,8 @@ __global__ void __launch_bounds__(kFirstThreads, 2) norm_first_bwd_kernel(const 
         else
 #pragma unroll
           for (int e = 0; e < VEC; e++) gv[e] = r.gc;
-        if (with_df) act_both<VEC>(p.act, gv, v.f, v.df);
-        else act_fwd<VEC>(p.act, gv, v.f);
+        if (with_df) act_both<TY, VEC>(p.act, gv, v.f, v.df);
+        else act_fwd<TY, VEC>(p.act, gv, v.f);
       }
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
