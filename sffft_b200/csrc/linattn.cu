@@ -173,41 +173,73 @@ cudaError_t device_facts(int device, DeviceFacts* f) {
   return ce;
 }
 
-// Segments for the general kernel: enough blocks to give every SM two, each of at least two chunks (the launches for the
-// segments' own states cost about that).
-void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
-  const int chunk = la_general_chunk(D);
-  const long long base = (long long)B * H * ((Dv + 63) / 64) * ntask;
-  const long long chunks = ((long long)L + chunk - 1) / chunk;
-  long long g = (2ll * sms + base - 1) / base;
-  if (g > chunks / 2) g = chunks / 2;
-  if (g > kMaxSegments) g = kMaxSegments;
-  if (g < 1) g = 1;
-  const long long per = (chunks + g - 1) / g;
-  *seg = (int)(per < 1 ? chunk : per * chunk);
-  *G = chunks ? (int)((chunks + per - 1) / per) : 1;
+// How many segments the rows are cut into.  Few heads leave SMs idle, which segments fill; they cost a second reading of k and
+// v and two more launches, so rows of many heads stay whole.  The choice is the least of, in us,
+//   whole:       start + waves * chunks * one           cut: cut + waves * (start_cut + chunks of a segment * both)
+// where `both` takes the segment's own state, too, and a wave is what the SMs hold at once.  The constants fit 572
+// measured times (head sizes 64, 128 and 256, forward and backward, 3 to 400 heads of 4 to 128 chunks, 1 to 32 segments): the choice is
+// within 12 % of the best of them, 0.7 % on average.  E.g. 96 heads x 4096 x 128 in bf16: whole 168 us, two segments 224, twelve 306;
+// 16 heads: whole 161, six segments 65.
+struct ChunkTimes {
+  double one, both, start, start_cut, cut;
+  bool pairs;   // two blocks on an SM, which together take 1.72 times as long as one
+};
+
+struct LaunchPlan {
+  long long blocks;   // in a segment
+  ChunkTimes t;
+};
+
+double waves(long long blocks, bool pairs, int sms) {
+  if (!pairs) return (double)((blocks + sms - 1) / sms);
+  const long long full = blocks / (2 * sms), rest = blocks % (2 * sms);
+  return (double)full * 1.72 + (rest == 0 ? 0.0 : rest <= sms ? 1.0 : 1.72);
 }
 
-// Segments for the tensor-core kernel, one CTA on an SM.  A CTA's time is that of its chunks one after the other, so cutting
-// pays until the CTAs fill the SMs.  It costs two more launches, and a reading of k and v.  Measured (us a chunk, with one
-// CTA on each SM): 3.1 at head size 128 and 2.0 at 64; of a segment's own state 2.3 and 1.5; 10 for the launches.  At head
-// size 128 a chunk whose state is an output takes 5.0 (its third part of X waits for the product of the others), which
-// with G > 1 is the last segment's lot alone.
-void plan_tc(int B, int H, int L, int D, int Dv, int ntask, bool out, int sms, int* G, int* seg) {
-  const long long units = (long long)B * H * ntask * la_tc_slices(D, Dv);
-  const int chunks = (L + kLaTcChunk - 1) / kLaTcChunk;
-  const double one = D > 64 ? 3.1 : 2.0, local = D > 64 ? 2.3 : 1.5;
+void plan_segments(const LaunchPlan* l, int n, long long chunks, int sms, int* G, long long* per) {
   double best = 0;
-  *G = 1;
+  *G = 1, *per = chunks;
   for (int g = 1; g <= kMaxSegments && g <= chunks; g++) {
-    const long long waves = (units * g + sms - 1) / sms;
-    const int per = (chunks + g - 1) / g;
-    const double cost = (double)waves * per * (g > 1 ? one + local : D > 64 && out ? 5.0 : one) + (g > 1 ? 10.0 : 0.0);
-    if (g == 1 || cost < best) best = cost, *G = g;
+    const long long m = (chunks + g - 1) / g;
+    if ((chunks + m - 1) / m != g) continue;   // as many chunks a segment as with fewer of them
+    double cost = 0;
+    for (int i = 0; i < n; i++) {
+      const ChunkTimes& t = l[i].t;
+      const double w = waves(l[i].blocks * g, t.pairs, sms);
+      cost += g == 1 ? t.start + w * (double)m * t.one : t.cut + w * (t.start_cut + (double)m * t.both);
+    }
+    if (g == 1 || cost < best) best = cost, *G = g, *per = m;
   }
-  const int per = chunks ? (chunks + *G - 1) / *G : 1;
-  *seg = per * kLaTcChunk;
-  *G = chunks ? (chunks + per - 1) / per : 1;
+}
+
+void plan_general(int B, int H, int L, int D, int Dv, int ntask, int sms, int* G, int* seg) {
+  const int chunk = la_general_chunk(D);
+  const LaunchPlan l = {(long long)B * H * ((Dv + 63) / 64) * ntask, D <= 64    ? ChunkTimes{12.6, 16, 11, 4, 18, true}
+                                                                     : D <= 128 ? ChunkTimes{19.8, 26, 12, 8, 20, false}
+                                                                                : ChunkTimes{23.3, 35, 16, 8, 30, false}};
+  long long per;
+  plan_segments(&l, 1, ((long long)L + chunk - 1) / chunk, sms, G, &per);
+  *seg = (int)(per < 1 ? chunk : per * chunk);
+}
+
+// One launch for each tile shape.  `out`: the state is an output, whose third part of X waits for the product of the others
+// at head sizes above 64; with segments that is the last one's lot alone.
+void plan_tc(int B, int H, int L, int D, int Dv, bool backward, int sms, int* G, int* seg) {
+  auto launch = [&](int d, int dv, int tasks, bool out) {
+    const bool wide = la_tc_tile(d, dv) == 128;
+    return LaunchPlan{(long long)B * H * tasks * la_tc_slices(d, dv),
+                      d <= 64 ? ChunkTimes{2.1, 3.5, 11, 10, 16, false}
+                      : wide  ? (out ? ChunkTimes{4.6, 6.4, 14, 17, 20, false} : ChunkTimes{3.4, 5.4, 11, 16, 16, false})
+                              : (out ? ChunkTimes{3.6, 5.4, 13, 14, 16, false} : ChunkTimes{2.9, 4.6, 11, 14, 16, false})};
+  };
+  LaunchPlan l[2];
+  int n = 1;
+  if (!backward) l[0] = launch(D, Dv, 1, true);
+  else if ((D > 64) == (Dv > 64)) l[0] = launch(D > Dv ? D : Dv, D > Dv ? D : Dv, 3, false);   // of one shape
+  else l[0] = launch(Dv, D, 2, false), l[1] = launch(D, Dv, 1, false), n = 2;
+  long long per;
+  plan_segments(l, n, ((long long)L + kLaTcChunk - 1) / kLaTcChunk, sms, G, &per);
+  *seg = (int)(per < 1 ? kLaTcChunk : per * kLaTcChunk);
 }
 
 size_t io_size(int io) { return io == SFFFT_IO_BF16 ? 2 : 4; }
@@ -245,7 +277,7 @@ Sizes sizes(const sffft_linear_attention_t* p, int backward, int G) {
 
 void plan(const sffft_linear_attention_t* p, int backward, bool tc, int sms, int* G, int* seg) {
   const int D = backward ? (p->D > p->Dv ? p->D : p->Dv) : p->D, Dv = backward ? D : p->Dv;
-  if (tc) plan_tc(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, !backward, sms, G, seg);
+  if (tc) plan_tc(p->B, p->H, p->L, p->D, p->Dv, backward != 0, sms, G, seg);
   else plan_general(p->B, p->H, p->L, D, Dv, backward ? 3 : 1, sms, G, seg);
 }
 

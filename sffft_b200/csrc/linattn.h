@@ -89,6 +89,7 @@ cudaError_t la_tc_word(int device, int** word);
 int la_tc_reported(int device);
 cudaError_t la_tc_status(int device, int* status);
 constexpr int kLaTcChunk = 128;
+int la_tc_tile(int D, int Dv);     // columns of v in a CTA
 int la_tc_slices(int D, int Dv);   // CTAs over the columns of v
 
 }  // namespace sffft

@@ -974,9 +974,6 @@ bool make_map(CUtensorMap* m, const void* p, const long long (&s)[3], int B, int
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Columns of v in a CTA.
-int tile_v(int D, int Dv) { return D > 64 && Dv > 64 ? 128 : 64; }
-
 template <int DQ, int DV>
 cudaError_t launch_shape(LaTcParams& prm, cudaStream_t st) {
   const dim3 grid((unsigned)(prm.p.B * prm.p.H * prm.p.G * prm.p.ntask * prm.slices));
@@ -1008,7 +1005,9 @@ bool la_tc_takes(const LaParams& p) {
   return true;
 }
 
-int la_tc_slices(int D, int Dv) { return (Dv + tile_v(D, Dv) - 1) / tile_v(D, Dv); }
+int la_tc_tile(int D, int Dv) { return D > 64 && Dv > 64 ? 128 : 64; }
+
+int la_tc_slices(int D, int Dv) { return (Dv + la_tc_tile(D, Dv) - 1) / la_tc_tile(D, Dv); }
 
 cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
   // tasks of one tile shape go into one launch
@@ -1021,10 +1020,10 @@ cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
     prm.blocks = p.seg / kTok;
     prm.slices = 1;
     const bool q2 = p.task[i].D > 64;
-    const int dv = tile_v(p.task[i].D, p.task[i].Dv);
+    const int dv = la_tc_tile(p.task[i].D, p.task[i].Dv);
     for (int j = i; j < p.ntask; j++) {
       const LaTask& t = p.task[j];
-      if (done[j] || (t.D > 64) != q2 || tile_v(t.D, t.Dv) != dv) continue;
+      if (done[j] || (t.D > 64) != q2 || la_tc_tile(t.D, t.Dv) != dv) continue;
       done[j] = true;
       const int k = prm.p.ntask++;
       prm.p.task[k] = t;
