@@ -657,7 +657,10 @@ __global__ void __launch_bounds__(kFirstThreads) norm_first_kernel(const __grid_
   const TY *y = (const TY*)p.y + ft.base, *gate = (const TY*)p.gate;
   const TX* x = (const TX*)p.x + ft.base;
   const long long L = p.inner;
-  constexpr int kAhead = VEC == 1 || sizeof(TX) + sizeof(TY) <= 6 ? 4 : 2;   // with fp32 alone, [8][768][1024]: 33 us; 4: 37
+  // Channels ahead, two against four (us): with fp32 alone [8][768][1024] 41, 45, [8][768][4096] 121, 135, [8][256][8192] 88,
+  // 141, but [4][1024][2048] 53, 49 and [2][2048][2048] 72, 66; in bf16 [8][768][4096] 108, 105, [8][256][8192] 76, 74,
+  // [2][2048][4096] 82, 74.
+  constexpr int kAhead = VEC == 1 || sizeof(TX) + sizeof(TY) <= 6 ? 4 : 2;
   if (p.pw) {
     float* const out[1] = {r1};
     if constexpr (KEEP) {   // y's tile first, many loads at a time: the sums over groups would wait for each

@@ -65,9 +65,16 @@ struct __align__(64) LaTcParams {
 };
 
 // The row that the CTAs numbered b take.  Where they come to between one and two for each SM, a long row that starts last
-// leaves the other SMs idle behind it: 8 rows of 600 to 1999 tokens x 12 heads of 64 x 128 took 58 to 70 us in their own
-// order and 57 to 65 longest first.  With more CTAs, or a row cut into segments, the order of lengths won nothing (16 x 6 x
-// 1999 x 128: 233 and 245 us).  Called by whole warps, each for itself: a lane ranks one row, ties by number.
+// leaves the other SMs idle behind it.  Own order against longest first, rows of random lengths, and two long ones among rows
+// of a quarter (us):
+//   8 rows x 12 heads x 1999 x 64 x 128, 192 CTAs     71, 70     68, 53
+//   16 x 16 x 2000 x 64, 256                          84, 74     74, 58
+//   30 x 8 x 4000 x 64, 240                          141, 131   123, 91
+//   24 x 12 x 1024 x 128 x 64, 288                    78, 68     66, 64
+//   10 x 15 x 3000 x 128, 150                        187, 176   205, 164
+//   16 x 32 x 2000 x 64, 512                         137, 141   119, 105
+// and no shape of up to two CTAs an SM was slower.  Beyond, either order may win.  Called by whole warps, each for itself: a
+// lane ranks one row, ties by number.
 constexpr int kMaxSorted = 32;
 __device__ __forceinline__ int row_of(const LaTcParams& prm, int b) {
   if (!prm.by_length) return b;
