@@ -236,12 +236,13 @@ int sffft_multi_pipe_destroy(sffft_multi_t multi);
  * Calls run on `device` in stream order and can be captured in graphs; the caller's current device is left as it was.
  * Results do not depend on scheduling: no atomics.
  *
- * Accuracy.  Outputs are rounded once to their type, and states are sums in fp32, whichever kernel runs.  bf16 with D up to
- * 128, D and Dv multiples of 8 and rows on 16 bytes (strides multiples of 8) runs on the tensor cores, where one factor of
- * each of y's products (the weighted q . k, and the state) is rounded to bf16 first: y, dq, dk and dv are off by up to
- * 2^-8 of their terms' magnitudes beside their own rounding (relative L2 2.35e-3, the rounding alone 1.66e-3).  Other sizes,
- * addresses and strides, and fp32, run on the CUDA cores in fp32 throughout; the same bf16 values in a view that lies
- * between have the smaller error.  To have it everywhere, pass fp32 tensors. */
+ * Accuracy.  Outputs are rounded once to their type, and states are sums in fp32, whichever kernel runs (on the tensor cores
+ * of terms held to 2^-24, or to 2^-16 where final_state is NULL and only y uses them).  bf16 with D up to 128, D and Dv
+ * multiples of 8 and rows on 16 bytes (strides multiples of 8) runs on the tensor cores, where one factor of each of y's
+ * products (the weighted q . k, and the state) is rounded to bf16 first: y, dq, dk and dv are off by up to 2^-8 of their
+ * terms' magnitudes beside their own rounding (relative L2 2.35e-3, the rounding alone 1.66e-3).  Other sizes, addresses
+ * and strides, and fp32, run on the CUDA cores in fp32 throughout; the same bf16 values in a view that lies between have
+ * the smaller error.  To have it everywhere, pass fp32 tensors. */
 typedef struct {
   int B, H, Hkv, L, D, Dv;
   int io;                 /* SFFFT_IO_* of q, k, v, y and their gradients */

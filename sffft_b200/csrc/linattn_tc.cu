@@ -1051,12 +1051,13 @@ cudaError_t launch_la_tc(const LaParams& p, cudaStream_t st) {
 
 // Status words of the devices, in page-locked host memory that every device can write.
 namespace {
-std::atomic<int*> g_words{nullptr};
+std::atomic<int*> g_words{nullptr}, g_device_word[kLaMaxDevices];   // and their addresses on the devices
 }
 
 cudaError_t la_tc_word(int device, int** word) {
   static std::mutex mutex;
   if (device < 0 || device >= kLaMaxDevices) return cudaErrorInvalidDevice;
+  if ((*word = g_device_word[device].load(std::memory_order_acquire))) return cudaSuccess;
   int* p = g_words.load(std::memory_order_acquire);
   if (!p) {
     std::lock_guard<std::mutex> lock(mutex);
@@ -1077,7 +1078,7 @@ cudaError_t la_tc_word(int device, int** word) {
   }
   void* on_device = nullptr;
   const cudaError_t ce = cudaHostGetDevicePointer(&on_device, p + device, 0);
-  *word = (int*)on_device;
+  if (ce == cudaSuccess) g_device_word[device].store(*word = (int*)on_device, std::memory_order_release);
   return ce;
 }
 
