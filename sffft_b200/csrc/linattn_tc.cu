@@ -33,8 +33,8 @@
 // registers at 128 (spills, 167 -> 194 us), the next launch's prologue overlapped with the last one's end (no gain).
 //
 // Every wait on an mbarrier is bounded: after LaParams::wait_ns the waiting role raises the CTA's flag, all roles leave, and
-// the device's status word says so, which lies in host memory so that a later call can look at it without waiting.  The named barriers (bar.sync) stand where every thread of theirs comes by, given up or
-// not: behind the state warpgroups' loop, and at the block's ends.
+// the device's status word says so, which lies in host memory so that a later call can look at it without waiting.  The
+// named barriers (bar.sync) stand where every thread of theirs comes by, given up or not: behind the state warpgroups' loop.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(Shape<DQ, DV, LOCAL>::threads, 1) la_tc_kernel
       for (int c = 0; any(c < nc); c++)
         if (!q_k(c) || !x_v(c) || !q_s(c) || !p_v(c) || (any(later) && !x_v_third(c))) break;
     }
-    if (*stop) {   // products in flight end before TMEM is given back
+    if (any(*stop != 0)) {   // products in flight end before TMEM is given back; the election needs the whole warp
       if (elect_one()) {
         mma_commit(bars + B_FIN);
         mbar_wait_bounded(bars + B_FIN, 0, kCopyLimit);
